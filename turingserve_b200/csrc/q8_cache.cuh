@@ -1,0 +1,45 @@
+// Keys and values held in 8 bits: e4m3 values in pages [pages, KVH, page, D] with one scale (float32) for each
+// (page, kv head): what a row stands for is its value times its page's scale.
+//
+// A scale is 2^e, e the least integer >= -50 with max |x| <= 448 * 2^e over the rows of the page.  Powers of two cost an
+// e4m3 value nothing (it has its own exponent), and a page whose scale has to grow for a new row only moves its rows'
+// exponents: no second rounding but below 2^-6 of the scale's unit, 2^-18 of the page's largest value.  A page with a
+// value that is not finite, or above 448 * 2^50, has the scale NaN: all that it holds reads as NaN until its first row is
+// written again.  The range of e, 101 steps, is what lets the attention kernels keep one reference for a score and a
+// value's scale together (attention_q8_decode.cu).
+#pragma once
+
+#include <cuda_fp16.h>
+#include <cuda_fp8.h>
+
+#include "common.cuh"
+
+namespace q8 {
+
+constexpr int MIN_EXP = -50, MAX_EXP = 50;
+constexpr unsigned NAN_BITS = 0x7fc00000u;
+
+// The scale of a page whose largest magnitude has these bits (of |x| as float32).
+__device__ __forceinline__ float scale_for(unsigned amax_bits) {
+  if (amax_bits > (((unsigned)(MAX_EXP + 8 + 127) << 23) | 0x600000u)) return __uint_as_float(NAN_BITS);   // 448 = 1.75 * 2^8
+  int e = (int)(amax_bits >> 23) - 127 - 8 + ((amax_bits & 0x7fffffu) > 0x600000u ? 1 : 0);
+  e = e < MIN_EXP ? MIN_EXP : e;
+  return __uint_as_float((unsigned)(e + 127) << 23);
+}
+
+// The larger of a page's scale and what new rows need; NaN stays.
+__device__ __forceinline__ float larger_scale(float held, float need) {
+  return (held != held || need != need) ? __uint_as_float(NAN_BITS) : fmaxf(held, need);
+}
+
+// 1 / s of a power of two s (exact); 0 for NaN, under which rows are stored as zeros.
+__device__ __forceinline__ float inverse_scale(float s) { return s != s ? 0.f : __uint_as_float(0x7f000000u - __float_as_uint(s)); }
+
+__device__ __forceinline__ unsigned char to_e4m3(float x) { return (unsigned char)__nv_cvt_float_to_fp8(x, __NV_SATFINITE, __NV_E4M3); }
+__device__ __forceinline__ float from_e4m3(unsigned char b) {
+  return __half2float(__half(__nv_cvt_fp8_to_halfraw((__nv_fp8_storage_t)b, __NV_E4M3)));
+}
+// x times 1 / s on its way to 8 bits; a page that reads as NaN stores zeros (x may be infinite: no product then).
+__device__ __forceinline__ unsigned char quantise(float x, float inv) { return inv == 0.f ? 0 : to_e4m3(x * inv); }
+
+}  // namespace q8

@@ -1,0 +1,97 @@
+// A step's maps out of its requests' lengths and the page tables that stay on the GPU.
+//
+// Request b has row r[b] of the tables (-1: a row that only pads the batch), start[b] tokens in the cache and brings q[b]:
+//   q_start = 0, q[0], q[0] + q[1], ...      seq_lens[b] = start[b] + q[b]  (0 for padding)
+//   token i of request b:  token_request = b, position p = start[b] + i,
+//                          slot[g] = tables[g, r, p / page] * page + p % page  (-1 for padding)
+//   block_tables[g, b, i] = tables[g, r, i] for i < ceil(seq_lens[b] / page), else 0, the page that nobody owns
+// after `updates` (group, row, index, page) have gone into the tables; of updates of the same place the last one holds.
+//
+// One block a request, which sums the lengths before its own, puts its row's updates in place and writes its tokens and its
+// table rows; one more block for the updates of rows that are not in the step.  One launch whatever the step: 8 requests of 2,048
+// tokens are bound by its latency; 129 requests with tables of 2,048 entries move 3 MB.  The kernel does not let kernels behind
+// it start early: they may read the maps before they wait.
+#include "common.cuh"
+
+namespace {
+
+constexpr int THREADS = 256;
+
+struct MapArgs {
+  const int* requests;                 // [3][B]: table row, tokens before, tokens brought
+  const int4* updates;                 // [U]
+  int* tables;                         // [G][R][P]
+  int *q_start, *seq_lens, *token_request, *positions, *slots, *block_tables;
+  int B, T, U, G, R, P, W, page;
+};
+
+__global__ void __launch_bounds__(THREADS) step_maps_kernel(const MapArgs a) {
+  pdl_wait();
+  const int b = blockIdx.x, tid = threadIdx.x;
+  const bool extra = b == a.B;
+  __shared__ int sums[THREADS / 32];
+  const int upto = extra ? a.B : b;
+  int mine = 0;
+  for (int i = tid; i < upto; i += THREADS) mine += max(0, a.requests[2 * a.B + i]);
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) mine += __shfl_xor_sync(0xffffffffu, mine, o);
+  if ((tid & 31) == 0) sums[tid >> 5] = mine;
+  const int row = extra ? -1 : a.requests[b], start = extra ? 0 : a.requests[a.B + b], n = extra ? 0 : max(0, a.requests[2 * a.B + b]);
+  const bool real = row >= 0 && row < a.R;
+  for (int u = tid; u < a.U; u += THREADS) {
+    const int4 up = a.updates[u];
+    if ((!extra && up.y != row) || up.x < 0 || up.x >= a.G || up.y < 0 || up.y >= a.R || up.z < 0 || up.z >= a.P) continue;
+    bool holds = true;
+    for (int w = u + 1; w < a.U && holds; ++w) {
+      const int4 later = a.updates[w];
+      holds = later.x != up.x || later.y != up.y || later.z != up.z;
+    }
+    if (holds) a.tables[((size_t)up.x * a.R + up.y) * a.P + up.z] = up.w;
+  }
+  __syncthreads();
+  int first = 0;
+#pragma unroll
+  for (int i = 0; i < THREADS / 32; ++i) first += sums[i];
+  if (extra) {                                                     // tokens that no request brings: none, where the lengths add up
+    if (tid == 0) a.q_start[0] = 0;
+    for (int t = first + tid; t < a.T; t += THREADS) {
+      a.token_request[t] = 0;
+      a.positions[t] = 0;
+      for (int g = 0; g < a.G; ++g) a.slots[(size_t)g * a.T + t] = -1;
+    }
+    return;
+  }
+  const int len = real ? start + n : 0, live = len > 0 ? (len + a.page - 1) / a.page : 0;
+  if (tid == 0) {
+    a.q_start[b + 1] = first + n;
+    a.seq_lens[b] = len;
+  }
+  for (int g = 0; g < a.G; ++g) {
+    const int* tab = a.tables + ((size_t)g * a.R + (real ? row : 0)) * a.P;
+    int* bt = a.block_tables + ((size_t)g * a.B + b) * a.W;
+    for (int i = tid; i < a.W; i += THREADS) bt[i] = (i < live && i < a.P) ? tab[i] : 0;
+    for (int i = tid; i < n && first + i < a.T; i += THREADS) {
+      const int p = start + i, lp = p / a.page;
+      a.slots[(size_t)g * a.T + first + i] = (real && p >= 0 && lp < a.P) ? tab[lp] * a.page + p % a.page : -1;
+    }
+  }
+  for (int i = tid; i < n && first + i < a.T; i += THREADS) {
+    a.token_request[first + i] = b;
+    a.positions[first + i] = start + i;
+  }
+}
+
+}  // namespace
+
+TS_API int ts_step_maps(const int* requests, const int* updates, int* tables, int* q_start, int* seq_lens, int* token_request,
+                        int* positions, int* slots, int* block_tables, int B, int T, int U, int G, int R, int P, int W, int page,
+                        void* stream) {
+  if (B <= 0) return 0;
+  if (T < 0 || U < 0 || G < 0 || R <= 0 || P <= 0 || W < 0 || page <= 0)
+    TS_REFUSE(TS_ERR_SHAPE, "ts_step_maps: T=%d U=%d G=%d R=%d P=%d W=%d page=%d", T, U, G, R, P, W, page);
+  if (((uintptr_t)updates & 15) != 0) TS_REFUSE(TS_ERR_ALIGN, "ts_step_maps: updates must be 16-byte aligned");
+  MapArgs a = {requests, (const int4*)updates, tables, q_start, seq_lens, token_request, positions, slots, block_tables,
+               B, T, U, G, R, P, W, page};
+  ts_launch(step_maps_kernel, dim3(B + 1), dim3(THREADS), 0, (cudaStream_t)stream, a);
+  TS_LAUNCH_CHECK();
+}

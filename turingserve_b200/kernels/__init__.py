@@ -68,7 +68,7 @@ class LazyProduct:
 class CudaOps:
     """ctypes front of ``libturingserve_b200.so``."""
 
-    ABI = 26
+    ABI = 27
     UNSUPPORTED = -4            # a kernel's refusal of a shape or layout another kernel takes
 
     def __init__(self, lib_path: str) -> None:
@@ -104,6 +104,9 @@ class CudaOps:
             "ts_linear_tc_ex": [P, P, P, P, P, I, I, I, I, I, I, P, P],
             "ts_reduce_rmsnorm": [P, P, I, P, P, P, F, I, I, I, P],
             "ts_feed_tokens": [P, P, P, P, I, I, P],
+            "ts_rope_kv_write_q8": [P, L, P, P, P, P, P, P, P, P, P, I, I, I, I, I, I, I, P],
+            "ts_attention_q8": [P, L, P, L, P, P, P, P, P, P, P, I, I, I, I, I, I, I, F, I, I, P],
+            "ts_step_maps": [P, P, P, P, P, P, P, P, P, I, I, I, I, I, I, I, I, P],
             "ts_sample": [P, P, P, P, I, I, P, P],
             "ts_penalize": [P, P, P, P, I, I, P],
             "ts_sample_greedy": [P, P, I, I, P, P, P, P],
@@ -686,6 +689,99 @@ class CudaOps:
         self._check(self.lib.ts_linear_simt(_ptr(out), _ptr(x), _ptr(w), _ptr(bias), _ptr(rows), M, N, K,
                                             _code(x.dtype), _code(out.dtype), self._stream()), "linear")
         return out
+
+    # -- a cache in 8 bits -------------------------------------------------------------------------------------
+    @staticmethod
+    def _check_q8_cache(what: str, k_cache, v_cache, k_scale, v_scale, KVH: int, D: int, page_size: int, device) -> None:
+        pages = None
+        for c, s in ((k_cache, k_scale), (v_cache, v_scale)):
+            if c is None or s is None:
+                raise ValueError(f"{what}: keys and values come together, each with its scales")
+            if c.dtype is not torch.float8_e4m3fn or s.dtype is not torch.float32:
+                raise TypeError(f"{what}: keys and values in float8_e4m3fn with float32 scales, not {c.dtype} with {s.dtype}")
+            n = c.shape[0] if pages is None else pages
+            if c.shape != (n, KVH, page_size, D) or s.shape != (n, KVH) or not c.is_contiguous() or not s.is_contiguous():
+                raise ValueError(f"{what}: contiguous pages [n, {KVH}, {page_size}, {D}] with scales [n, {KVH}], not {tuple(c.shape)} "
+                                 f"with {tuple(s.shape)}")
+            if c.device != device or s.device != device:
+                raise ValueError(f"{what}: pages and scales must be on the tokens' device")
+            pages = n
+
+    def rope_kv_write_q8(self, q_out, qkv, positions, cos, sin, H: int, KVH: int, D: int, rotary_dim: int, k_cache, v_cache,
+                         k_scale, v_scale, slots, page_size: int) -> None:
+        """q_out [T, H D] = the rotated queries of ``qkv`` [T, (H + 2 KVH) D]; the rotated keys and the values go to pages of
+        8 bits (float8_e4m3fn [pages, KVH, page, D], scales float32 [pages, KVH]: a power of two per page and kv head,
+        from 2^-50 to 2^50, NaN for a page with a value that is not finite or above 448 * 2^50).  ``qkv`` stays as it is.
+        A page's scale grows with what is written to it, its other rows are brought to the new one; a call that writes the page's
+        first row begins the page anew.  The rows of one page stand next to each other among the tokens that are written and no slot
+        appears twice.  ``k_cache`` None: queries only; ``slots`` -1: that token is not written."""
+        T, code = qkv.shape[0], _code(qkv.dtype)
+        if qkv.shape != (T, (H + 2 * KVH) * D) or q_out.shape != (T, H * D) or q_out.dtype is not qkv.dtype:
+            raise ValueError(f"rope_kv_write_q8: [T, {(H + 2 * KVH) * D}] to [T, {H * D}] of one type, not {tuple(qkv.shape)} to "
+                             f"{tuple(q_out.shape)}")
+        if not qkv.is_contiguous() or q_out.stride(1) != 1:
+            raise ValueError("rope_kv_write_q8: rows must be contiguous")
+        if positions.dtype is not torch.int32 or positions.shape != (T,) or not positions.is_contiguous():
+            raise ValueError("rope_kv_write_q8: an int32 position for each token")
+        if rotary_dim < 0 or rotary_dim > D or rotary_dim % 2:
+            raise ValueError(f"rope_kv_write_q8: rotary_dim {rotary_dim} for head_dim {D}")
+        if rotary_dim:
+            for t in (cos, sin):
+                if t is None or t.dtype is not torch.float32 or t.shape[-1] != rotary_dim // 2 or not t.is_contiguous():
+                    raise ValueError(f"rope_kv_write_q8: float32 tables [positions, {rotary_dim // 2}]")
+        if k_cache is not None:
+            self._check_q8_cache("rope_kv_write_q8", k_cache, v_cache, k_scale, v_scale, KVH, D, page_size, qkv.device)
+            if slots is None or slots.dtype is not torch.int32 or slots.shape != (T,) or not slots.is_contiguous():
+                raise ValueError("rope_kv_write_q8: an int32 slot for each token")
+        self._check(self.lib.ts_rope_kv_write_q8(
+            _ptr(q_out), q_out.stride(0), _ptr(qkv), _ptr(positions), _ptr(cos), _ptr(sin), _ptr(k_cache), _ptr(v_cache),
+            _ptr(k_scale), _ptr(v_scale), _ptr(slots), T, H, KVH, D, rotary_dim, page_size, code, self._stream()), "rope_kv_write_q8")
+
+    def attention_q8(self, out, q, k_cache, v_cache, k_scale, v_scale, block_tables, step, KVH: int, page_size: int, scale: float,
+                     window) -> None:
+        """out [T, H D] = attention of q [T, H, D] (a view with contiguous heads) over pages of 8 bits as ``rope_kv_write_q8``
+        writes them: causal, with a ``window`` (None or 0: none) over the last that many keys.  The first
+        ``step.num_decode`` requests bring one token each.  A row that sees a page whose scale is NaN gives NaN."""
+        (T, H, D), code = q.shape, _code(q.dtype)
+        if KVH <= 0 or H % KVH:
+            raise ValueError(f"attention_q8: {H} heads over {KVH} kv heads")
+        if q.stride(2) != 1 or q.stride(1) != D or out.shape != (T, H * D) or out.stride(1) != 1 or out.dtype is not q.dtype:
+            raise ValueError("attention_q8: rows of contiguous heads, outputs [T, H D] in the queries' type")
+        B = step.num_requests
+        if block_tables.dtype is not torch.int32 or not block_tables.is_contiguous() or block_tables.shape[0] < B:
+            raise ValueError("attention_q8: an int32 block table for each request, rows contiguous")
+        self._check_q8_cache("attention_q8", k_cache, v_cache, k_scale, v_scale, KVH, D, page_size, q.device)
+        w = 0 if window is None else int(window)
+        if w < 0:
+            raise ValueError(f"attention_q8: a window of {w} keys")
+        self._check(self.lib.ts_attention_q8(
+            _ptr(out), out.stride(0), _ptr(q), q.stride(0), _ptr(k_cache), _ptr(v_cache), _ptr(k_scale), _ptr(v_scale),
+            _ptr(block_tables), _ptr(step.q_start), _ptr(step.seq_lens), B, block_tables.shape[1], step.max_q_len, H,
+            KVH, D, page_size, float(scale), w, code, self._stream()), "attention_q8")
+
+    # -- a step's maps -----------------------------------------------------------------------------------------
+    def step_maps(self, requests, updates, tables, page_size: int, q_start, seq_lens, token_request, positions, slot_mapping,
+                  block_tables) -> None:
+        """The maps of a step out of its requests' lengths, all int32.  ``requests`` [3, B]: each request's row of the page
+        tables (-1: a row that only pads the batch), its tokens in the cache, the tokens it brings; ``tables`` [groups, rows, pages]:
+        the pages of every request, kept on the GPU; ``updates`` [U, 4]: (group, row, index, page) put into the tables first (of
+        updates of one place the last holds).  Written: ``q_start`` [B + 1], ``seq_lens`` [B], ``token_request`` and
+        ``positions`` [T], ``slot_mapping`` [groups, T] (-1 for padding), ``block_tables`` [groups, B, width] (0 behind a
+        request's last page).  Kernels that read their step's arrays before they wait (``attention``) may not follow without a copy
+        or an event between."""
+        B, T, G = requests.shape[-1], positions.shape[0], tables.shape[0]
+        for name, t, shape in (("requests", requests, (3, B)), ("updates", updates, (updates.shape[0], 4)),
+                               ("tables", tables, (G, *tables.shape[1:3])), ("q_start", q_start, (B + 1,)), ("seq_lens", seq_lens, (B,)),
+                               ("token_request", token_request, (T,)), ("positions", positions, (T,)),
+                               ("slot_mapping", slot_mapping, (G, T)), ("block_tables", block_tables, (G, B, block_tables.shape[-1]))):
+            if t.dtype is not torch.int32 or t.shape != shape or not t.is_contiguous():
+                raise ValueError(f"step_maps: {name} is a contiguous int32 tensor {list(shape)}, not {t.dtype} {list(t.shape)}")
+        if tables.dim() != 3 or page_size < 1:
+            raise ValueError("step_maps: tables [groups, rows, pages] of pages of a token or more")
+        self._check(self.lib.ts_step_maps(
+            _ptr(requests), _ptr(updates), _ptr(tables), _ptr(q_start), _ptr(seq_lens), _ptr(token_request), _ptr(positions),
+            _ptr(slot_mapping), _ptr(block_tables), B, T, updates.shape[0], G, tables.shape[1], tables.shape[2],
+            block_tables.shape[2], page_size, self._stream()), "step_maps")
 
     # -- a residual stream in 32-bit ---------------------------------------------------------------------
     def rmsnorm_stream(self, out, stream, add1, add2, weight, eps: float, first: bool = False, alpha: float = 1.0,
