@@ -1,0 +1,586 @@
+// Attention of single tokens over an 8-bit paged cache (q8_cache.cuh): bfloat16 queries, heads of 64 or 128, up to 16
+// query heads a kv head, pages of any size.
+//
+// Mathematics.  Key j of a request has the score s_j = scale * log2(e) * (q . k8_j) * ks_j and the value v8_j * vs_j, the scales
+// powers of two.  With t_j = s_j + log2(vs_j) and a reference M >= every t_j,
+//   out = sum_j 2^(t_j - M) v8_j / sum_j 2^(t_j - M) / vs_j :
+// one exponential a key gives the weight of the value as it lies in the page, and the denominator takes it back to the
+// softmax's with an exact factor.  So both products run on what the pages hold, turned to half floats (exact for e4m3, one
+// instruction for two values): the queries as half floats too, each head scaled by a power of two to 128..256 (a bfloat16 fits
+// whole down to 2^-21 of the head's largest), the weights, at most 1, rounded to 2^-11 (2^-25 of the largest for the
+// smallest).  Scales span 2^-50..2^50, so a weight that vanishes here is below 2^-26 of the softmax's denominator.
+//
+// Layout.  Keys are the 16 rows of mma.sync m16n8k16 and heads its 8 columns (scores as K Q^T, outputs as V^T P^T): a group of up to
+// 8 heads leaves no row idle, half the instructions of heads on the rows.  A thread's four bytes of a key row, as ldmatrix
+// brings them, are two pairs of columns of the A operand under an order of the head's columns that the queries share; value
+// bytes come transposed in pairs, one byte permutation puts two keys of a column side by side.
+//
+// Work.  One block of four warps a (split, kv head, request); every warp walks tiles of 32 keys of its own with a ring of three
+// stages filled by its own cp.async (16 bytes a lane, rows outside the visible range filled with zeros): no barrier and
+// no other warp in the loop.  The warps' sums meet in shared memory; the splits' in a cluster's distributed shared memory
+// where the blocks of a request and kv head form one, else a second kernel sums what they left in scratch.
+#include "mma_utils.cuh"
+#include "q8_cache.cuh"
+
+namespace {
+
+using namespace q8;
+
+constexpr int WARPS = 4, THREADS = WARPS * 32, TILE = 32, STAGES = 3;
+constexpr float LOG2E_Q8 = 1.4426950408889634f;
+
+struct DecArgs {
+  bf16* out;
+  long long o_ts;
+  const bf16* q;
+  long long q_ts;
+  const unsigned char* cache[2];
+  const float* scales[2];
+  const int* block_tables;
+  const int* q_start;
+  const int* seq_lens;
+  float* part;                   // [B][KVH][nsplit][G][D] sums, then [B][KVH][nsplit][G][2] (reference, denominator)
+  int B, table_width, H, KVH, page;
+  float scale;
+  int window, nsplit, cluster, early;
+};
+
+__device__ __forceinline__ float ex2_q8(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+__device__ __forceinline__ unsigned half2_of(unsigned short e4m3x2) {
+  unsigned r;
+  asm("cvt.rn.f16x2.e4m3x2 %0, %1;" : "=r"(r) : "h"(e4m3x2));
+  return r;
+}
+__device__ __forceinline__ void halves_of(unsigned w, unsigned& lo, unsigned& hi) {
+  lo = half2_of((unsigned short)(w & 0xffffu));
+  hi = half2_of((unsigned short)(w >> 16));
+}
+__device__ __forceinline__ unsigned pack_half(float lo, float hi) {
+  const __half2 h = __floats2half2_rn(lo, hi);
+  return *reinterpret_cast<const unsigned*>(&h);
+}
+__device__ __forceinline__ unsigned transpose8x8(unsigned a) {
+  unsigned r;
+  asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(a));
+  return r;
+}
+__device__ __forceinline__ void mma_f16(float (&d)[4], unsigned a0, unsigned a1, unsigned a2, unsigned a3, unsigned b0, unsigned b1) {
+  asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};\n"
+               : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+               : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ void cp_async_4(void* smem, const void* gmem, bool valid) {
+  const unsigned s = (unsigned)__cvta_generic_to_shared(smem);
+  const int bytes = valid ? 4 : 0;
+  asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;\n" ::"r"(s), "l"(gmem), "r"(bytes));
+}
+
+// A stage: key rows, value rows (32 of D bytes each), their scales.
+template <int D>
+struct Stage {
+  static constexpr int TILE_BYTES = TILE * D;
+  static constexpr int BYTES = 2 * TILE_BYTES + 2 * TILE * 4;
+  static constexpr int WARP_BYTES = STAGES * BYTES;
+  static constexpr size_t SMEM = (size_t)WARPS * WARP_BYTES;
+  static constexpr int O_ROW = D + 4;                            // floats of a head's sums in shared memory
+};
+// Byte offset of 16-byte piece c of a tile's row: pieces of a 128-byte line (one row of 128, two of 64) swapped by the line's number,
+// so that eight rows' pieces lie in different banks.
+template <int D>
+__device__ __forceinline__ int piece_off(int row, int c) {
+  const int line = D == 128 ? row : row >> 1, at = D == 128 ? c : (row & 1) * 4 + c;
+  return line * 128 + ((at ^ (line & 7)) << 4);
+}
+
+template <int D, int NG>
+__global__ void __launch_bounds__(THREADS) attention_q8_decode_kernel(const DecArgs a) {
+  pdl_launch_dependents();
+  using ST = Stage<D>;
+  constexpr int KS = D / 16, CPR = D / 16;                       // k-steps of a score; 16-byte pieces of a row
+  constexpr int LPT = TILE * CPR / 32;                           // pieces a lane fetches of a tile
+  extern __shared__ __align__(128) unsigned char smem[];
+  const int split = blockIdx.x, kvh = blockIdx.y, b = blockIdx.z;
+  const int G = a.H / a.KVH, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int g = lane >> 2, c = lane & 3;
+  if (!a.early) pdl_wait();
+  const int seq_len = a.seq_lens[b], row_q = a.q_start[b];
+  const int lo = a.window > 0 ? max(0, seq_len - a.window) : 0;
+  const int tile_first = lo / TILE, total = seq_len > 0 ? (seq_len - 1) / TILE - tile_first + 1 : 0;
+  const int shares = a.nsplit * WARPS, share = split * WARPS + warp;
+  const int my_first = tile_first + (int)((long long)total * share / shares);
+  const int n_tiles = tile_first + (int)((long long)total * (share + 1) / shares) - my_first;
+
+  unsigned char* ring = smem + warp * ST::WARP_BYTES;
+  const int* table = a.block_tables + (size_t)b * a.table_width;
+  // the cache row of key my_first * TILE + lane + 32 i, or -1 outside the visible range
+  auto row_of = [&](int i) {
+    const int j = (my_first + i) * TILE + lane, lp = j / a.page;
+    if (i >= n_tiles || j < lo || j >= seq_len || lp >= a.table_width) return -1;
+    return (table[lp] * a.KVH + kvh) * a.page + (j - lp * a.page);
+  };
+  auto fetch = [&](int i, int row) {                             // this lane's key's row; i < n_tiles
+    unsigned char* st = ring + (i % STAGES) * ST::BYTES;
+    const int c16 = lane % CPR;
+#pragma unroll
+    for (int u = 0; u < LPT; ++u) {
+      const int key = lane / CPR + u * (32 / CPR);
+      const int r = __shfl_sync(0xffffffffu, row, key);
+      const size_t off = (size_t)(r < 0 ? 0 : r) * D + c16 * 16;
+      const int at = piece_off<D>(key, c16);
+      cp_async_16(st + at, a.cache[0] + off, r >= 0);
+      cp_async_16(st + ST::TILE_BYTES + at, a.cache[1] + off, r >= 0);
+    }
+    float* sc = reinterpret_cast<float*>(st + 2 * ST::TILE_BYTES);
+    const int pk = row < 0 ? 0 : row / a.page;                   // page * KVH + kv head
+    cp_async_4(sc + lane, a.scales[0] + pk, row >= 0);
+    cp_async_4(sc + TILE + lane, a.scales[1] + pk, row >= 0);
+  };
+
+  int issued = 0;
+  if (a.early) {
+    // Rows before the page that takes the new token were written by earlier steps: fetched while the kernels before still run.
+    // (That page's scale may still grow, and its rows move with it.)
+    const int settled = (seq_len - 1) / a.page * a.page;
+    while (issued < min(n_tiles, STAGES - 1) && (my_first + issued + 1) * TILE <= settled) {
+      fetch(issued, row_of(issued));
+      cp_async_commit();
+      ++issued;
+    }
+    pdl_wait();
+  }
+  for (; issued < STAGES - 1; ++issued) {
+    if (issued < n_tiles) fetch(issued, row_of(issued));
+    cp_async_commit();
+  }
+  int next_row = row_of(STAGES - 1);
+
+  // queries: head g of the group (and g + 8), columns in the order of the keys' bytes
+  unsigned qf[NG][KS][2];
+  float factor[NG][2];                                           // of the heads that are this lane's columns: 2c, 2c + 1
+#pragma unroll
+  for (int ng = 0; ng < NG; ++ng) {
+    const int head = ng * 8 + g;
+    const bf16* src = a.q + (size_t)row_q * a.q_ts + (size_t)(kvh * G + min(head, G - 1)) * D + 4 * c;
+    uint2 raw[KS];
+    float amax = 0.f;
+    bool finite = true;
+#pragma unroll
+    for (int ks = 0; ks < KS; ++ks) {
+      raw[ks] = head < G && n_tiles > 0 ? *reinterpret_cast<const uint2*>(src + ks * 16) : make_uint2(0u, 0u);
+      const float2 x = __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&raw[ks].x));
+      const float2 y = __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&raw[ks].y));
+      const float m4 = fmaxf(fmaxf(fabsf(x.x), fabsf(x.y)), fmaxf(fabsf(y.x), fabsf(y.y)));
+      amax = fmaxf(amax, m4);
+      finite = finite && x.x - x.x == 0.f && x.y - x.y == 0.f && y.x - y.x == 0.f && y.y - y.y == 0.f;
+    }
+    amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 1));
+    amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 2));
+    const unsigned bad = __ballot_sync(0xffffffffu, !finite);
+    const int e = max((int)(__float_as_uint(amax) >> 23) - 127, -110);
+    const float to_half = __uint_as_float((unsigned)(127 + 7 - e) << 23);
+    float f = a.scale * LOG2E_Q8 * __uint_as_float((unsigned)(127 - 7 + e) << 23);
+    if ((bad >> (lane & ~3)) & 0xfu) f = __uint_as_float(NAN_BITS);
+#pragma unroll
+    for (int ks = 0; ks < KS; ++ks) {
+      const float2 x = __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&raw[ks].x));
+      const float2 y = __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&raw[ks].y));
+      qf[ng][ks][0] = pack_half(x.x * to_half, x.y * to_half);
+      qf[ng][ks][1] = pack_half(y.x * to_half, y.y * to_half);
+    }
+    factor[ng][0] = __shfl_sync(0xffffffffu, f, 8 * c);
+    factor[ng][1] = __shfl_sync(0xffffffffu, f, 8 * c + 4);
+  }
+
+  float o[NG][KS][4];
+  float m[NG][2], l[NG][2];                                      // per head of this lane's columns; l of this lane's keys alone
+#pragma unroll
+  for (int ng = 0; ng < NG; ++ng) {
+#pragma unroll
+    for (int t = 0; t < KS; ++t) o[ng][t][0] = o[ng][t][1] = o[ng][t][2] = o[ng][t][3] = 0.f;
+    m[ng][0] = m[ng][1] = -INFINITY;
+    l[ng][0] = l[ng][1] = 0.f;
+  }
+  const int mat = lane >> 3, r8 = lane & 7;
+  for (int i = 0; i < n_tiles; ++i) {
+    cp_async_wait<STAGES - 2>();
+    __syncwarp();                                                // every lane's copies of tile i are in, and tile i - 1 is read
+    if (i + STAGES - 1 < n_tiles) fetch(i + STAGES - 1, next_row);
+    cp_async_commit();
+    next_row = row_of(i + STAGES);
+    const unsigned char* ks_ = ring + (i % STAGES) * ST::BYTES;
+    const unsigned char* vs_ = ks_ + ST::TILE_BYTES;
+    const float* sc = reinterpret_cast<const float*>(ks_ + 2 * ST::TILE_BYTES);
+    const int j0 = (my_first + i) * TILE;
+    const bool edge = j0 < lo || j0 + TILE > seq_len;
+    // scores [32 keys x 8 heads]: rows g and g + 8 of two tiles of 16 keys, columns 2c and 2c + 1
+    float s[NG][2][4];
+#pragma unroll
+    for (int ng = 0; ng < NG; ++ng)
+#pragma unroll
+      for (int mt = 0; mt < 2; ++mt) s[ng][mt][0] = s[ng][mt][1] = s[ng][mt][2] = s[ng][mt][3] = 0.f;
+#pragma unroll
+    for (int ks = 0; ks < KS; ks += 2)
+#pragma unroll
+      for (int mt = 0; mt < 2; ++mt) {
+        unsigned w0, w1, w2, w3, x0, x1, x2, x3;
+        ldmatrix_x4(w0, w1, w2, w3, ks_ + piece_off<D>(mt * 16 + (mat & 1) * 8 + r8, ks + (mat >> 1)));
+        halves_of(w0, x0, x2);
+        halves_of(w1, x1, x3);
+#pragma unroll
+        for (int ng = 0; ng < NG; ++ng) mma_f16(s[ng][mt], x0, x1, x2, x3, qf[ng][ks][0], qf[ng][ks][1]);
+        halves_of(w2, x0, x2);
+        halves_of(w3, x1, x3);
+#pragma unroll
+        for (int ng = 0; ng < NG; ++ng) mma_f16(s[ng][mt], x0, x1, x2, x3, qf[ng][ks + 1][0], qf[ng][ks + 1][1]);
+      }
+    // t = score + log2 of the value's scale; online maximum per head
+    float kf[2][2], back[2][2], lift[2][2];                      // [tile of 16][row g or g + 8]
+#pragma unroll
+    for (int mt = 0; mt < 2; ++mt)
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        const int key = mt * 16 + h * 8 + g;
+        const float kscale = sc[key], vscale = sc[TILE + key];
+        kf[mt][h] = vscale != vscale ? vscale : kscale;
+        back[mt][h] = inverse_scale(vscale);
+        lift[mt][h] = (float)((int)(__float_as_uint(vscale) >> 23) - 127);
+      }
+#pragma unroll
+    for (int ng = 0; ng < NG; ++ng) {
+      float mx[2] = {-INFINITY, -INFINITY};
+#pragma unroll
+      for (int mt = 0; mt < 2; ++mt)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const int h = e >> 1;
+          float t = fmaf(s[ng][mt][e] * kf[mt][h], factor[ng][e & 1], lift[mt][h]);
+          if (edge) {
+            const int j = j0 + mt * 16 + h * 8 + g;
+            t = j >= lo && j < seq_len ? t : -INFINITY;
+          }
+          s[ng][mt][e] = t;
+          mx[e & 1] = fmaxf(mx[e & 1], t);
+        }
+      float corr[2];
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        mx[e] = fmaxf(mx[e], __shfl_xor_sync(0xffffffffu, mx[e], 4));
+        mx[e] = fmaxf(mx[e], __shfl_xor_sync(0xffffffffu, mx[e], 8));
+        mx[e] = fmaxf(mx[e], __shfl_xor_sync(0xffffffffu, mx[e], 16));
+        const float now = fmaxf(m[ng][e], mx[e]);                // finite, unless all that is seen is NaN (then so are the sums)
+        corr[e] = ex2_q8(m[ng][e] - now);
+        m[ng][e] = now;
+        l[ng][e] *= corr[e];
+      }
+      unsigned pf[2][2];
+#pragma unroll
+      for (int mt = 0; mt < 2; ++mt) {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const float p = ex2_q8(s[ng][mt][e] - m[ng][e & 1]);
+          s[ng][mt][e] = p;
+          l[ng][e & 1] = fmaf(p, back[mt][e >> 1], l[ng][e & 1]);
+        }
+        pf[mt][0] = transpose8x8(pack_half(s[ng][mt][0], s[ng][mt][1]));
+        pf[mt][1] = transpose8x8(pack_half(s[ng][mt][2], s[ng][mt][3]));
+      }
+#pragma unroll
+      for (int t = 0; t < KS; ++t) {
+        o[ng][t][0] *= corr[0];
+        o[ng][t][1] *= corr[1];
+        o[ng][t][2] *= corr[0];
+        o[ng][t][3] *= corr[1];
+      }
+      s[ng][0][0] = __uint_as_float(pf[0][0]);
+      s[ng][0][1] = __uint_as_float(pf[0][1]);
+      s[ng][1][0] = __uint_as_float(pf[1][0]);
+      s[ng][1][1] = __uint_as_float(pf[1][1]);
+    }
+    // outputs [D x 8 heads] += values^T [D x 32 keys] weights^T [32 keys x 8 heads]; row g of a tile of 16 columns is column 2g, row
+    // g + 8 column 2g + 1
+#pragma unroll
+    for (int mt = 0; mt < 2; ++mt)
+#pragma unroll
+      for (int t = 0; t < KS; t += 2) {
+        unsigned w0, w1, w2, w3, x0, x1, x2, x3;
+        ldmatrix_x4_trans(w0, w1, w2, w3, vs_ + piece_off<D>(mt * 16 + (mat & 1) * 8 + r8, t + (mat >> 1)));
+        halves_of(__byte_perm(w0, 0, 0x3120), x0, x1);
+        halves_of(__byte_perm(w1, 0, 0x3120), x2, x3);
+#pragma unroll
+        for (int ng = 0; ng < NG; ++ng)
+          mma_f16(o[ng][t], x0, x1, x2, x3, __float_as_uint(s[ng][mt][0]), __float_as_uint(s[ng][mt][1]));
+        halves_of(__byte_perm(w2, 0, 0x3120), x0, x1);
+        halves_of(__byte_perm(w3, 0, 0x3120), x2, x3);
+#pragma unroll
+        for (int ng = 0; ng < NG; ++ng)
+          mma_f16(o[ng][t + 1], x0, x1, x2, x3, __float_as_uint(s[ng][mt][0]), __float_as_uint(s[ng][mt][1]));
+      }
+  }
+  cp_async_wait<0>();
+  __syncthreads();                                               // the rings are free: the warps' sums go over them
+
+  constexpr int O_ROW = ST::O_ROW;
+  float* o_s = reinterpret_cast<float*>(smem);                   // [WARPS][G][O_ROW]
+  float* m_s = o_s + WARPS * G * O_ROW;                          // [WARPS][G]
+  float* l_s = m_s + WARPS * G;                                  // [WARPS][G]
+  float* M_s = l_s + WARPS * G;                                  // [G]: the block's
+  float* L_s = M_s + G;
+#pragma unroll
+  for (int ng = 0; ng < NG; ++ng)
+#pragma unroll
+    for (int e = 0; e < 2; ++e) {
+      const int head = ng * 8 + 2 * c + e;
+      float sum = l[ng][e];
+      sum += __shfl_xor_sync(0xffffffffu, sum, 4);
+      sum += __shfl_xor_sync(0xffffffffu, sum, 8);
+      sum += __shfl_xor_sync(0xffffffffu, sum, 16);
+      if (head < G) {
+        if (g == 0) {
+          m_s[warp * G + head] = m[ng][e];
+          l_s[warp * G + head] = sum;
+        }
+        float* dst = o_s + (size_t)(warp * G + head) * O_ROW + 2 * g;
+#pragma unroll
+        for (int t = 0; t < KS; ++t) *reinterpret_cast<float2*>(dst + t * 16) = make_float2(o[ng][t][e], o[ng][t][2 + e]);
+      }
+    }
+  __syncthreads();
+  // weight of a part: 2^(m - M); a part without keys (m = -inf, l = 0) has none, one whose keys are all NaN keeps that
+  auto weight = [](float m1, float l1, float M) { return m1 == -INFINITY ? l1 : ex2_q8(m1 - M); };
+  if ((int)threadIdx.x < G) {
+    float M = -INFINITY, L = 0.f;
+#pragma unroll
+    for (int w = 0; w < WARPS; ++w) M = fmaxf(M, m_s[w * G + threadIdx.x]);
+#pragma unroll
+    for (int w = 0; w < WARPS; ++w) {
+      const float l1 = l_s[w * G + threadIdx.x], f = weight(m_s[w * G + threadIdx.x], l1, M);
+      L = fmaf(l1, f, L);
+      m_s[w * G + threadIdx.x] = f;
+    }
+    M_s[threadIdx.x] = M;
+    L_s[threadIdx.x] = L;
+  }
+  __syncthreads();
+  const bool whole = a.nsplit == 1;
+  for (int idx = threadIdx.x; idx < G * (D / 4); idx += THREADS) {
+    const int h = idx / (D / 4), d = (idx % (D / 4)) * 4;
+    float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+    for (int w = 0; w < WARPS; ++w) {
+      const float f = m_s[w * G + h];
+      const float4 x = *reinterpret_cast<const float4*>(o_s + (size_t)(w * G + h) * O_ROW + d);
+      acc.x = fmaf(x.x, f, acc.x);
+      acc.y = fmaf(x.y, f, acc.y);
+      acc.z = fmaf(x.z, f, acc.z);
+      acc.w = fmaf(x.w, f, acc.w);
+    }
+    if (whole) {
+      const float L = L_s[h], inv = L > 0.f ? 1.f / L : L;       // nothing seen: 0
+      bf16* dst = a.out + (size_t)row_q * a.o_ts + (size_t)(kvh * G + h) * D + d;
+      *reinterpret_cast<uint2*>(dst) = make_uint2(pack_bf16(acc.x * inv, acc.y * inv), pack_bf16(acc.z * inv, acc.w * inv));
+    } else if (a.cluster) {
+      *reinterpret_cast<float4*>(o_s + (size_t)h * O_ROW + d) = acc;      // over the first warp's, which this thread alone reads here
+    } else {
+      const size_t at = ((size_t)(b * a.KVH + kvh) * a.nsplit + split) * G + h;
+      *reinterpret_cast<float4*>(a.part + at * D + d) = acc;
+      if (d == 0)
+        *reinterpret_cast<float2*>(a.part + (size_t)a.B * a.KVH * a.nsplit * G * D + at * 2) = make_float2(M_s[h], L_s[h]);
+    }
+  }
+  if (whole || !a.cluster) return;
+  // Block `split` finishes the pieces split, split + nsplit, ... out of its peers' shared memory, in split order.
+  cluster_sync_all();
+  for (int piece = split + a.nsplit * (int)threadIdx.x; piece < G * (D / 4); piece += a.nsplit * THREADS) {
+    const int h = piece / (D / 4), d = (piece % (D / 4)) * 4;
+    float m1[8], l1[8];
+    float4 x[8];
+    float M = -INFINITY;
+#pragma unroll
+    for (int s2 = 0; s2 < 8; ++s2)
+      if (s2 < a.nsplit) {
+        m1[s2] = ld_peer_f32(peer_shared(M_s + h, s2));
+        l1[s2] = ld_peer_f32(peer_shared(L_s + h, s2));
+        x[s2] = ld_peer_v4(peer_shared(o_s + (size_t)h * O_ROW + d, s2));
+        M = fmaxf(M, m1[s2]);
+      }
+    float L = 0.f;
+    float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+    for (int s2 = 0; s2 < 8; ++s2)
+      if (s2 < a.nsplit) {
+        const float f = weight(m1[s2], l1[s2], M);
+        L = fmaf(l1[s2], f, L);
+        acc.x = fmaf(x[s2].x, f, acc.x);
+        acc.y = fmaf(x[s2].y, f, acc.y);
+        acc.z = fmaf(x[s2].z, f, acc.z);
+        acc.w = fmaf(x[s2].w, f, acc.w);
+      }
+    const float inv = L > 0.f ? 1.f / L : L;
+    bf16* dst = a.out + (size_t)row_q * a.o_ts + (size_t)(kvh * G + h) * D + d;
+    *reinterpret_cast<uint2*>(dst) = make_uint2(pack_bf16(acc.x * inv, acc.y * inv), pack_bf16(acc.z * inv, acc.w * inv));
+  }
+  cluster_sync_all();                                            // no block leaves while a peer still reads it
+}
+
+// The splits' sums out of scratch: one block a (kv head, request) and head of its group, a thread four columns, split order.
+template <int D>
+__global__ void __launch_bounds__(D / 4 * 4) attention_q8_merge_kernel(const DecArgs a) {
+  pdl_launch_dependents();
+  pdl_wait();
+  constexpr int COLS = D / 4, PARTS = 4;                         // four threads a column cut the splits among themselves
+  __shared__ float4 acc_s[PARTS][COLS];
+  __shared__ float L_s[PARTS];
+  const int h = blockIdx.x, kvh = blockIdx.y, b = blockIdx.z, G = a.H / a.KVH;
+  const int col = threadIdx.x % COLS, part = threadIdx.x / COLS;
+  const size_t first = (size_t)(b * a.KVH + kvh) * a.nsplit;
+  const float* ml = a.part + (size_t)a.B * a.KVH * a.nsplit * G * D;
+  float M = -INFINITY;
+  for (int s = 0; s < a.nsplit; ++s) M = fmaxf(M, ml[((first + s) * G + h) * 2]);
+  float L = 0.f;
+  float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 4
+  for (int s = part; s < a.nsplit; s += PARTS) {
+    const float2 x = *reinterpret_cast<const float2*>(ml + ((first + s) * G + h) * 2);
+    const float4 y = *reinterpret_cast<const float4*>(a.part + ((first + s) * G + h) * D + col * 4);
+    const float f = x.x == -INFINITY ? x.y : ex2_q8(x.x - M);
+    L = fmaf(x.y, f, L);
+    acc.x = fmaf(y.x, f, acc.x);
+    acc.y = fmaf(y.y, f, acc.y);
+    acc.z = fmaf(y.z, f, acc.z);
+    acc.w = fmaf(y.w, f, acc.w);
+  }
+  acc_s[part][col] = acc;
+  if (col == 0) L_s[part] = L;
+  __syncthreads();
+  if (part != 0) return;
+  for (int p = 1; p < PARTS; ++p) {
+    const float4 y = acc_s[p][col];
+    acc.x += y.x;
+    acc.y += y.y;
+    acc.z += y.z;
+    acc.w += y.w;
+    L += L_s[p];
+  }
+  const float inv = L > 0.f ? 1.f / L : L;
+  bf16* dst = a.out + (size_t)a.q_start[b] * a.o_ts + (size_t)(kvh * G + h) * D + col * 4;
+  *reinterpret_cast<uint2*>(dst) = make_uint2(pack_bf16(acc.x * inv, acc.y * inv), pack_bf16(acc.z * inv, acc.w * inv));
+}
+
+template <int D, int NG>
+int prepare_kernel() {
+  static const int slots = [] {
+    if (cudaFuncSetAttribute(attention_q8_decode_kernel<D, NG>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)Stage<D>::SMEM) != cudaSuccess) {
+      cudaGetLastError();
+      return 0;
+    }
+    int n = 0;
+    if (cudaOccupancyMaxActiveBlocksPerMultiprocessor(&n, attention_q8_decode_kernel<D, NG>, THREADS, Stage<D>::SMEM) != cudaSuccess) {
+      cudaGetLastError();
+      return 0;
+    }
+    return n;
+  }();
+  return slots;
+}
+
+// How many clusters of n blocks the chip holds at once.
+template <int D, int NG>
+int clusters_that_fit(int n) {
+  static int known[9];
+  int& k = known[n];
+  if (k == 0) {
+    k = -1;
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(n, 1, 1);
+    cfg.blockDim = dim3(THREADS);
+    cfg.dynamicSmemBytes = Stage<D>::SMEM;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim.x = (unsigned)n;
+    attr[0].val.clusterDim.y = 1;
+    attr[0].val.clusterDim.z = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    int clusters = 0;
+    if (cudaOccupancyMaxActiveClusters(&clusters, attention_q8_decode_kernel<D, NG>, &cfg) == cudaSuccess && clusters >= 1) k = clusters;
+    cudaGetLastError();                                          // a refusal is an answer, not an error
+  }
+  return k;
+}
+
+int g_splits = 0, g_cluster = 1;
+
+// Splits of a request's keys and whether they form clusters: (splits, cluster), the same for every call of these sizes.
+template <int D, int NG>
+int plan(int pairs, int reach, int& cluster) {
+  const int slots = prepare_kernel<D, NG>() * ts_sm_count();
+  const int most = reach <= 256 ? 1 : (reach + 255) / 256;       // two tiles a warp at least
+  int n = pairs > 0 ? slots / pairs : 1;
+  n = n < 1 ? 1 : n;
+  n = n > most ? most : n;
+  n = n > 128 ? 128 : n;
+  if (g_splits > 0) n = g_splits;
+  cluster = 0;
+  if (n >= 2 && n <= 8 && g_cluster && ts_clusters_enabled() && clusters_that_fit<D, NG>(n) >= pairs) cluster = 1;
+  return n;
+}
+
+template <int D, int NG>
+int launch(DecArgs a, int reach, cudaStream_t s) {
+  if (prepare_kernel<D, NG>() == 0) TS_REFUSE(TS_ERR_UNSUPPORTED, "ts_attention_q8_decode: the device does not hold a block");
+  a.nsplit = plan<D, NG>(a.B * a.KVH, reach, a.cluster);
+  if (a.nsplit > 1 && !a.cluster && a.part == nullptr) TS_REFUSE(TS_ERR_SHAPE, "ts_attention_q8_decode: %d splits need scratch", a.nsplit);
+  cudaError_t e = ts_launch_cluster(attention_q8_decode_kernel<D, NG>, dim3(a.cluster ? a.nsplit : 1, 1, 1), dim3(a.nsplit, a.KVH, a.B),
+                                    dim3(THREADS), Stage<D>::SMEM, s, a);
+  if (e != cudaSuccess) TS_REFUSE((int)e, "ts_attention_q8_decode: %s", cudaGetErrorString(e));
+  if (a.nsplit > 1 && !a.cluster) {
+    e = ts_launch(attention_q8_merge_kernel<D>, dim3(a.H / a.KVH, a.KVH, a.B), dim3(D), 0, s, a);
+    if (e != cudaSuccess) TS_REFUSE((int)e, "ts_attention_q8_decode: %s", cudaGetErrorString(e));
+  }
+  TS_LAUNCH_CHECK();
+}
+
+}  // namespace
+
+TS_API void ts_set_q8_decode(int splits, int cluster) {           // for measurements; 0: by the sizes
+  g_splits = splits < 0 || splits > 128 ? 0 : splits;
+  g_cluster = cluster;
+}
+
+TS_API int ts_attention_q8_decode_supported(int H, int KVH, int D, int dtype) {
+  return dtype == TS_BF16 && KVH > 0 && H % KVH == 0 && H / KVH <= 16 && (D == 64 || D == 128);
+}
+
+// Floats of scratch that B requests of up to `reach` visible keys take: 0 where the splits need none.
+TS_API long long ts_attention_q8_decode_scratch(int B, int H, int KVH, int D, int reach) {
+  int cluster = 0, n = 1;
+  const int pairs = B * KVH;
+  if (D == 64) n = H / KVH <= 8 ? plan<64, 1>(pairs, reach, cluster) : plan<64, 2>(pairs, reach, cluster);
+  else n = H / KVH <= 8 ? plan<128, 1>(pairs, reach, cluster) : plan<128, 2>(pairs, reach, cluster);
+  return n > 1 && !cluster ? (long long)B * H * n * (D + 2) : 0;
+}
+
+// One query token per request (rows q_start[b]).  reach: the most keys a request sees.  early: index arrays and cache rows before
+// each request's last page are in place already and are read before the wait for the kernels before.
+TS_API int ts_attention_q8_decode(void* out, long long o_ts, const void* q, long long q_ts, const void* k_cache, const void* v_cache,
+                                  const float* k_scale, const float* v_scale, const int* block_tables, const int* q_start,
+                                  const int* seq_lens, float* scratch, int B, int table_width, int reach, int H, int KVH, int D,
+                                  int page, int num_pages, float scale, int window, int early, void* stream) {
+  if (B <= 0) return 0;
+  if (!ts_attention_q8_decode_supported(H, KVH, D, TS_BF16) || page <= 0)
+    TS_REFUSE(TS_ERR_UNSUPPORTED, "ts_attention_q8_decode: H=%d KVH=%d D=%d page=%d is not taken by this kernel", H, KVH, D, page);
+  if (B > 65535 || KVH > 65535) TS_REFUSE(TS_ERR_UNSUPPORTED, "ts_attention_q8_decode: %d requests / %d kv heads", B, KVH);
+  if ((((uintptr_t)k_cache | (uintptr_t)v_cache | (uintptr_t)scratch) & 15) != 0 || (((uintptr_t)q | (uintptr_t)out) & 7) != 0 ||
+      (q_ts & 3) != 0 || (o_ts & 3) != 0)
+    TS_REFUSE(TS_ERR_UNSUPPORTED, "ts_attention_q8_decode: pages on 16 bytes, rows of queries and outputs on 8");
+  if ((long long)num_pages * KVH * page > 0x7fffffffLL) TS_REFUSE(TS_ERR_UNSUPPORTED, "ts_attention_q8_decode: a cache of more than 2^31 rows");
+  DecArgs a = {(bf16*)out, o_ts, (const bf16*)q, q_ts, {(const unsigned char*)k_cache, (const unsigned char*)v_cache},
+               {k_scale, v_scale}, block_tables, q_start, seq_lens, scratch, B, table_width, H, KVH, page, scale, window, 1, 0, early};
+  cudaStream_t s = (cudaStream_t)stream;
+  if (D == 64) return H / KVH <= 8 ? launch<64, 1>(a, reach, s) : launch<64, 2>(a, reach, s);
+  return H / KVH <= 8 ? launch<128, 1>(a, reach, s) : launch<128, 2>(a, reach, s);
+}

@@ -106,6 +106,8 @@ class CudaOps:
             "ts_feed_tokens": [P, P, P, P, I, I, P],
             "ts_rope_kv_write_q8": [P, L, P, P, P, P, P, P, P, P, P, I, I, I, I, I, I, I, P],
             "ts_attention_q8": [P, L, P, L, P, P, P, P, P, P, P, I, I, I, I, I, I, I, F, I, I, P],
+            "ts_attention_q8_decode": [P, L, P, L, P, P, P, P, P, P, P, P, I, I, I, I, I, I, I, I, F, I, I, P],
+            "ts_attention_q8_decode_supported": [I, I, I, I],
             "ts_step_maps": [P, P, P, P, P, P, P, P, P, I, I, I, I, I, I, I, I, P],
             "ts_sample": [P, P, P, P, I, I, P, P],
             "ts_penalize": [P, P, P, P, I, I, P],
@@ -177,6 +179,10 @@ class CudaOps:
             fn = getattr(self.lib, name)
             fn.argtypes = args
             fn.restype = c_int
+        self.lib.ts_attention_q8_decode_scratch.argtypes = [I, I, I, I, I]
+        self.lib.ts_attention_q8_decode_scratch.restype = L
+        self.lib.ts_set_q8_decode.argtypes = [I, I]
+        self.lib.ts_set_q8_decode.restype = None
         self.lib.ts_attention_diff_mma_supported.argtypes = [I, I, I, I, I]
         self.lib.ts_attention_diff_mma_supported.restype = c_int
         self.lib.ts_attention_diff_mma_scratch_floats.argtypes = [I, I, I, I]
@@ -754,10 +760,31 @@ class CudaOps:
         w = 0 if window is None else int(window)
         if w < 0:
             raise ValueError(f"attention_q8: a window of {w} keys")
+        nd, width, max_seq = step.num_decode, block_tables.shape[1], step.max_seq_len
+        if nd and self.use_fast_attention and self.lib.ts_attention_q8_decode_supported(H, KVH, D, code):
+            reach = min(max_seq, w) if w else max_seq
+            need = self.lib.ts_attention_q8_decode_scratch(nd, H, KVH, D, reach)
+            # (a work buffer of this call's own: calls on two streams, or in two captured graphs, do not meet in it)
+            scratch = torch.empty(need, dtype=torch.float32, device=q.device) if need else None
+            rc = self.lib.ts_attention_q8_decode(
+                out.data_ptr(), out.stride(0), q.data_ptr(), q.stride(0), k_cache.data_ptr(), v_cache.data_ptr(), k_scale.data_ptr(),
+                v_scale.data_ptr(), block_tables.data_ptr(), step.q_start.data_ptr(), step.seq_lens.data_ptr(), _ptr(scratch), nd, width,
+                reach, H, KVH, D, page_size, k_cache.shape[0], scale, w, 1 if getattr(step, "settled", False) else 0, self._stream())
+            if rc == self.UNSUPPORTED:
+                nd = 0
+            else:
+                self._check(rc, "attention_q8_decode")
+                if need:
+                    self.launches += 1
+        else:
+            nd = 0
+        if nd == B:
+            return
         self._check(self.lib.ts_attention_q8(
-            _ptr(out), out.stride(0), _ptr(q), q.stride(0), _ptr(k_cache), _ptr(v_cache), _ptr(k_scale), _ptr(v_scale),
-            _ptr(block_tables), _ptr(step.q_start), _ptr(step.seq_lens), B, block_tables.shape[1], step.max_q_len, H,
-            KVH, D, page_size, float(scale), w, code, self._stream()), "attention_q8")
+            out.data_ptr(), out.stride(0), q.data_ptr(), q.stride(0), k_cache.data_ptr(), v_cache.data_ptr(), k_scale.data_ptr(),
+            v_scale.data_ptr(), block_tables.data_ptr() + 4 * nd * width, step.q_start.data_ptr() + 4 * nd,
+            step.seq_lens.data_ptr() + 4 * nd, B - nd, width, step.max_q_len, H, KVH, D, page_size, float(scale), w, code,
+            self._stream()), "attention_q8")
 
     # -- a step's maps -----------------------------------------------------------------------------------------
     def step_maps(self, requests, updates, tables, page_size: int, q_start, seq_lens, token_request, positions, slot_mapping,
