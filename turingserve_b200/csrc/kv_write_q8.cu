@@ -37,7 +37,7 @@ __device__ __forceinline__ float rotated(const T* x, int d, int rot, const float
   return d < half ? a * c - b * s : b * c + a * s;
 }
 
-// Any sizes: block (token, head).  A query head is turned; for a key or value head the block of a page's first token among the
+// Any sizes (the float32 path and what the variant below does not take): block (token, head).  A query head is turned; for a key or value head the block of a page's first token among the
 // tokens writes all of the page's rows, the others have nothing to do.
 template <typename T>
 __global__ void kv_write_q8_kernel(const WriteArgs a) {
@@ -106,12 +106,287 @@ __global__ void kv_write_q8_kernel(const WriteArgs a) {
   if (threadIdx.x == 0) *sp = now;
 }
 
+
+// bfloat16 heads of 64 or 128, rotated whole or not at all.  A row of a head is D / 16 lanes of 16 values (8 of each half, so that a
+// lane turns its own pairs).  A block takes `span` neighbouring tokens.
+//   Queries (blockIdx.y >= kv_blocks): some heads of those tokens; a lane keeps its table row for all of them.
+//   Keys or values of one kv head: the pages' rows among the tokens, `runs`, reach over the block's edges, so the block reads on to both
+//   sides until the first and the last run end: their largest values then are every block's that shares a run, no block waits for
+//   another, and all compute the same scale (the scale that a page had is a lower bound: reading it after the run's first
+//   block has put the new one there gives the same).  The run's first block brings the page's other rows to a larger scale.
+// What bounds it: a few tokens the chain of loads (slots, rows, scale: three trips), thousands the bytes of qkv once and of the
+// outputs, at 64 tokens a block the rows read twice come out of L1 or L2.
+constexpr int FAST_THREADS = 128, SPAN_MAX = 64;
+
+struct FastArgs {
+  WriteArgs w;
+  const float* part;                  // [splits][T][(H + 2 KVH) D]: the product's partial sums (null: qkv is finished)
+  const bf16* bias;
+  int splits;
+  int span, kv_blocks, q_heads;
+};
+
+// 16 values of a row: 8 at column c1 and 8 at c2 of token t's row of qkv, summed over the splits where it is not finished, and then
+// rounded as the product's own end would have rounded them
+template <bool PART>
+__device__ __forceinline__ void load16(const FastArgs& a, int t, int row_elems, int c1, int c2, float (&x)[16]) {
+  if constexpr (!PART) {
+    const bf16* r = (const bf16*)a.w.qkv + (size_t)t * row_elems;
+    const uint4 u = *reinterpret_cast<const uint4*>(r + c1), v = *reinterpret_cast<const uint4*>(r + c2);
+    const unsigned w[8] = {u.x, u.y, u.z, u.w, v.x, v.y, v.z, v.w};
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      x[2 * i] = __uint_as_float(w[i] << 16);
+      x[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < 16; ++i) x[i] = 0.f;
+    const float* p = a.part + (size_t)t * row_elems;
+    const size_t stride = (size_t)a.w.T * row_elems;
+#pragma unroll 4
+    for (int s = 0; s < a.splits; ++s) {
+#pragma unroll
+      for (int q = 0; q < 4; ++q) {
+        const float4 v = __ldcg(reinterpret_cast<const float4*>(p + s * stride + (q < 2 ? c1 : c2 - 8) + 4 * q));
+        x[4 * q] += v.x;
+        x[4 * q + 1] += v.y;
+        x[4 * q + 2] += v.z;
+        x[4 * q + 3] += v.w;
+      }
+    }
+#pragma unroll
+    for (int i = 0; i < 16; ++i) {
+      if (a.bias != nullptr) x[i] += to_f(a.bias[(i < 8 ? c1 : c2 - 8) + i]);
+      x[i] = round_to<bf16>(x[i]);
+    }
+  }
+}
+__device__ __forceinline__ void load_table(const WriteArgs& a, int t, int half, int j, float (&c)[8], float (&s)[8]) {
+  const size_t at = (size_t)a.positions[t] * half + 8 * j;
+#pragma unroll
+  for (int i = 0; i < 8; i += 4) {
+    const float4 u = *reinterpret_cast<const float4*>(a.cos_t + at + i), v = *reinterpret_cast<const float4*>(a.sin_t + at + i);
+    c[i] = round_to<bf16>(u.x); c[i + 1] = round_to<bf16>(u.y); c[i + 2] = round_to<bf16>(u.z); c[i + 3] = round_to<bf16>(u.w);
+    s[i] = round_to<bf16>(v.x); s[i + 1] = round_to<bf16>(v.y); s[i + 2] = round_to<bf16>(v.z); s[i + 3] = round_to<bf16>(v.w);
+  }
+}
+__device__ __forceinline__ void turn(float (&x)[16], const float (&c)[8], const float (&s)[8]) {
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    const float a = x[i], b = x[8 + i];
+    x[i] = a * c[i] - b * s[i];
+    x[8 + i] = b * c[i] + a * s[i];
+  }
+}
+__device__ __forceinline__ unsigned four_e4m3(float a, float b, float c, float d) {
+  const unsigned lo = __nv_cvt_float2_to_fp8x2(make_float2(a, b), __NV_SATFINITE, __NV_E4M3);
+  const unsigned hi = __nv_cvt_float2_to_fp8x2(make_float2(c, d), __NV_SATFINITE, __NV_E4M3);
+  return lo | hi << 16;
+}
+
+template <int D, bool PART>
+__global__ void __launch_bounds__(FAST_THREADS) kv_write_q8_fast_kernel(const FastArgs f) {
+  pdl_launch_dependents();
+  pdl_wait();
+  constexpr int LPR = D / 16, ROWS = FAST_THREADS / LPR, HALF = D / 2;
+  const WriteArgs& a = f.w;
+  const int tid = threadIdx.x, j = tid % LPR, r = tid / LPR, row_elems = (a.H + 2 * a.KVH) * D;
+  const int w0 = blockIdx.x * f.span, w1 = min(a.T, w0 + f.span);
+  if ((int)blockIdx.y >= f.kv_blocks) {
+    const int h0 = (blockIdx.y - f.kv_blocks) * f.q_heads, h1 = min(a.H, h0 + f.q_heads);
+    const int rows = min(f.span, ROWS), abreast = ROWS / rows;
+    for (int t = w0 + r % rows; t < w1; t += rows) {
+      float c[8], s[8];
+      if (a.rot) load_table(a, t, HALF, j, c, s);
+      bf16* dst = (bf16*)a.q_out + (size_t)t * a.q_stride;
+#pragma unroll 2
+      for (int h = h0 + r / rows; h < h1; h += abreast) {
+        float x[16];
+        load16<PART>(f, t, row_elems, h * D + 8 * j, h * D + HALF + 8 * j, x);
+        if (a.rot) turn(x, c, s);
+        unsigned w[8];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          const __nv_bfloat162 p = __floats2bfloat162_rn(x[2 * i], x[2 * i + 1]);
+          w[i] = *reinterpret_cast<const unsigned*>(&p);
+        }
+        *reinterpret_cast<uint4*>(dst + h * D + 8 * j) = make_uint4(w[0], w[1], w[2], w[3]);
+        *reinterpret_cast<uint4*>(dst + h * D + HALF + 8 * j) = make_uint4(w[4], w[5], w[6], w[7]);
+      }
+    }
+    return;
+  }
+  const int kv = blockIdx.y / a.KVH, kvh = blockIdx.y % a.KVH, lane = tid & 31;
+  __shared__ int slot_s[SPAN_MAX], lead_s[SPAN_MAX], edge_s[2], fresh_s[SPAN_MAX];
+  __shared__ unsigned mask_s[2][2], amax_s[SPAN_MAX];             // leaders, live tokens
+  __shared__ float inv_s[SPAN_MAX];
+  if (tid < SPAN_MAX) {
+    const int t = w0 + tid;
+    slot_s[tid] = t < w1 ? a.slots[t] : -1;
+    fresh_s[tid] = 0;
+    amax_s[tid] = 0;
+  }
+  __syncthreads();
+  if (tid < SPAN_MAX) {
+    const int s = slot_s[tid];
+    int before = tid - 1;
+    while (before >= 0 && slot_s[before] < 0) --before;
+    const bool lead = s >= 0 && (before < 0 || slot_s[before] / a.page != s / a.page);
+    const unsigned leads = __ballot_sync(0xffffffffu, lead), live = __ballot_sync(0xffffffffu, s >= 0);
+    if (lane == 0) {
+      mask_s[0][tid >> 5] = leads;
+      mask_s[1][tid >> 5] = live;
+    }
+  }
+  __syncthreads();
+  const unsigned long long leads = mask_s[0][0] | (unsigned long long)mask_s[0][1] << 32;
+  const unsigned long long live = mask_s[1][0] | (unsigned long long)mask_s[1][1] << 32;
+  if (live == 0) return;
+  const int n_runs = __popcll(leads);
+  auto run_at = [&](int i) { return __popcll(leads & (~0ull >> (63 - i))) - 1; };
+  if (tid < SPAN_MAX && (leads >> tid & 1)) lead_s[run_at(tid)] = tid;
+  if (tid < 64) {
+    // where the first run begins (warp 0) and the last one ends (warp 1): 128 tokens a turn
+    const bool back = tid < 32;
+    const int pg = slot_s[back ? __ffsll((long long)live) - 1 : 63 - __clzll((long long)live)] / a.page;
+    int edge = back ? w0 : w1, at = back ? w0 - 1 : w1;           // tokens [edge of the run]; next token to look at
+    for (;;) {
+      int s[4];
+#pragma unroll
+      for (int u = 0; u < 4; ++u) {
+        const int t = back ? at - (u * 32 + lane) : at + u * 32 + lane;
+        s[u] = t >= 0 && t < a.T ? a.slots[t] : -2;
+      }
+      bool ended = false;
+#pragma unroll
+      for (int u = 0; u < 4 && !ended; ++u) {
+        const unsigned other = __ballot_sync(0xffffffffu, s[u] == -2 || (s[u] >= 0 && s[u] / a.page != pg));
+        unsigned same = __ballot_sync(0xffffffffu, s[u] >= 0 && s[u] / a.page == pg);
+        if (other) same &= (other & (~other + 1)) - 1;            // only those before the first that is not of the run
+        if (same) {
+          const int far = u * 32 + 31 - __clz(same);
+          edge = back ? at - far : at + far + 1;
+        }
+        ended = other != 0;
+      }
+      if (ended) break;
+      at += back ? -128 : 128;
+    }
+    if (lane == 0) edge_s[back ? 0 : 1] = edge;
+  }
+  __syncthreads();
+  const int e0 = edge_s[0], e1 = edge_s[1];
+  const int col = (a.H + kv * a.KVH + kvh) * D + 8 * j;
+  auto slot_of = [&](int t) { return t >= w0 && t < w1 ? slot_s[t - w0] : a.slots[t]; };
+  auto run_of = [&](int t) { return t < w0 ? 0 : (t >= w1 ? n_runs - 1 : run_at(t - w0)); };
+  auto load_row = [&](int t, float (&x)[16]) {
+    load16<PART>(f, t, row_elems, col, col + HALF, x);
+    if (kv == 0 && a.rot) {
+      float c[8], s[8];
+      load_table(a, t, HALF, j, c, s);
+      turn(x, c, s);
+    }
+  };
+  float x[16];
+  for (int base = e0; base < e1; base += ROWS) {                  // (every lane of a warp takes every turn: the maxima are shuffled)
+    const int t = base + r, s = t < e1 ? slot_of(t) : -1;
+    unsigned amax = 0;
+    if (s >= 0) {
+      load_row(t, x);
+#pragma unroll
+      for (int i = 0; i < 16; ++i) amax = max(amax, __float_as_uint(fabsf(x[i])));
+    }
+#pragma unroll
+    for (int o = LPR / 2; o > 0; o >>= 1) amax = max(amax, __shfl_xor_sync(0xffffffffu, amax, o));
+    if (s >= 0 && j == 0) {
+      const int run = run_of(t);
+      atomicMax(&amax_s[run], amax);
+      if (s % a.page == 0) fresh_s[run] = 1;
+    }
+  }
+  __syncthreads();
+  // (a run belongs to the block that has its first token)
+  auto begins_here = [&](int run) { return run > 0 || e0 >= w0; };
+  __shared__ float held_s[SPAN_MAX], now_s[SPAN_MAX];
+  if (tid < n_runs) {
+    const float* sp = a.scale[kv] + (size_t)(slot_s[lead_s[tid]] / a.page) * a.KVH + kvh;
+    const float held = *sp, need = scale_for(amax_s[tid]), now = fresh_s[tid] ? need : larger_scale(held, need);
+    held_s[tid] = held;
+    now_s[tid] = now;
+    inv_s[tid] = inverse_scale(now);
+  }
+  __syncthreads();
+  auto page_rows = [&](int slot) { return a.cache[kv] + ((size_t)(slot / a.page) * a.KVH + kvh) * a.page * D; };
+  for (int run = 0; run < n_runs; ++run) {
+    if (fresh_s[run] || !(now_s[run] > held_s[run]) || !begins_here(run)) continue;         // (uniform over the block)
+    unsigned char* rows = page_rows(slot_s[lead_s[run]]);
+    const float ratio = held_s[run] * inv_s[run];
+    const int first = w0 + lead_s[run], last = run + 1 < n_runs ? w0 + lead_s[run + 1] : e1;
+    for (int row = r; row < a.page; row += ROWS) {
+      bool written = false;
+      for (int t = first; t < last; ++t) {
+        const int s = slot_of(t);
+        written = written || (s >= 0 && s % a.page == row);
+      }
+      if (written) continue;
+      uint4* p = reinterpret_cast<uint4*>(rows + (size_t)row * D + 16 * j);
+      uint4 v = *p;
+      unsigned* w = reinterpret_cast<unsigned*>(&v);
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+        w[i] = four_e4m3(from_e4m3(w[i] & 255) * ratio, from_e4m3(w[i] >> 8 & 255) * ratio, from_e4m3(w[i] >> 16 & 255) * ratio,
+                         from_e4m3(w[i] >> 24) * ratio);
+      *p = v;
+    }
+  }
+  const bool once = e1 - e0 <= ROWS;                              // the rows are still in registers
+  for (int t = once ? e0 + r : w0 + r; t < w1; t += ROWS) {
+    const int s = t >= w0 ? slot_s[t - w0] : -1;
+    if (s < 0) continue;
+    if (!once) load_row(t, x);
+    const float inv = inv_s[run_at(t - w0)];
+    unsigned w[4] = {0, 0, 0, 0};
+    if (inv != 0.f) {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) w[i] = four_e4m3(x[4 * i] * inv, x[4 * i + 1] * inv, x[4 * i + 2] * inv, x[4 * i + 3] * inv);
+    }
+    unsigned char* dst = page_rows(s) + (size_t)(s % a.page) * D + 8 * j;
+    *reinterpret_cast<uint2*>(dst) = make_uint2(w[0], w[1]);
+    *reinterpret_cast<uint2*>(dst + HALF) = make_uint2(w[2], w[3]);
+  }
+  if (tid < n_runs && begins_here(tid)) a.scale[kv][(size_t)(slot_s[lead_s[tid]] / a.page) * a.KVH + kvh] = now_s[tid];
+}
+
+template <int D>
+cudaError_t launch_fast(FastArgs f, cudaStream_t s) {
+  const WriteArgs& a = f.w;
+  constexpr int ROWS = FAST_THREADS / (D / 16);
+  // a token a block while there are few (its page's other rows among the tokens are read by every one of them), then wider spans
+  f.span = a.T <= 64 ? 1 : (a.T <= 1024 ? 16 : SPAN_MAX);
+  f.kv_blocks = a.cache[0] != nullptr ? 2 * a.KVH : 0;
+  // query heads a block: as many as keep about 2,048 threads on every SM, at least one row of lanes each
+  const int least = f.span < ROWS ? ROWS / f.span : 1;
+  const long long lanes = (long long)a.T * (D / 16) * a.H, want = lanes / ((long long)ts_sm_count() * 2048);
+  f.q_heads = (int)(want < least ? least : (want > a.H ? a.H : want));
+  const dim3 grid(ceil_div(a.T, f.span), f.kv_blocks + ceil_div(a.H, f.q_heads)), block(FAST_THREADS);
+  return f.part != nullptr ? ts_launch(kv_write_q8_fast_kernel<D, true>, grid, block, 0, s, f)
+                           : ts_launch(kv_write_q8_fast_kernel<D, false>, grid, block, 0, s, f);
+}
+
 }  // namespace
 
-// qkv [T, (H + 2 KVH) * D], q_out [T, H * D] with rows q_stride elements apart.  k_cache null: queries only.
+static bool write_is_fast(int D, int rot, int dtype) { return dtype == TS_BF16 && (D == 64 || D == 128) && (rot == 0 || rot == D); }
+
+// Whether the write also takes an unfinished product (its partial sums).
+TS_API int ts_rope_kv_write_q8_takes_parts(int D, int rot, int dtype) { return write_is_fast(D, rot, dtype); }
+
+// qkv [T, (H + 2 KVH) * D], q_out [T, H * D] with rows q_stride elements apart.  k_cache null: queries only.  part (float
+// [splits, T, (H + 2 KVH) * D]) set: qkv is the sum of the splits and the bias, rounded, and is not read.
 TS_API int ts_rope_kv_write_q8(void* q_out, long long q_stride, const void* qkv, const int* positions, const float* cos_t,
                                const float* sin_t, void* k_cache, void* v_cache, float* k_scale, float* v_scale,
-                               const int* slots, int T, int H, int KVH, int D, int rot, int page, int dtype, void* stream) {
+                               const int* slots, int T, int H, int KVH, int D, int rot, int page, int dtype, const float* part,
+                               int splits, const void* bias, void* stream) {
   if (T <= 0) return 0;
   if (H <= 0 || KVH <= 0 || D <= 0 || page <= 0 || H + 2 * KVH > 65535)
     TS_REFUSE(TS_ERR_SHAPE, "ts_rope_kv_write_q8: H=%d KVH=%d D=%d page=%d", H, KVH, D, page);
@@ -123,6 +398,16 @@ TS_API int ts_rope_kv_write_q8(void* q_out, long long q_stride, const void* qkv,
   WriteArgs a = {qkv, q_out, q_stride, positions, cos_t, sin_t, {(unsigned char*)k_cache, (unsigned char*)v_cache},
                  {k_scale, v_scale}, slots, T, H, KVH, D, rot, page};
   cudaStream_t s = (cudaStream_t)stream;
+  const bool aligned = (((uintptr_t)qkv | (uintptr_t)q_out | (uintptr_t)cos_t | (uintptr_t)sin_t | (uintptr_t)k_cache | (uintptr_t)v_cache |
+                         (uintptr_t)part) & 15) == 0 && q_stride % 8 == 0;
+  if (write_is_fast(D, rot, dtype) && aligned) {
+    FastArgs f = {a, part, (const bf16*)bias, splits, 0, 0, 0};
+    const cudaError_t e = D == 64 ? launch_fast<64>(f, s) : launch_fast<128>(f, s);
+    if (e != cudaSuccess) TS_REFUSE((int)e, "ts_rope_kv_write_q8: %s", cudaGetErrorString(e));
+    TS_LAUNCH_CHECK();
+  }
+  if (part != nullptr) TS_REFUSE(TS_ERR_UNSUPPORTED, "ts_rope_kv_write_q8: partial sums with head_dim %d, rotary_dim %d or buffers that "
+                                 "are not on 16 bytes", D, rot);
   const dim3 grid(T, k_cache != nullptr ? H + 2 * KVH : H), block(D >= 128 ? 128 : 64);
   if (dtype == TS_F32) ts_launch(kv_write_q8_kernel<float>, grid, block, 0, s, a);
   else ts_launch(kv_write_q8_kernel<bf16>, grid, block, 0, s, a);

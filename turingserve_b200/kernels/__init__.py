@@ -104,7 +104,8 @@ class CudaOps:
             "ts_linear_tc_ex": [P, P, P, P, P, I, I, I, I, I, I, P, P],
             "ts_reduce_rmsnorm": [P, P, I, P, P, P, F, I, I, I, P],
             "ts_feed_tokens": [P, P, P, P, I, I, P],
-            "ts_rope_kv_write_q8": [P, L, P, P, P, P, P, P, P, P, P, I, I, I, I, I, I, I, P],
+            "ts_rope_kv_write_q8": [P, L, P, P, P, P, P, P, P, P, P, I, I, I, I, I, I, I, P, I, P, P],
+            "ts_rope_kv_write_q8_takes_parts": [I, I, I],
             "ts_attention_q8": [P, L, P, L, P, P, P, P, P, P, P, I, I, I, I, I, I, I, F, I, I, P],
             "ts_attention_q8_decode": [P, L, P, L, P, P, P, P, P, P, P, P, I, I, I, I, I, I, I, I, F, I, I, P],
             "ts_attention_q8_decode_supported": [I, I, I, I],
@@ -741,7 +742,8 @@ class CudaOps:
                 raise ValueError("rope_kv_write_q8: an int32 slot for each token")
         self._check(self.lib.ts_rope_kv_write_q8(
             _ptr(q_out), q_out.stride(0), _ptr(qkv), _ptr(positions), _ptr(cos), _ptr(sin), _ptr(k_cache), _ptr(v_cache),
-            _ptr(k_scale), _ptr(v_scale), _ptr(slots), T, H, KVH, D, rotary_dim, page_size, code, self._stream()), "rope_kv_write_q8")
+            _ptr(k_scale), _ptr(v_scale), _ptr(slots), T, H, KVH, D, rotary_dim, page_size, code, None, 0, None, self._stream()),
+            "rope_kv_write_q8")
 
     def attention_q8(self, out, q, k_cache, v_cache, k_scale, v_scale, block_tables, step, KVH: int, page_size: int, scale: float,
                      window) -> None:
