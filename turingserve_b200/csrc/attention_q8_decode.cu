@@ -45,24 +45,6 @@ struct DecArgs {
   int window, nsplit, cluster, early;
 };
 
-__device__ __forceinline__ float ex2_q8(float x) {
-  float y;
-  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-  return y;
-}
-__device__ __forceinline__ unsigned half2_of(unsigned short e4m3x2) {
-  unsigned r;
-  asm("cvt.rn.f16x2.e4m3x2 %0, %1;" : "=r"(r) : "h"(e4m3x2));
-  return r;
-}
-__device__ __forceinline__ void halves_of(unsigned w, unsigned& lo, unsigned& hi) {
-  lo = half2_of((unsigned short)(w & 0xffffu));
-  hi = half2_of((unsigned short)(w >> 16));
-}
-__device__ __forceinline__ unsigned pack_half(float lo, float hi) {
-  const __half2 h = __floats2half2_rn(lo, hi);
-  return *reinterpret_cast<const unsigned*>(&h);
-}
 __device__ __forceinline__ unsigned transpose8x8(unsigned a) {
   unsigned r;
   asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(a));
@@ -167,23 +149,17 @@ __global__ void __launch_bounds__(THREADS) attention_q8_decode_kernel(const DecA
     const bf16* src = a.q + (size_t)row_q * a.q_ts + (size_t)(kvh * G + min(head, G - 1)) * D + 4 * c;
     uint2 raw[KS];
     float amax = 0.f;
-    bool finite = true;
 #pragma unroll
     for (int ks = 0; ks < KS; ++ks) {
       raw[ks] = head < G && n_tiles > 0 ? *reinterpret_cast<const uint2*>(src + ks * 16) : make_uint2(0u, 0u);
       const float2 x = __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&raw[ks].x));
       const float2 y = __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&raw[ks].y));
-      const float m4 = fmaxf(fmaxf(fabsf(x.x), fabsf(x.y)), fmaxf(fabsf(y.x), fabsf(y.y)));
-      amax = fmaxf(amax, m4);
-      finite = finite && x.x - x.x == 0.f && x.y - x.y == 0.f && y.x - y.x == 0.f && y.y - y.y == 0.f;
+      amax = fmaxf(fmaxf(fmaxf(abs_or_inf(x.x), abs_or_inf(x.y)), fmaxf(abs_or_inf(y.x), abs_or_inf(y.y))), amax);
     }
     amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 1));
     amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 2));
-    const unsigned bad = __ballot_sync(0xffffffffu, !finite);
-    const int e = max((int)(__float_as_uint(amax) >> 23) - 127, -110);
-    const float to_half = __uint_as_float((unsigned)(127 + 7 - e) << 23);
-    float f = a.scale * LOG2E_Q8 * __uint_as_float((unsigned)(127 - 7 + e) << 23);
-    if ((bad >> (lane & ~3)) & 0xfu) f = __uint_as_float(NAN_BITS);
+    float f;
+    const float to_half = query_to_half(amax, a.scale * LOG2E_Q8, f);
 #pragma unroll
     for (int ks = 0; ks < KS; ++ks) {
       const float2 x = __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&raw[ks].x));

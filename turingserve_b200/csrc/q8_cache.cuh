@@ -42,4 +42,33 @@ __device__ __forceinline__ float from_e4m3(unsigned char b) {
 // x times 1 / s on its way to 8 bits; a page that reads as NaN stores zeros (x may be infinite: no product then).
 __device__ __forceinline__ unsigned char quantise(float x, float inv) { return inv == 0.f ? 0 : to_e4m3(x * inv); }
 
+// Two e4m3 values as half floats (exact).
+__device__ __forceinline__ unsigned half2_of(unsigned short e4m3x2) {
+  unsigned r;
+  asm("cvt.rn.f16x2.e4m3x2 %0, %1;" : "=r"(r) : "h"(e4m3x2));
+  return r;
+}
+__device__ __forceinline__ void halves_of(unsigned w, unsigned& lo, unsigned& hi) {
+  lo = half2_of((unsigned short)(w & 0xffffu));
+  hi = half2_of((unsigned short)(w >> 16));
+}
+__device__ __forceinline__ unsigned pack_half(float lo, float hi) {
+  const __half2 h = __floats2half2_rn(lo, hi);
+  return *reinterpret_cast<const unsigned*>(&h);
+}
+__device__ __forceinline__ float ex2_q8(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+
+// A query head as half floats: times 2^(7 - e), e the exponent of its largest magnitude, so that a bfloat16 fits whole down to 2^-21
+// of that; a score's factor takes it back.  A head that is not finite gets the factor NaN.
+__device__ __forceinline__ float query_to_half(float amax, float scale, float& factor) {
+  const int e = max((int)(__float_as_uint(amax) >> 23) - 127, -110);
+  factor = amax <= 3.4028235e38f ? scale * __uint_as_float((unsigned)(127 - 7 + e) << 23) : __uint_as_float(NAN_BITS);
+  return __uint_as_float((unsigned)(127 + 7 - e) << 23);
+}
+__device__ __forceinline__ float abs_or_inf(float x) { return x != x ? INFINITY : fabsf(x); }
+
 }  // namespace q8

@@ -109,6 +109,8 @@ class CudaOps:
             "ts_attention_q8": [P, L, P, L, P, P, P, P, P, P, P, I, I, I, I, I, I, I, F, I, I, P],
             "ts_attention_q8_decode": [P, L, P, L, P, P, P, P, P, P, P, P, I, I, I, I, I, I, I, I, F, I, I, P],
             "ts_attention_q8_decode_supported": [I, I, I, I],
+            "ts_attention_q8_prefill": [P, L, P, L, P, P, P, P, P, P, P, I, I, I, I, I, I, I, F, I, P],
+            "ts_attention_q8_prefill_supported": [I, I, I, I, I],
             "ts_step_maps": [P, P, P, P, P, P, P, P, P, I, I, I, I, I, I, I, I, P],
             "ts_sample": [P, P, P, P, I, I, P, P],
             "ts_penalize": [P, P, P, P, I, I, P],
@@ -184,6 +186,8 @@ class CudaOps:
         self.lib.ts_attention_q8_decode_scratch.restype = L
         self.lib.ts_set_q8_decode.argtypes = [I, I]
         self.lib.ts_set_q8_decode.restype = None
+        self.lib.ts_set_q8_prefill.argtypes = [I]
+        self.lib.ts_set_q8_prefill.restype = None
         self.lib.ts_attention_diff_mma_supported.argtypes = [I, I, I, I, I]
         self.lib.ts_attention_diff_mma_supported.restype = c_int
         self.lib.ts_attention_diff_mma_scratch_floats.argtypes = [I, I, I, I]
@@ -782,6 +786,15 @@ class CudaOps:
             nd = 0
         if nd == B:
             return
+        if (self.use_fast_attention and self.use_tc_attention
+                and self.lib.ts_attention_q8_prefill_supported(H, KVH, D, page_size, code)):
+            rc = self.lib.ts_attention_q8_prefill(
+                out.data_ptr(), out.stride(0), q.data_ptr(), q.stride(0), k_cache.data_ptr(), v_cache.data_ptr(), k_scale.data_ptr(),
+                v_scale.data_ptr(), block_tables.data_ptr() + 4 * nd * width, step.q_start.data_ptr() + 4 * nd,
+                step.seq_lens.data_ptr() + 4 * nd, B - nd, width, step.max_q_len, H, KVH, D, page_size, scale, w, self._stream())
+            if rc != self.UNSUPPORTED:
+                self._check(rc, "attention_q8_prefill")
+                return
         self._check(self.lib.ts_attention_q8(
             out.data_ptr(), out.stride(0), q.data_ptr(), q.stride(0), k_cache.data_ptr(), v_cache.data_ptr(), k_scale.data_ptr(),
             v_scale.data_ptr(), block_tables.data_ptr() + 4 * nd * width, step.q_start.data_ptr() + 4 * nd,
