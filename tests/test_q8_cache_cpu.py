@@ -125,3 +125,55 @@ def test_rounding_is_torchs():
     x = torch.cat([torch.randn(4000, dtype=torch.float64, generator=torch.Generator().manual_seed(0)) * s for s in (200.0, 1.0, 0.01, 0.002)])
     x = x.clamp(-448, 448).float()
     assert torch.equal(plain.e4m3(x.double()), x.to(F8).double())
+
+
+# -- the engine's side, without a GPU ---------------------------------------------------------------------------------------
+
+def test_engine_option():
+    from turingserve_b200 import EngineConfig
+    from turingserve_b200.config.engine_config import add_engine_arguments, engine_config_from_namespace
+    import argparse
+
+    assert EngineConfig(model="x").torch_cache_dtype is BF16
+    assert EngineConfig(model="x", dtype="float32").torch_cache_dtype is torch.float32
+    assert EngineConfig(model="x", dtype="float32", kv_cache_dtype="fp8").torch_cache_dtype is F8
+    with pytest.raises(ValueError, match="kv-cache-dtype"):
+        EngineConfig(model="x", kv_cache_dtype="int8").validate()
+    p = argparse.ArgumentParser()
+    add_engine_arguments(p)
+    assert engine_config_from_namespace(p.parse_args(["--model", "x", "--kv-cache-dtype", "fp8"])).kv_cache_dtype == "fp8"
+    assert engine_config_from_namespace(p.parse_args(["--model", "x"])).kv_cache_dtype == "auto"
+
+
+def test_cache_manager_in_8_bits():
+    from turingserve_b200.cache import CacheManager, RunNeeds
+    from turingserve_b200.parts.base import CacheNeed
+    needs = [RunNeeds(CacheNeed(2, 8), None), RunNeeds(CacheNeed(2, 8, 16), None), RunNeeds(CacheNeed(2, 8), None), RunNeeds(None, None, 0)]
+    m = CacheManager(needs, 4, 6, 3, F8, "cpu")
+    v = m.views()
+    assert v[0].k.dtype == F8 and v[0].k.shape == (6, 2, 4, 8) and v[2].v_scale.shape == (6, 2) and v[1].k_scale.shape == (6, 2)
+    assert v[0].k_scale.data_ptr() != v[2].k_scale.data_ptr() != v[2].v_scale.data_ptr()
+    assert v[3].k_scale.data_ptr() == v[0].k_scale.data_ptr() and not v[3].writable
+    assert all(x.k_scale.is_contiguous() and x.k_scale.eq(1).all() for x in v)
+    assert CacheManager(needs, 4, 6, 3, BF16, "cpu").views()[0].k_scale is None
+    with pytest.raises(ValueError, match="one width"):
+        CacheManager([RunNeeds(CacheNeed(1, 8, value_dim=4), None)], 4, 6, 3, F8, "cpu")
+    a, b = m.admit("a"), m.admit("b")
+    m.release(a)
+    assert b.admission != a.admission != m.admit("c").admission
+
+
+def test_models_whose_mixers_keep_the_engines_type_are_refused():
+    from turingserve_b200.engine.runner import check_cache_dtype
+
+    class Mixer:
+        def __init__(self, need, takes):
+            self.takes_q8_cache, self._need = takes, need
+
+        def cache_need(self):
+            return self._need
+    make = lambda *mixers: SimpleNamespace(cfg=SimpleNamespace(schedule=range(len(mixers))), run_mixer=lambda r: mixers[r])  # noqa: E731
+    check_cache_dtype(make(Mixer(1, True), Mixer(None, False)), F8)
+    check_cache_dtype(make(Mixer(1, False)), BF16)
+    with pytest.raises(ValueError, match="Mixer"):
+        check_cache_dtype(make(Mixer(1, True), Mixer(1, False)), F8)

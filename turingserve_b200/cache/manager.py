@@ -5,7 +5,8 @@ Runs of the schedule whose mixers want the same thing from the cache (same kv he
 window and block size) form a GROUP.  A group has its own pool ``[runs, 2, pages, kv_heads, page, head_dim]``
 (where a mixer's value rows are wider or narrower than its key rows: two tensors
 ``[runs, pages, kv_heads, page, head_dim]`` and ``[runs, pages, kv_heads, page, value_dim]``)
-(the reference's single ``[L, 2, NB, KVH, 16, D]`` tensor, turingserve/engine/builder.py:76-80,
+(and, where keys and values are held in 8 bits, scales ``[runs, 2, pages, kv_heads]``, one a page and kv head;
+the reference's single ``[L, 2, NB, KVH, 16, D]`` tensor, turingserve/engine/builder.py:76-80,
 is the one-group case), its own allocator and, per request, its own block table.  Pages go back
 to the group's free list when a request is released, and, in a group with a window (but for first tokens that
 stay visible) or with blocks of positions, as soon as no later position can see them; freed pages are re-issued first-in first-out.
@@ -50,6 +51,8 @@ class CacheView:
     v: torch.Tensor | None
     page_size: int
     writable: bool                  # False when this run reads another run's cache
+    k_scale: torch.Tensor | None = None         # [pages, kv_heads] float32, where the pages hold 8 bits
+    v_scale: torch.Tensor | None = None
 
 
 @dataclass
@@ -61,6 +64,7 @@ class RequestCache:
     tables: list[list[int]]                       # per group: logical page -> physical page (0 = none)
     num_tokens: int = 0                           # tokens whose keys/values are in the cache
     first_live_page: list[int] = field(default_factory=list)   # per group: pages before it were given back
+    admission: int = 0                            # which admission this is, counted from 1: a slot is used again and again
 
 
 class CacheGroup:
@@ -71,12 +75,14 @@ class CacheGroup:
         self.pool: torch.Tensor | None = None           # keys and values of one width
         self.k_pool: torch.Tensor | None = None         # keys and values of two widths
         self.v_pool: torch.Tensor | None = None
+        self.scales: torch.Tensor | None = None         # of a pool that holds 8 bits
 
 
 class CacheManager:
     def __init__(self, needs: list[RunNeeds], page_size: int, num_pages: int, max_requests: int,
                  dtype: torch.dtype = torch.float32, device=None) -> None:
-        """``device`` None keeps the bookkeeping only (no tensors): enough for scheduling tests."""
+        """``device`` None keeps the bookkeeping only (no tensors): enough for scheduling tests.  ``dtype`` is what keys and
+        values are held in; float8_e4m3fn: 8 bits and a scale for each page and kv head (``kernels.rope_kv_write_q8``)."""
         self.page_size = page_size
         self.num_pages = num_pages
         self.max_requests = max_requests
@@ -109,6 +115,10 @@ class CacheManager:
         if device is not None:
             for grp in self.groups:
                 n = grp.need
+                if dtype == torch.float8_e4m3fn:
+                    if n.v_dim != n.head_dim:
+                        raise ValueError("a cache in 8 bits holds keys and values of one width")
+                    grp.scales = torch.ones((len(grp.runs), 2, num_pages, n.num_kv_heads), dtype=torch.float32, device=device)
                 if n.v_dim == n.head_dim:
                     grp.pool = torch.zeros((len(grp.runs), 2, num_pages, n.num_kv_heads, page_size, n.head_dim),
                                            dtype=dtype, device=device)
@@ -123,6 +133,7 @@ class CacheManager:
                                                  device=device)
         self.null_slot = max_requests
         self._free_slots = list(range(max_requests - 1, -1, -1))
+        self._admissions = 0
         self.live: dict[str, RequestCache] = {}
 
     # -- sizing -----------------------------------------------------------------------------------
@@ -130,7 +141,8 @@ class CacheManager:
     def bytes_per_page(needs: list[RunNeeds], page_size: int, dtype: torch.dtype) -> int:
         """Bytes one page index costs across all groups (each group has ``num_pages`` pages)."""
         elem = torch.empty((), dtype=dtype).element_size()
-        return sum(n.cache.num_kv_heads * (n.cache.head_dim + n.cache.v_dim) * page_size * elem
+        scales = 8 if dtype == torch.float8_e4m3fn else 0
+        return sum(n.cache.num_kv_heads * ((n.cache.head_dim + n.cache.v_dim) * page_size * elem + scales)
                    for n in needs if n.cache is not None and n.cache_from is None)
 
     # -- views --------------------------------------------------------------------------------------
@@ -142,12 +154,14 @@ class CacheManager:
             return None
         grp = self.groups[g]
         i = self._run_index_in_group[src]
-        k = v = None
+        k = v = ks = vs = None
+        if grp.scales is not None:
+            ks, vs = grp.scales[i, 0], grp.scales[i, 1]
         if grp.pool is not None:
             k, v = grp.pool[i, 0], grp.pool[i, 1]
         elif grp.k_pool is not None:
             k, v = grp.k_pool[i], grp.v_pool[i]
-        return CacheView(g, k, v, self.page_size, writable=n.cache_from is None)
+        return CacheView(g, k, v, self.page_size, n.cache_from is None, ks, vs)
 
     def views(self) -> list[CacheView | None]:
         return [self.view(r) for r in range(len(self._needs))]
@@ -162,7 +176,8 @@ class CacheManager:
         for st in self.states:
             if st is not None:
                 st[slot].zero_()
-        rc = RequestCache(request_id, slot, [[] for _ in self.groups], 0, [0] * len(self.groups))
+        self._admissions += 1
+        rc = RequestCache(request_id, slot, [[] for _ in self.groups], 0, [0] * len(self.groups), self._admissions)
         self.live[request_id] = rc
         return rc
 

@@ -362,8 +362,9 @@ template <int D>
 cudaError_t launch_fast(FastArgs f, cudaStream_t s) {
   const WriteArgs& a = f.w;
   constexpr int ROWS = FAST_THREADS / (D / 16);
-  // a token a block while there are few (its page's other rows among the tokens are read by every one of them), then wider spans
-  f.span = a.T <= 64 ? 1 : (a.T <= 1024 ? 16 : SPAN_MAX);
+  // spans of as many tokens as a block takes in one turn (no slower than a token a block: its rows lie side by side in the block's
+  // warps), wider where there are blocks enough; every block of a page's rows reads all of them
+  f.span = a.T <= 8 ? 1 : (a.T <= 1024 ? ROWS : SPAN_MAX);
   f.kv_blocks = a.cache[0] != nullptr ? 2 * a.KVH : 0;
   // query heads a block: as many as keep about 2,048 threads on every SM, at least one row of lanes each
   const int least = f.span < ROWS ? ROWS / f.span : 1;

@@ -22,7 +22,7 @@ from turingserve_b200.config.engine_config import EngineConfig
 from turingserve_b200.engine.batch import StepEntry
 from turingserve_b200.engine.request import Request, RequestOutput, Status
 from turingserve_b200.engine.scheduler import Scheduler, StepPlan
-from turingserve_b200.engine.runner import ModelRunner, run_needs
+from turingserve_b200.engine.runner import ModelRunner, check_cache_dtype, run_needs
 
 from turingserve_b200.sampling.params import SamplingParams
 from turingserve_b200.sampling.sampler import Sampler, SampleRow, derive_seed
@@ -101,15 +101,16 @@ class LLMEngine:
         kernels.ops()                                   # build/load the CUDA library; fails loudly
         device = torch.device("cuda", torch.cuda.current_device())
         model, mcfg = load_model(cfg.model, cfg.torch_dtype, device, max_len)
+        check_cache_dtype(model, cfg.torch_cache_dtype)
         needs = run_needs(model)
         num_pages = cfg.num_blocks
         if num_pages is None:
             free, total = torch.cuda.mem_get_info(device)
-            per_page = max(1, CacheManager.bytes_per_page(needs, cfg.block_size, cfg.torch_dtype))
+            per_page = max(1, CacheManager.bytes_per_page(needs, cfg.block_size, cfg.torch_cache_dtype))
             budget = free - (1.0 - cfg.gpu_memory_utilization) * total - (2 << 30)
             wanted = cfg.max_num_seqs * cfg.max_blocks_per_seq(max_len) + 1
             num_pages = int(max(2, min(budget // per_page, wanted)))
-        cache = CacheManager(needs, cfg.block_size, num_pages, cfg.max_num_seqs, cfg.torch_dtype, device)
+        cache = CacheManager(needs, cfg.block_size, num_pages, cfg.max_num_seqs, cfg.torch_cache_dtype, device)
         runner = ModelRunner(model, cache, max(cfg.max_num_batched_tokens, cfg.max_num_seqs),
                              cfg.max_num_seqs, max_len,
                              cfg.graph_batch_sizes if cfg.cuda_graphs else (), cfg.graph_portion_sizes())

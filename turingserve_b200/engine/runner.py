@@ -33,12 +33,23 @@ def run_needs(model: DecoderModel) -> list[RunNeeds]:
     return out
 
 
+def check_cache_dtype(model: DecoderModel, dtype: torch.dtype) -> None:
+    """Refuses a cache in 8 bits for a model with a mixer that reads only caches in the engine's type."""
+    if dtype != torch.float8_e4m3fn:
+        return
+    kinds = sorted({type(m).__name__ for m in (model.run_mixer(r) for r in range(len(model.cfg.schedule)))
+                    if m.cache_need() is not None and not m.takes_q8_cache})
+    if kinds:
+        raise ValueError(f"--kv-cache-dtype fp8: {', '.join(kinds)} keeps its cache in the engine's type")
+
+
 class ModelRunner:
     supports_feedback = True            # entries may take their token id from the previous sampler output
 
     def __init__(self, model: DecoderModel, cache: CacheManager, max_tokens: int, max_requests: int,
                  max_model_len: int, graph_batch_sizes: tuple[int, ...] = (),
                  graph_portion_sizes: tuple[int, ...] = ()) -> None:
+        check_cache_dtype(model, cache.dtype)
         self.model, self.cache = model, cache
         self.max_model_len = max_model_len
         self.max_pages = -(-max_model_len // cache.page_size)

@@ -722,16 +722,15 @@ class CudaOps:
                          k_scale, v_scale, slots, page_size: int) -> None:
         """q_out [T, H D] = the rotated queries of ``qkv`` [T, (H + 2 KVH) D]; the rotated keys and the values go to pages of
         8 bits (float8_e4m3fn [pages, KVH, page, D], scales float32 [pages, KVH]: a power of two per page and kv head,
-        from 2^-50 to 2^50, NaN for a page with a value that is not finite or above 448 * 2^50).  ``qkv`` stays as it is.
-        A page's scale grows with what is written to it, its other rows are brought to the new one; a call that writes the page's
+        from 2^-50 to 2^50, NaN for a page with a value that is not finite or above 448 * 2^50).  ``qkv`` stays as it is (it may
+        be a product that is not finished: the kernel sums it, and finished it is written nowhere).  A page's scale grows with what is written to it, its other rows are brought to the new one; a call that writes the page's
         first row begins the page anew.  The rows of one page stand next to each other among the tokens that are written and no slot
         appears twice.  ``k_cache`` None: queries only; ``slots`` -1: that token is not written."""
+        qkv = self._settle(qkv)
         T, code = qkv.shape[0], _code(qkv.dtype)
         if qkv.shape != (T, (H + 2 * KVH) * D) or q_out.shape != (T, H * D) or q_out.dtype is not qkv.dtype:
             raise ValueError(f"rope_kv_write_q8: [T, {(H + 2 * KVH) * D}] to [T, {H * D}] of one type, not {tuple(qkv.shape)} to "
                              f"{tuple(q_out.shape)}")
-        if not qkv.is_contiguous() or q_out.stride(1) != 1:
-            raise ValueError("rope_kv_write_q8: rows must be contiguous")
         if positions.dtype is not torch.int32 or positions.shape != (T,) or not positions.is_contiguous():
             raise ValueError("rope_kv_write_q8: an int32 position for each token")
         if rotary_dim < 0 or rotary_dim > D or rotary_dim % 2:
@@ -744,10 +743,20 @@ class CudaOps:
             self._check_q8_cache("rope_kv_write_q8", k_cache, v_cache, k_scale, v_scale, KVH, D, page_size, qkv.device)
             if slots is None or slots.dtype is not torch.int32 or slots.shape != (T,) or not slots.is_contiguous():
                 raise ValueError("rope_kv_write_q8: an int32 slot for each token")
+        part, splits, bias = None, 0, None
+        if isinstance(qkv, Deferred):
+            if (self.lib.ts_rope_kv_write_q8_takes_parts(D, rotary_dim, code) and q_out.stride(0) % 8 == 0
+                    and all(t is None or t.data_ptr() % 16 == 0 for t in (q_out, cos, sin, k_cache, v_cache, qkv.part))):
+                part, splits, bias = qkv.part, qkv.splits, qkv.bias
+                qkv = qkv.out
+            else:
+                qkv = self.materialize(qkv)
+        if not qkv.is_contiguous() or q_out.stride(1) != 1:
+            raise ValueError("rope_kv_write_q8: rows must be contiguous")
         self._check(self.lib.ts_rope_kv_write_q8(
             _ptr(q_out), q_out.stride(0), _ptr(qkv), _ptr(positions), _ptr(cos), _ptr(sin), _ptr(k_cache), _ptr(v_cache),
-            _ptr(k_scale), _ptr(v_scale), _ptr(slots), T, H, KVH, D, rotary_dim, page_size, code, None, 0, None, self._stream()),
-            "rope_kv_write_q8")
+            _ptr(k_scale), _ptr(v_scale), _ptr(slots), T, H, KVH, D, rotary_dim, page_size, code, _ptr(part), splits, _ptr(bias),
+            self._stream()), "rope_kv_write_q8")
 
     def attention_q8(self, out, q, k_cache, v_cache, k_scale, v_scale, block_tables, step, KVH: int, page_size: int, scale: float,
                      window) -> None:

@@ -15,6 +15,7 @@ from turingserve_b200.parts.base import BuildContext, CacheNeed, Mixer, ParamSpe
 
 
 class Attention(Mixer):
+    takes_q8_cache = True
     MAX_HEAD_DIM = 256          # the any-size attention kernel's limit; the faster ones take 64 and 128
 
     def __init__(self, spec, ctx: BuildContext) -> None:
@@ -63,6 +64,8 @@ class Attention(Mixer):
         qkv = torch.empty((T, self.q_dim + 2 * self.kv_dim), dtype=x.dtype, device=x.device)
         grp = step.groups[cache.group]
         pos = self.position
+        if cache.k_scale is not None:
+            return self._forward_q8(qkv, x, step, cache, grp)
         qkv = ops.qkv_rope(
             qkv, x, self.w_qkv, self.b_qkv, step.positions, None if pos is None else pos.cos,
             None if pos is None else pos.sin, self.H, self.KVH, self.D, 0 if pos is None else pos.rotary_dim,
@@ -71,6 +74,22 @@ class Attention(Mixer):
         attn = torch.empty((T, self.q_dim), dtype=x.dtype, device=x.device)
         ops.attention(attn, qkv, cache.k, cache.v, grp.block_tables, step, self.H, self.KVH, self.D,
                       cache.page_size, self.scale, self.window)
+        out = torch.empty((T, self.hidden), dtype=x.dtype, device=x.device)
+        return ops.linear(out, attn, self.w_o, self.b_o, may_defer=True)
+
+    def _forward_q8(self, qkv: torch.Tensor, x: torch.Tensor, step, cache, grp) -> torch.Tensor:
+        """The same over a cache in 8 bits: the product, then rotation and write in one kernel (a page's scale is its rows' business, not
+        one token's, so the product's own end cannot write it)."""
+        ops, T, pos = kernels.ops(), x.shape[0], self.position
+        qkv = ops.linear(qkv, x, self.w_qkv, self.b_qkv, may_defer=True)
+        q = torch.empty((T, self.q_dim), dtype=x.dtype, device=x.device)
+        w = cache.writable
+        ops.rope_kv_write_q8(q, qkv, step.positions, None if pos is None else pos.cos, None if pos is None else pos.sin, self.H,
+                             self.KVH, self.D, 0 if pos is None else pos.rotary_dim, cache.k if w else None, cache.v if w else None,
+                             cache.k_scale if w else None, cache.v_scale if w else None, grp.slot_mapping, cache.page_size)
+        attn = torch.empty((T, self.q_dim), dtype=x.dtype, device=x.device)
+        ops.attention_q8(attn, q.view(T, self.H, self.D), cache.k, cache.v, cache.k_scale, cache.v_scale, grp.block_tables, step,
+                         self.KVH, cache.page_size, self.scale, self.window)
         out = torch.empty((T, self.hidden), dtype=x.dtype, device=x.device)
         return ops.linear(out, attn, self.w_o, self.b_o, may_defer=True)
 

@@ -105,6 +105,9 @@ class Norm(Part):
 
 
 class Mixer(Part):
+    # whether it also writes and reads a cache in 8 bits (``CacheView.k_scale`` set)
+    takes_q8_cache = False
+
     def cache_need(self) -> CacheNeed | None:
         return None
 
