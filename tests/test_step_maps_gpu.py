@@ -91,3 +91,67 @@ def test_captured_and_replayed(ops):
         want = plain.maps(req.cpu(), upd.cpu(), start, 16, 2, 30)
         for got, w in zip([*out, tables], want):
             assert torch.equal(got.cpu(), torch.as_tensor(w, dtype=torch.int32).view(got.shape))
+
+
+def test_a_builders_steps_are_the_same_from_the_gpu_and_from_the_host():
+    """Requests that come, grow, are thrown out and come back on other slots; a full group, a window, a window that keeps first tokens;
+    eager steps, and steps padded into an arena of their own; more new pages at once than the arena brings."""
+    import random
+
+    from turingserve_b200 import kernels
+    from turingserve_b200.cache import CacheManager, RunNeeds
+    from turingserve_b200.engine.batch import StepEntry, StepInputBuilder
+    from turingserve_b200.parts.base import CacheNeed
+
+    kernels.use(None)
+    rng = random.Random(3)
+    page, width = 8, 40
+    needs = [RunNeeds(CacheNeed(1, 8), None), RunNeeds(CacheNeed(1, 8, 20), None), RunNeeds(CacheNeed(1, 8, 17, keep_first=9), None)]
+    cache = CacheManager(needs, page, 400, 6, torch.bfloat16, "cuda")
+    on, off = (StepInputBuilder(cache, 90, 7, width, "cuda") for _ in range(2))
+    off.tables, on.device_map_rows = None, 1
+    assert on.tables is not None
+    arenas = [torch.zeros(b.capacity, dtype=torch.int32, device="cuda") for b in (on, off)]
+    live = []
+
+    def compare(entries, **kw):
+        steps = [b.build(entries, arena=a if kw else None, **kw) for b, a in zip((on, off), arenas)]
+        x, y = steps
+        for name in ("input_ids", "positions", "token_request", "q_start", "seq_lens", "state_slots", "sample_rows", "feedback_rows",
+                     "feedback_src"):
+            assert torch.equal(getattr(x, name), getattr(y, name)), name
+        for name in ("num_tokens", "num_requests", "num_decode", "q_lens", "starts", "max_q_len", "max_seq_len", "streaming_decode"):
+            assert getattr(x, name) == getattr(y, name), name
+        assert (x.host_ids is None) == (y.host_ids is None) and (x.host_ids is None or (x.host_ids == y.host_ids).all())
+        for a, b in zip(x.groups, y.groups):
+            assert torch.equal(a.block_tables, b.block_tables) and torch.equal(a.slot_mapping, b.slot_mapping)
+            assert a.table_width == b.table_width and a.block_tables.is_contiguous() and a.slot_mapping.is_contiguous()
+
+    for turn in range(120):
+        on.device_map_rows = rng.choice([1, 1, 1, 4])               # (steps that the host lays out leave the GPU's tables behind)
+        while len(live) < 6 and rng.random() < 0.7:
+            live.append(cache.admit(f"r{turn}-{len(live)}"))
+        entries = []
+        for rc in rng.sample(live, rng.randint(1, len(live))) if live else []:
+            n = 1 if rng.random() < 0.7 else rng.randint(2, 14)
+            if rc.num_tokens + n > page * width:
+                continue
+            entries.append(StepEntry(rc, [rng.randint(0, 99) for _ in range(n)], [n - 1] if rng.random() < 0.8 else [],
+                                     feedback=rng.randint(0, 5) if n == 1 and rng.random() < 0.3 else None))
+        if not entries:
+            continue
+        for e in entries:
+            cache.grow(e.cache, len(e.tokens))
+        if rng.random() < 0.3:
+            on.max_updates = 0 if rng.random() < 0.5 else on.max_updates
+        compare(entries)
+        if sum(len(e.tokens) == 1 for e in entries) + 1 <= 7 - sum(len(e.tokens) != 1 for e in entries):
+            on.device_map_rows = 1
+            compare(entries, fixed_width=width, pad_requests=7 - len(entries))
+        for e in entries:
+            cache.advance(e.cache, len(e.tokens))
+        for rc in list(live):
+            if rng.random() < 0.08 or rc.num_tokens > page * width - 20:
+                live.remove(rc)
+                cache.release(rc)
+    cache.check()

@@ -22,6 +22,7 @@ struct MapArgs {
   const int4* updates;                 // [U]
   int* tables;                         // [G][R][P]
   int *q_start, *seq_lens, *token_request, *positions, *slots, *block_tables;
+  long long slots_g, tables_g;         // elements between the groups of slots and of block_tables
   int B, T, U, G, R, P, W, page;
 };
 
@@ -57,7 +58,7 @@ __global__ void __launch_bounds__(THREADS) step_maps_kernel(const MapArgs a) {
     for (int t = first + tid; t < a.T; t += THREADS) {
       a.token_request[t] = 0;
       a.positions[t] = 0;
-      for (int g = 0; g < a.G; ++g) a.slots[(size_t)g * a.T + t] = -1;
+      for (int g = 0; g < a.G; ++g) a.slots[g * a.slots_g + t] = -1;
     }
     return;
   }
@@ -68,11 +69,11 @@ __global__ void __launch_bounds__(THREADS) step_maps_kernel(const MapArgs a) {
   }
   for (int g = 0; g < a.G; ++g) {
     const int* tab = a.tables + ((size_t)g * a.R + (real ? row : 0)) * a.P;
-    int* bt = a.block_tables + ((size_t)g * a.B + b) * a.W;
+    int* bt = a.block_tables + g * a.tables_g + (size_t)b * a.W;
     for (int i = tid; i < a.W; i += THREADS) bt[i] = (i < live && i < a.P) ? tab[i] : 0;
     for (int i = tid; i < n && first + i < a.T; i += THREADS) {
       const int p = start + i, lp = p / a.page;
-      a.slots[(size_t)g * a.T + first + i] = (real && p >= 0 && lp < a.P) ? tab[lp] * a.page + p % a.page : -1;
+      a.slots[g * a.slots_g + first + i] = (real && p >= 0 && lp < a.P) ? tab[lp] * a.page + p % a.page : -1;
     }
   }
   for (int i = tid; i < n && first + i < a.T; i += THREADS) {
@@ -84,14 +85,14 @@ __global__ void __launch_bounds__(THREADS) step_maps_kernel(const MapArgs a) {
 }  // namespace
 
 TS_API int ts_step_maps(const int* requests, const int* updates, int* tables, int* q_start, int* seq_lens, int* token_request,
-                        int* positions, int* slots, int* block_tables, int B, int T, int U, int G, int R, int P, int W, int page,
-                        void* stream) {
+                        int* positions, int* slots, long long slots_g, int* block_tables, long long tables_g, int B, int T, int U,
+                        int G, int R, int P, int W, int page, void* stream) {
   if (B <= 0) return 0;
   if (T < 0 || U < 0 || G < 0 || R <= 0 || P <= 0 || W < 0 || page <= 0)
     TS_REFUSE(TS_ERR_SHAPE, "ts_step_maps: T=%d U=%d G=%d R=%d P=%d W=%d page=%d", T, U, G, R, P, W, page);
   if (((uintptr_t)updates & 15) != 0) TS_REFUSE(TS_ERR_ALIGN, "ts_step_maps: updates must be 16-byte aligned");
   MapArgs a = {requests, (const int4*)updates, tables, q_start, seq_lens, token_request, positions, slots, block_tables,
-               B, T, U, G, R, P, W, page};
+               slots_g, tables_g, B, T, U, G, R, P, W, page};
   ts_launch(step_maps_kernel, dim3(B + 1), dim3(THREADS), 0, (cudaStream_t)stream, a);
   TS_LAUNCH_CHECK();
 }

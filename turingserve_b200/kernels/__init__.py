@@ -111,7 +111,7 @@ class CudaOps:
             "ts_attention_q8_decode_supported": [I, I, I, I],
             "ts_attention_q8_prefill": [P, L, P, L, P, P, P, P, P, P, P, I, I, I, I, I, I, I, F, I, P],
             "ts_attention_q8_prefill_supported": [I, I, I, I, I],
-            "ts_step_maps": [P, P, P, P, P, P, P, P, P, I, I, I, I, I, I, I, I, P],
+            "ts_step_maps": [P, P, P, P, P, P, P, P, L, P, L, I, I, I, I, I, I, I, I, P],
             "ts_sample": [P, P, P, P, I, I, P, P],
             "ts_penalize": [P, P, P, P, I, I, P],
             "ts_sample_greedy": [P, P, I, I, P, P, P, P],
@@ -818,21 +818,26 @@ class CudaOps:
         the pages of every request, kept on the GPU; ``updates`` [U, 4]: (group, row, index, page) put into the tables first (of
         updates of one place the last holds).  Written: ``q_start`` [B + 1], ``seq_lens`` [B], ``token_request`` and
         ``positions`` [T], ``slot_mapping`` [groups, T] (-1 for padding), ``block_tables`` [groups, B, width] (0 behind a
-        request's last page).  Kernels that read their step's arrays before they wait (``attention``) may not follow without a copy
+        request's last page); the groups of the last two may lie any distance apart.  Kernels that read their step's arrays before they wait (``attention``) may not follow without a copy
         or an event between."""
-        B, T, G = requests.shape[-1], positions.shape[0], tables.shape[0]
-        for name, t, shape in (("requests", requests, (3, B)), ("updates", updates, (updates.shape[0], 4)),
-                               ("tables", tables, (G, *tables.shape[1:3])), ("q_start", q_start, (B + 1,)), ("seq_lens", seq_lens, (B,)),
-                               ("token_request", token_request, (T,)), ("positions", positions, (T,)),
-                               ("slot_mapping", slot_mapping, (G, T)), ("block_tables", block_tables, (G, B, block_tables.shape[-1]))):
-            if t.dtype is not torch.int32 or t.shape != shape or not t.is_contiguous():
-                raise ValueError(f"step_maps: {name} is a contiguous int32 tensor {list(shape)}, not {t.dtype} {list(t.shape)}")
+        B, T, U, i32 = requests.shape[-1], positions.shape[0], updates.shape[0], torch.int32
         if tables.dim() != 3 or page_size < 1:
             raise ValueError("step_maps: tables [groups, rows, pages] of pages of a token or more")
+        G, R, P = tables.shape
+        for name, t, shape in (("requests", requests, (3, B)), ("updates", updates, (U, 4)), ("tables", tables, (G, R, P)),
+                               ("q_start", q_start, (B + 1,)), ("seq_lens", seq_lens, (B,)), ("token_request", token_request, (T,)),
+                               ("positions", positions, (T,))):
+            if t.dtype is not i32 or t.shape != shape or not t.is_contiguous():
+                raise ValueError(f"step_maps: {name} is a contiguous int32 tensor {list(shape)}, not {t.dtype} {list(t.shape)}")
+        W = block_tables.shape[-1]
+        if (slot_mapping.dtype is not i32 or slot_mapping.shape != (G, T) or (T > 1 and slot_mapping.stride(1) != 1)
+                or block_tables.dtype is not i32 or block_tables.shape != (G, B, W) or (W > 1 and block_tables.stride(2) != 1)
+                or (B > 1 and block_tables.stride(1) != W)):
+            raise ValueError(f"step_maps: int32 slots [{G}, {T}] and block tables [{G}, {B}, width], each group contiguous")
         self._check(self.lib.ts_step_maps(
-            _ptr(requests), _ptr(updates), _ptr(tables), _ptr(q_start), _ptr(seq_lens), _ptr(token_request), _ptr(positions),
-            _ptr(slot_mapping), _ptr(block_tables), B, T, updates.shape[0], G, tables.shape[1], tables.shape[2],
-            block_tables.shape[2], page_size, self._stream()), "step_maps")
+            requests.data_ptr(), updates.data_ptr(), tables.data_ptr(), q_start.data_ptr(), seq_lens.data_ptr(), token_request.data_ptr(),
+            positions.data_ptr(), slot_mapping.data_ptr(), slot_mapping.stride(0), block_tables.data_ptr(), block_tables.stride(0), B, T, U,
+            G, R, P, W, page_size, self._stream()), "step_maps")
 
     # -- a residual stream in 32-bit ---------------------------------------------------------------------
     def rmsnorm_stream(self, out, stream, add1, add2, weight, eps: float, first: bool = False, alpha: float = 1.0,

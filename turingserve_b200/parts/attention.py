@@ -64,7 +64,7 @@ class Attention(Mixer):
         qkv = torch.empty((T, self.q_dim + 2 * self.kv_dim), dtype=x.dtype, device=x.device)
         grp = step.groups[cache.group]
         pos = self.position
-        if cache.k_scale is not None:
+        if getattr(cache, "k_scale", None) is not None:
             return self._forward_q8(qkv, x, step, cache, grp)
         qkv = ops.qkv_rope(
             qkv, x, self.w_qkv, self.b_qkv, step.positions, None if pos is None else pos.cos,
