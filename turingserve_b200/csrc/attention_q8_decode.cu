@@ -488,28 +488,9 @@ int clusters_that_fit(int n) {
   return k;
 }
 
-int g_splits = 0, g_cluster = 1;
-
-// Splits of a request's keys and whether they form clusters: (splits, cluster), the same for every call of these sizes.
 template <int D, int NG>
-int plan(int pairs, int reach, int& cluster) {
-  const int slots = prepare_kernel<D, NG>() * ts_sm_count();
-  const int most = reach <= 256 ? 1 : (reach + 255) / 256;       // two tiles a warp at least
-  int n = pairs > 0 ? slots / pairs : 1;
-  n = n < 1 ? 1 : n;
-  n = n > most ? most : n;
-  n = n > 128 ? 128 : n;
-  if (g_splits > 0) n = g_splits;
-  cluster = 0;
-  if (n >= 2 && n <= 8 && g_cluster && ts_clusters_enabled() && clusters_that_fit<D, NG>(n) >= pairs) cluster = 1;
-  return n;
-}
-
-template <int D, int NG>
-int launch(DecArgs a, int reach, cudaStream_t s) {
+int launch(const DecArgs& a, cudaStream_t s) {
   if (prepare_kernel<D, NG>() == 0) TS_REFUSE(TS_ERR_UNSUPPORTED, "ts_attention_q8_decode: the device does not hold a block");
-  a.nsplit = plan<D, NG>(a.B * a.KVH, reach, a.cluster);
-  if (a.nsplit > 1 && !a.cluster && a.part == nullptr) TS_REFUSE(TS_ERR_SHAPE, "ts_attention_q8_decode: %d splits need scratch", a.nsplit);
   cudaError_t e = ts_launch_cluster(attention_q8_decode_kernel<D, NG>, dim3(a.cluster ? a.nsplit : 1, 1, 1), dim3(a.nsplit, a.KVH, a.B),
                                     dim3(THREADS), Stage<D>::SMEM, s, a);
   if (e != cudaSuccess) TS_REFUSE((int)e, "ts_attention_q8_decode: %s", cudaGetErrorString(e));
@@ -522,41 +503,43 @@ int launch(DecArgs a, int reach, cudaStream_t s) {
 
 }  // namespace
 
-TS_API void ts_set_q8_decode(int splits, int cluster) {           // for measurements; 0: by the sizes
-  g_splits = splits < 0 || splits > 128 ? 0 : splits;
-  g_cluster = cluster;
+static bool decode_takes(int H, int KVH, int D) { return KVH > 0 && H % KVH == 0 && H / KVH <= 16 && (D == 64 || D == 128); }
+
+// Blocks of the kernel that an SM holds at once, for groups of G heads of D.
+TS_API int ts_attention_q8_decode_blocks_per_sm(int G, int D) {
+  if (!decode_takes(G, 1, D)) return 0;
+  if (D == 64) return G <= 8 ? prepare_kernel<64, 1>() : prepare_kernel<64, 2>();
+  return G <= 8 ? prepare_kernel<128, 1>() : prepare_kernel<128, 2>();
 }
 
-TS_API int ts_attention_q8_decode_supported(int H, int KVH, int D, int dtype) {
-  return dtype == TS_BF16 && KVH > 0 && H % KVH == 0 && H / KVH <= 16 && (D == 64 || D == 128);
+// Clusters of n blocks (2 to 8) that the device holds at once; 0: none.
+TS_API int ts_attention_q8_decode_clusters(int G, int D, int n) {
+  if (n < 2 || n > 8 || !ts_clusters_enabled() || ts_attention_q8_decode_blocks_per_sm(G, D) == 0) return 0;
+  const int k = D == 64 ? (G <= 8 ? clusters_that_fit<64, 1>(n) : clusters_that_fit<64, 2>(n))
+                        : (G <= 8 ? clusters_that_fit<128, 1>(n) : clusters_that_fit<128, 2>(n));
+  return k < 0 ? 0 : k;
 }
 
-// Floats of scratch that B requests of up to `reach` visible keys take: 0 where the splits need none.
-TS_API long long ts_attention_q8_decode_scratch(int B, int H, int KVH, int D, int reach) {
-  int cluster = 0, n = 1;
-  const int pairs = B * KVH;
-  if (D == 64) n = H / KVH <= 8 ? plan<64, 1>(pairs, reach, cluster) : plan<64, 2>(pairs, reach, cluster);
-  else n = H / KVH <= 8 ? plan<128, 1>(pairs, reach, cluster) : plan<128, 2>(pairs, reach, cluster);
-  return n > 1 && !cluster ? (long long)B * H * n * (D + 2) : 0;
-}
-
-// One query token per request (rows q_start[b]).  reach: the most keys a request sees.  early: index arrays and cache rows before
+// One query token per request (rows q_start[b]).  nsplit: blocks that cut the keys of a (request, kv head) among themselves; cluster: as one
+// cluster (2 to 8 of them), else with B * H * nsplit * (D + 2) floats of scratch.  early: index arrays and cache rows before
 // each request's last page are in place already and are read before the wait for the kernels before.
 TS_API int ts_attention_q8_decode(void* out, long long o_ts, const void* q, long long q_ts, const void* k_cache, const void* v_cache,
                                   const float* k_scale, const float* v_scale, const int* block_tables, const int* q_start,
-                                  const int* seq_lens, float* scratch, int B, int table_width, int reach, int H, int KVH, int D,
+                                  const int* seq_lens, float* scratch, int B, int table_width, int nsplit, int cluster, int H, int KVH, int D,
                                   int page, int num_pages, float scale, int window, int early, void* stream) {
   if (B <= 0) return 0;
-  if (!ts_attention_q8_decode_supported(H, KVH, D, TS_BF16) || page <= 0)
+  if (!decode_takes(H, KVH, D) || page <= 0)
     TS_REFUSE(TS_ERR_UNSUPPORTED, "ts_attention_q8_decode: H=%d KVH=%d D=%d page=%d is not taken by this kernel", H, KVH, D, page);
+  if (nsplit < 1 || nsplit > 128 || (cluster && (nsplit < 2 || nsplit > 8)) || (nsplit > 1 && !cluster && scratch == nullptr))
+    TS_REFUSE(TS_ERR_LIMIT, "ts_attention_q8_decode: %d splits%s", nsplit, cluster ? " as a cluster" : "");
   if (B > 65535 || KVH > 65535) TS_REFUSE(TS_ERR_UNSUPPORTED, "ts_attention_q8_decode: %d requests / %d kv heads", B, KVH);
   if ((((uintptr_t)k_cache | (uintptr_t)v_cache | (uintptr_t)scratch) & 15) != 0 || (((uintptr_t)q | (uintptr_t)out) & 7) != 0 ||
       (q_ts & 3) != 0 || (o_ts & 3) != 0)
     TS_REFUSE(TS_ERR_UNSUPPORTED, "ts_attention_q8_decode: pages on 16 bytes, rows of queries and outputs on 8");
   if ((long long)num_pages * KVH * page > 0x7fffffffLL) TS_REFUSE(TS_ERR_UNSUPPORTED, "ts_attention_q8_decode: a cache of more than 2^31 rows");
   DecArgs a = {(bf16*)out, o_ts, (const bf16*)q, q_ts, {(const unsigned char*)k_cache, (const unsigned char*)v_cache},
-               {k_scale, v_scale}, block_tables, q_start, seq_lens, scratch, B, table_width, H, KVH, page, scale, window, 1, 0, early};
+               {k_scale, v_scale}, block_tables, q_start, seq_lens, scratch, B, table_width, H, KVH, page, scale, window, nsplit, cluster, early};
   cudaStream_t s = (cudaStream_t)stream;
-  if (D == 64) return H / KVH <= 8 ? launch<64, 1>(a, reach, s) : launch<64, 2>(a, reach, s);
-  return H / KVH <= 8 ? launch<128, 1>(a, reach, s) : launch<128, 2>(a, reach, s);
+  if (D == 64) return H / KVH <= 8 ? launch<64, 1>(a, s) : launch<64, 2>(a, s);
+  return H / KVH <= 8 ? launch<128, 1>(a, s) : launch<128, 2>(a, s);
 }

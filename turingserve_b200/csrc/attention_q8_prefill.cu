@@ -455,17 +455,13 @@ cudaError_t launch(const PreArgs& a, int B, int max_q_len, cudaStream_t s) {
 
 TS_API void ts_set_q8_prefill(int row_tiles) { g_row_tiles = row_tiles == 1 || row_tiles == 2 ? row_tiles : 0; }   // for measurements
 
-TS_API int ts_attention_q8_prefill_supported(int H, int KVH, int D, int page, int dtype) {
-  return dtype == TS_BF16 && KVH > 0 && H % KVH == 0 && (D == 64 || D == 128) && page >= 16 && page % 16 == 0;
-}
-
 // Requests of any number of tokens (rows q_start[b] ..).  q, out: rows [H, D] q_ts / o_ts elements apart.
 TS_API int ts_attention_q8_prefill(void* out, long long o_ts, const void* q, long long q_ts, const void* k_cache, const void* v_cache,
                                    const float* k_scale, const float* v_scale, const int* block_tables, const int* q_start,
                                    const int* seq_lens, int B, int table_width, int max_q_len, int H, int KVH, int D, int page,
                                    float scale, int window, void* stream) {
   if (B <= 0 || max_q_len <= 0) return 0;
-  if (!ts_attention_q8_prefill_supported(H, KVH, D, page, TS_BF16))
+  if (KVH <= 0 || H % KVH != 0 || (D != 64 && D != 128) || page < 16 || page % 16 != 0)
     TS_REFUSE(TS_ERR_UNSUPPORTED, "ts_attention_q8_prefill: H=%d KVH=%d D=%d page=%d is not taken by this kernel", H, KVH, D, page);
   if (B > 65535 || KVH > 65535 || (long long)max_q_len * (H / KVH) > 0x7fffff00LL)
     TS_REFUSE(TS_ERR_UNSUPPORTED, "ts_attention_q8_prefill: %d requests of up to %d tokens, %d kv heads", B, max_q_len, KVH);

@@ -107,10 +107,10 @@ class CudaOps:
             "ts_rope_kv_write_q8": [P, L, P, P, P, P, P, P, P, P, P, I, I, I, I, I, I, I, P, I, P, P],
             "ts_rope_kv_write_q8_takes_parts": [I, I, I],
             "ts_attention_q8": [P, L, P, L, P, P, P, P, P, P, P, I, I, I, I, I, I, I, F, I, I, P],
-            "ts_attention_q8_decode": [P, L, P, L, P, P, P, P, P, P, P, P, I, I, I, I, I, I, I, I, F, I, I, P],
-            "ts_attention_q8_decode_supported": [I, I, I, I],
+            "ts_attention_q8_decode": [P, L, P, L, P, P, P, P, P, P, P, P, I, I, I, I, I, I, I, I, I, F, I, I, P],
+            "ts_attention_q8_decode_blocks_per_sm": [I, I],
+            "ts_attention_q8_decode_clusters": [I, I, I],
             "ts_attention_q8_prefill": [P, L, P, L, P, P, P, P, P, P, P, I, I, I, I, I, I, I, F, I, P],
-            "ts_attention_q8_prefill_supported": [I, I, I, I, I],
             "ts_step_maps": [P, P, P, P, P, P, P, P, L, P, L, I, I, I, I, I, I, I, I, P],
             "ts_sample": [P, P, P, P, I, I, P, P],
             "ts_penalize": [P, P, P, P, I, I, P],
@@ -182,10 +182,6 @@ class CudaOps:
             fn = getattr(self.lib, name)
             fn.argtypes = args
             fn.restype = c_int
-        self.lib.ts_attention_q8_decode_scratch.argtypes = [I, I, I, I, I]
-        self.lib.ts_attention_q8_decode_scratch.restype = L
-        self.lib.ts_set_q8_decode.argtypes = [I, I]
-        self.lib.ts_set_q8_decode.restype = None
         self.lib.ts_set_q8_prefill.argtypes = [I]
         self.lib.ts_set_q8_prefill.restype = None
         self.lib.ts_attention_diff_mma_supported.argtypes = [I, I, I, I, I]
@@ -277,6 +273,7 @@ class CudaOps:
         self._buffers: dict[str, torch.Tensor] = {}
         self._outgrown: list[torch.Tensor] = []
         self._decode_slots: dict = {}
+        self._q8_plans: dict = {}
         self.use_fast_attention = True
         self.use_tma_decode = True          # (off after a fault of that kernel)
         self.use_fused_step = True          # a whole decode step as one kernel where the model allows it
@@ -703,20 +700,20 @@ class CudaOps:
 
     # -- a cache in 8 bits -------------------------------------------------------------------------------------
     @staticmethod
-    def _check_q8_cache(what: str, k_cache, v_cache, k_scale, v_scale, KVH: int, D: int, page_size: int, device) -> None:
-        pages = None
-        for c, s in ((k_cache, k_scale), (v_cache, v_scale)):
-            if c is None or s is None:
-                raise ValueError(f"{what}: keys and values come together, each with its scales")
-            if c.dtype is not torch.float8_e4m3fn or s.dtype is not torch.float32:
-                raise TypeError(f"{what}: keys and values in float8_e4m3fn with float32 scales, not {c.dtype} with {s.dtype}")
-            n = c.shape[0] if pages is None else pages
-            if c.shape != (n, KVH, page_size, D) or s.shape != (n, KVH) or not c.is_contiguous() or not s.is_contiguous():
-                raise ValueError(f"{what}: contiguous pages [n, {KVH}, {page_size}, {D}] with scales [n, {KVH}], not {tuple(c.shape)} "
-                                 f"with {tuple(s.shape)}")
-            if c.device != device or s.device != device:
-                raise ValueError(f"{what}: pages and scales must be on the tokens' device")
-            pages = n
+    def _check_q8_cache(what: str, k_cache, v_cache, k_scale, v_scale, KVH: int, D: int, page_size: int, device: int) -> None:
+        if k_cache is None or v_cache is None or k_scale is None or v_scale is None:
+            raise ValueError(f"{what}: keys and values come together, each with its scales")
+        f8, f32, n = torch.float8_e4m3fn, torch.float32, k_cache.shape[0]
+        if k_cache.dtype is not f8 or v_cache.dtype is not f8 or k_scale.dtype is not f32 or v_scale.dtype is not f32:
+            raise TypeError(f"{what}: keys and values in float8_e4m3fn with float32 scales, not {k_cache.dtype}, {v_cache.dtype} with "
+                            f"{k_scale.dtype}, {v_scale.dtype}")
+        pages, scales = (n, KVH, page_size, D), (n, KVH)
+        if (k_cache.shape != pages or v_cache.shape != pages or k_scale.shape != scales or v_scale.shape != scales
+                or not (k_cache.is_contiguous() and v_cache.is_contiguous() and k_scale.is_contiguous() and v_scale.is_contiguous())):
+            raise ValueError(f"{what}: contiguous pages [n, {KVH}, {page_size}, {D}] with scales [n, {KVH}], not {tuple(k_cache.shape)}, "
+                             f"{tuple(v_cache.shape)} with {tuple(k_scale.shape)}, {tuple(v_scale.shape)}")
+        if not k_cache.get_device() == v_cache.get_device() == k_scale.get_device() == v_scale.get_device() == device:
+            raise ValueError(f"{what}: pages and scales must be on the tokens' device")
 
     def rope_kv_write_q8(self, q_out, qkv, positions, cos, sin, H: int, KVH: int, D: int, rotary_dim: int, k_cache, v_cache,
                          k_scale, v_scale, slots, page_size: int) -> None:
@@ -726,25 +723,27 @@ class CudaOps:
         be a product that is not finished: the kernel sums it, and finished it is written nowhere).  A page's scale grows with what is written to it, its other rows are brought to the new one; a call that writes the page's
         first row begins the page anew.  The rows of one page stand next to each other among the tokens that are written and no slot
         appears twice.  ``k_cache`` None: queries only; ``slots`` -1: that token is not written."""
-        qkv = self._settle(qkv)
-        T, code = qkv.shape[0], _code(qkv.dtype)
-        if qkv.shape != (T, (H + 2 * KVH) * D) or q_out.shape != (T, H * D) or q_out.dtype is not qkv.dtype:
-            raise ValueError(f"rope_kv_write_q8: [T, {(H + 2 * KVH) * D}] to [T, {H * D}] of one type, not {tuple(qkv.shape)} to "
-                             f"{tuple(q_out.shape)}")
-        if positions.dtype is not torch.int32 or positions.shape != (T,) or not positions.is_contiguous():
+        finished, part, splits, bias = isinstance(qkv, torch.Tensor), None, 0, None
+        if not finished:
+            qkv = self._settle(qkv)
+        T, n, code, i32 = q_out.shape[0], (H + 2 * KVH) * D, _DTYPE_CODE.get(q_out.dtype), torch.int32
+        if code is None or qkv.dtype is not q_out.dtype or qkv.shape != (T, n) or q_out.shape != (T, H * D):
+            raise ValueError(f"rope_kv_write_q8: [T, {n}] to [T, {H * D}] of one type, float32 or bfloat16, not {tuple(qkv.shape)} "
+                             f"{qkv.dtype} to {tuple(q_out.shape)} {q_out.dtype}")
+        if positions.dtype is not i32 or positions.shape != (T,) or not positions.is_contiguous():
             raise ValueError("rope_kv_write_q8: an int32 position for each token")
-        if rotary_dim < 0 or rotary_dim > D or rotary_dim % 2:
-            raise ValueError(f"rope_kv_write_q8: rotary_dim {rotary_dim} for head_dim {D}")
         if rotary_dim:
-            for t in (cos, sin):
-                if t is None or t.dtype is not torch.float32 or t.shape[-1] != rotary_dim // 2 or not t.is_contiguous():
-                    raise ValueError(f"rope_kv_write_q8: float32 tables [positions, {rotary_dim // 2}]")
+            half = rotary_dim // 2
+            if rotary_dim < 0 or rotary_dim > D or rotary_dim % 2:
+                raise ValueError(f"rope_kv_write_q8: rotary_dim {rotary_dim} for head_dim {D}")
+            if (cos is None or sin is None or cos.dtype is not torch.float32 or sin.dtype is not torch.float32 or cos.shape[-1] != half
+                    or sin.shape[-1] != half or not (cos.is_contiguous() and sin.is_contiguous())):
+                raise ValueError(f"rope_kv_write_q8: float32 tables [positions, {half}]")
         if k_cache is not None:
-            self._check_q8_cache("rope_kv_write_q8", k_cache, v_cache, k_scale, v_scale, KVH, D, page_size, qkv.device)
-            if slots is None or slots.dtype is not torch.int32 or slots.shape != (T,) or not slots.is_contiguous():
+            self._check_q8_cache("rope_kv_write_q8", k_cache, v_cache, k_scale, v_scale, KVH, D, page_size, q_out.get_device())
+            if slots is None or slots.dtype is not i32 or slots.shape != (T,) or not slots.is_contiguous():
                 raise ValueError("rope_kv_write_q8: an int32 slot for each token")
-        part, splits, bias = None, 0, None
-        if isinstance(qkv, Deferred):
+        if not finished and isinstance(qkv, Deferred):
             if (self.lib.ts_rope_kv_write_q8_takes_parts(D, rotary_dim, code) and q_out.stride(0) % 8 == 0
                     and all(t is None or t.data_ptr() % 16 == 0 for t in (q_out, cos, sin, k_cache, v_cache, qkv.part))):
                 part, splits, bias = qkv.part, qkv.splits, qkv.bias
@@ -753,62 +752,77 @@ class CudaOps:
                 qkv = self.materialize(qkv)
         if not qkv.is_contiguous() or q_out.stride(1) != 1:
             raise ValueError("rope_kv_write_q8: rows must be contiguous")
+        if k_cache is None:
+            pages = (None,) * 5
+        else:
+            pages = (k_cache.data_ptr(), v_cache.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr(), slots.data_ptr())
         self._check(self.lib.ts_rope_kv_write_q8(
-            _ptr(q_out), q_out.stride(0), _ptr(qkv), _ptr(positions), _ptr(cos), _ptr(sin), _ptr(k_cache), _ptr(v_cache),
-            _ptr(k_scale), _ptr(v_scale), _ptr(slots), T, H, KVH, D, rotary_dim, page_size, code, _ptr(part), splits, _ptr(bias),
-            self._stream()), "rope_kv_write_q8")
+            q_out.data_ptr(), q_out.stride(0), qkv.data_ptr(), positions.data_ptr(), _ptr(cos), _ptr(sin), *pages, T, H, KVH, D,
+            rotary_dim, page_size, code, _ptr(part), splits, _ptr(bias), self._stream()), "rope_kv_write_q8")
+
+    # the most blocks that cut the keys of one (request, kv head) among themselves (0: by the sizes), whether as clusters
+    q8_splits, q8_clusters = 0, True
+
+    def _q8_plan(self, pairs: int, G: int, D: int, reach: int) -> tuple[int, bool]:
+        """(blocks a (request, kv head), as one cluster) of the single tokens' attention: as many blocks as the chip holds at once, with
+        two tiles of 32 keys or more for each of a block's four warps; a cluster where at most 8 are wanted and all of them fit."""
+        key = (G > 8, D)
+        plan = self._q8_plans.get(key)
+        if plan is None:
+            fits = [0, 0] + [self.lib.ts_attention_q8_decode_clusters(G, D, n) for n in range(2, 9)]
+            plan = self._q8_plans[key] = (self.num_sms * self.lib.ts_attention_q8_decode_blocks_per_sm(G, D), fits)
+        n = self.q8_splits or max(1, min(plan[0] // pairs, -(-reach // 256), 128))
+        return n, 2 <= n <= 8 and self.q8_clusters and plan[1][n] >= pairs
 
     def attention_q8(self, out, q, k_cache, v_cache, k_scale, v_scale, block_tables, step, KVH: int, page_size: int, scale: float,
                      window) -> None:
         """out [T, H D] = attention of q [T, H, D] (a view with contiguous heads) over pages of 8 bits as ``rope_kv_write_q8``
         writes them: causal, with a ``window`` (None or 0: none) over the last that many keys.  The first
         ``step.num_decode`` requests bring one token each.  A row that sees a page whose scale is NaN gives NaN."""
-        (T, H, D), code = q.shape, _code(q.dtype)
+        (T, H, D), code, B = q.shape, _DTYPE_CODE.get(q.dtype), step.num_requests
         if KVH <= 0 or H % KVH:
             raise ValueError(f"attention_q8: {H} heads over {KVH} kv heads")
-        if q.stride(2) != 1 or q.stride(1) != D or out.shape != (T, H * D) or out.stride(1) != 1 or out.dtype is not q.dtype:
-            raise ValueError("attention_q8: rows of contiguous heads, outputs [T, H D] in the queries' type")
-        B = step.num_requests
+        q_ts, hs, one = q.stride()
+        if (code is None or one != 1 or (hs != D and H > 1) or out.dtype is not q.dtype or out.shape != (T, H * D)
+                or out.stride(1) != 1):
+            raise ValueError("attention_q8: rows of contiguous heads, float32 or bfloat16, outputs [T, H D] in the queries' type")
         if block_tables.dtype is not torch.int32 or not block_tables.is_contiguous() or block_tables.shape[0] < B:
             raise ValueError("attention_q8: an int32 block table for each request, rows contiguous")
-        self._check_q8_cache("attention_q8", k_cache, v_cache, k_scale, v_scale, KVH, D, page_size, q.device)
-        w = 0 if window is None else int(window)
+        self._check_q8_cache("attention_q8", k_cache, v_cache, k_scale, v_scale, KVH, D, page_size, q.get_device())
+        w = int(window) if window else 0
         if w < 0:
             raise ValueError(f"attention_q8: a window of {w} keys")
-        nd, width, max_seq = step.num_decode, block_tables.shape[1], step.max_seq_len
-        if nd and self.use_fast_attention and self.lib.ts_attention_q8_decode_supported(H, KVH, D, code):
-            reach = min(max_seq, w) if w else max_seq
-            need = self.lib.ts_attention_q8_decode_scratch(nd, H, KVH, D, reach)
-            # (a work buffer of this call's own: calls on two streams, or in two captured graphs, do not meet in it)
-            scratch = torch.empty(need, dtype=torch.float32, device=q.device) if need else None
+        G, nd, width, stream = H // KVH, 0, block_tables.shape[1], self._stream()
+        o_ptr, o_ts, q_ptr, tables, q_start, seq_lens = (out.data_ptr(), out.stride(0), q.data_ptr(), block_tables.data_ptr(),
+                                                         step.q_start.data_ptr(), step.seq_lens.data_ptr())
+        pages = (k_cache.data_ptr(), v_cache.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr())
+        fast = self.use_fast_attention and code == 1 and (D == 128 or D == 64)
+        if fast and G <= 16 and step.num_decode:
+            nd, reach = step.num_decode, step.max_seq_len
+            splits, cluster = self._q8_plan(nd * KVH, G, D, min(reach, w) if w else reach)
+            scratch = None
+            if splits > 1 and not cluster:
+                # (of this call's own: calls on two streams, or in two captured graphs, do not meet in it)
+                scratch = torch.empty(nd * H * splits * (D + 2), dtype=torch.float32, device=q.device)
+                self.launches += 1
             rc = self.lib.ts_attention_q8_decode(
-                out.data_ptr(), out.stride(0), q.data_ptr(), q.stride(0), k_cache.data_ptr(), v_cache.data_ptr(), k_scale.data_ptr(),
-                v_scale.data_ptr(), block_tables.data_ptr(), step.q_start.data_ptr(), step.seq_lens.data_ptr(), _ptr(scratch), nd, width,
-                reach, H, KVH, D, page_size, k_cache.shape[0], scale, w, 1 if getattr(step, "settled", False) else 0, self._stream())
+                o_ptr, o_ts, q_ptr, q_ts, *pages, tables, q_start, seq_lens, _ptr(scratch), nd, width, splits, cluster, H, KVH, D,
+                page_size, k_cache.shape[0], scale, w, getattr(step, "settled", False), stream)
             if rc == self.UNSUPPORTED:
                 nd = 0
             else:
                 self._check(rc, "attention_q8_decode")
-                if need:
-                    self.launches += 1
-        else:
-            nd = 0
-        if nd == B:
-            return
-        if (self.use_fast_attention and self.use_tc_attention
-                and self.lib.ts_attention_q8_prefill_supported(H, KVH, D, page_size, code)):
-            rc = self.lib.ts_attention_q8_prefill(
-                out.data_ptr(), out.stride(0), q.data_ptr(), q.stride(0), k_cache.data_ptr(), v_cache.data_ptr(), k_scale.data_ptr(),
-                v_scale.data_ptr(), block_tables.data_ptr() + 4 * nd * width, step.q_start.data_ptr() + 4 * nd,
-                step.seq_lens.data_ptr() + 4 * nd, B - nd, width, step.max_q_len, H, KVH, D, page_size, scale, w, self._stream())
+                if nd == B:
+                    return
+        where = (tables + 4 * nd * width, q_start + 4 * nd, seq_lens + 4 * nd)
+        if fast and self.use_tc_attention and page_size % 16 == 0:
+            rc = self.lib.ts_attention_q8_prefill(o_ptr, o_ts, q_ptr, q_ts, *pages, *where, B - nd, width, step.max_q_len, H, KVH, D,
+                                                  page_size, scale, w, stream)
             if rc != self.UNSUPPORTED:
                 self._check(rc, "attention_q8_prefill")
                 return
-        self._check(self.lib.ts_attention_q8(
-            out.data_ptr(), out.stride(0), q.data_ptr(), q.stride(0), k_cache.data_ptr(), v_cache.data_ptr(), k_scale.data_ptr(),
-            v_scale.data_ptr(), block_tables.data_ptr() + 4 * nd * width, step.q_start.data_ptr() + 4 * nd,
-            step.seq_lens.data_ptr() + 4 * nd, B - nd, width, step.max_q_len, H, KVH, D, page_size, float(scale), w, code,
-            self._stream()), "attention_q8")
+        self._check(self.lib.ts_attention_q8(o_ptr, o_ts, q_ptr, q_ts, *pages, *where, B - nd, width, step.max_q_len, H, KVH, D, page_size,
+                                             scale, w, code, stream), "attention_q8")
 
     # -- a step's maps -----------------------------------------------------------------------------------------
     def step_maps(self, requests, updates, tables, page_size: int, q_start, seq_lens, token_request, positions, slot_mapping,
@@ -820,24 +834,28 @@ class CudaOps:
         ``positions`` [T], ``slot_mapping`` [groups, T] (-1 for padding), ``block_tables`` [groups, B, width] (0 behind a
         request's last page); the groups of the last two may lie any distance apart.  Kernels that read their step's arrays before they wait (``attention``) may not follow without a copy
         or an event between."""
-        B, T, U, i32 = requests.shape[-1], positions.shape[0], updates.shape[0], torch.int32
-        if tables.dim() != 3 or page_size < 1:
-            raise ValueError("step_maps: tables [groups, rows, pages] of pages of a token or more")
-        G, R, P = tables.shape
-        for name, t, shape in (("requests", requests, (3, B)), ("updates", updates, (U, 4)), ("tables", tables, (G, R, P)),
-                               ("q_start", q_start, (B + 1,)), ("seq_lens", seq_lens, (B,)), ("token_request", token_request, (T,)),
-                               ("positions", positions, (T,))):
-            if t.dtype is not i32 or t.shape != shape or not t.is_contiguous():
-                raise ValueError(f"step_maps: {name} is a contiguous int32 tensor {list(shape)}, not {t.dtype} {list(t.shape)}")
-        W = block_tables.shape[-1]
-        if (slot_mapping.dtype is not i32 or slot_mapping.shape != (G, T) or (T > 1 and slot_mapping.stride(1) != 1)
-                or block_tables.dtype is not i32 or block_tables.shape != (G, B, W) or (W > 1 and block_tables.stride(2) != 1)
-                or (B > 1 and block_tables.stride(1) != W)):
-            raise ValueError(f"step_maps: int32 slots [{G}, {T}] and block tables [{G}, {B}, width], each group contiguous")
+        i32 = torch.int32
+        if tables.dim() != 3 or page_size < 1 or not tables.is_contiguous():
+            raise ValueError("step_maps: contiguous tables [groups, rows, pages] of pages of a token or more")
+        B, T, U, (G, R, P), W = requests.shape[-1], positions.shape[0], updates.shape[0], tables.shape, block_tables.shape[-1]
+        if (requests.dtype is not i32 or updates.dtype is not i32 or tables.dtype is not i32 or q_start.dtype is not i32
+                or seq_lens.dtype is not i32 or token_request.dtype is not i32 or positions.dtype is not i32
+                or slot_mapping.dtype is not i32 or block_tables.dtype is not i32):
+            raise ValueError("step_maps: all tensors are int32")
+        if (requests.shape != (3, B) or updates.shape != (U, 4) or q_start.shape != (B + 1,) or seq_lens.shape != (B,)
+                or token_request.shape != (T,) or positions.shape != (T,) or slot_mapping.shape != (G, T) or block_tables.shape != (G, B, W)
+                or not (requests.is_contiguous() and updates.is_contiguous() and q_start.is_contiguous() and seq_lens.is_contiguous()
+                        and token_request.is_contiguous() and positions.is_contiguous())):
+            raise ValueError(f"step_maps: contiguous requests [3, B], updates [U, 4], q_start [B + 1], seq_lens [B], token_request and "
+                             f"positions [T], slots [{G}, T], block tables [{G}, B, width]")
+        s_g, s_t = slot_mapping.stride()
+        t_g, t_b, t_w = block_tables.stride()
+        if (s_t != 1 and T > 1) or (t_w != 1 and W > 1) or (t_b != W and B > 1):
+            raise ValueError("step_maps: each group's slots and block tables are contiguous")
         self._check(self.lib.ts_step_maps(
             requests.data_ptr(), updates.data_ptr(), tables.data_ptr(), q_start.data_ptr(), seq_lens.data_ptr(), token_request.data_ptr(),
-            positions.data_ptr(), slot_mapping.data_ptr(), slot_mapping.stride(0), block_tables.data_ptr(), block_tables.stride(0), B, T, U,
-            G, R, P, W, page_size, self._stream()), "step_maps")
+            positions.data_ptr(), slot_mapping.data_ptr(), s_g, block_tables.data_ptr(), t_g, B, T, U, G, R, P, W, page_size,
+            self._stream()), "step_maps")
 
     # -- a residual stream in 32-bit ---------------------------------------------------------------------
     def rmsnorm_stream(self, out, stream, add1, add2, weight, eps: float, first: bool = False, alpha: float = 1.0,
