@@ -6,19 +6,24 @@
 // scaled by a power of two a row, P below 2^8.  The scales are constants of 16 keys, so a score costs one fused multiply-add as it would
 // without them, and a sum one more for 16 weights.
 //
-// One block = NR tiles of 128 query rows (a row is a (token, head-in-group) pair of one kv head) over the same keys, 64 a turn.
-// Softmax warps: eight a row tile, row r = tensor-memory lane r belongs to two threads, each half of a turn's keys; they exchange their
-// maxima through shared memory once a turn.  One warp issues the products (one lane): S(t) = Q K(t)^T into one of two buffers, two
-// turns ahead; O += P(t) V(t), P read from tensor memory where it lies over its own scores.  Four warps turn the pages' bytes into
-// half floats, two the keys and two the values: 16 bytes a load, a turn's loads in flight while the turn before is converted, stored with
-// the 128-byte swizzle that the products read (values with keys along the rows: MN-major).  Rows outside the visible range are zeros.
-// With NR = 2 a converted tile serves 256 rows: the conversion is half as much work beside each row's exponentials, and one block fills
-// an SM; NR = 1 is for launches of few row tiles, which are as slow as their longest block.
+// One block = NR tiles of 128 query rows (a row is a (token, head-in-group) pair of one kv head) over the same keys, 128 a turn.
+// Softmax: four warps a row tile, a thread a row = tensor-memory lane.  It reads its scores twice: for the maximum (the scale of 16 keys is
+// one factor, so that is the maximum of the products, three at a time, and one multiply-add), then 32 at a time for the weights, which
+// go back over scores already read as pairs of half floats.  One warp issues the products (one lane): S(t) = Q K(t)^T, O += P(t) V(t) with
+// P read from tensor memory.  Four warps turn the pages' bytes into half floats, two the keys and two the values: 16 bytes a piece, brought
+// by cp.async to a place that its thread alone reads, 128 rows and more ahead of the conversion, stored with the 128-byte swizzle that the products read (values with keys along
+// the rows: MN-major).  Rows outside the visible range are zeros.
+// NR = 2: a score buffer each, so that the softmax of one row tile runs beside the products of the other; a converted tile serves 256 rows;
+// tensor memory is full and a block fills an SM.  NR = 1, for launches of few row tiles, which are as slow as their longest block: two score
+// buffers, products two turns ahead.
 // The reference M moves only when a row's maximum has grown by more than 2^8 since: then O is rescaled in tensor memory.  Every wait is
 // bounded; a block that gives up records where, stops, and frees its tensor memory.
 //
 // NaN: a page whose scale is NaN (either) gives NaN scores, which the rows that do not see it drop by selection; its values are
 // finite bytes (writes store zeros under such a scale), so zero weights stay zeros.
+#include <type_traits>
+
+#include "mma_utils.cuh"
 #include "q8_cache.cuh"
 #include "tc_utils.cuh"
 
@@ -26,21 +31,25 @@ namespace {
 
 using namespace tc;
 
-constexpr int TQ = 128, TK = 64, STAGES = 2, SCALE_STAGES = 4, CONV_WARPS = 4;
+constexpr int TQ = 128, TK = 128, UNIT = 64, STAGES = 2, SCALE_STAGES = 4, CONV_WARPS = 4;
 constexpr float RESCALE_STEP = 8.f;
 constexpr float LOG2E_P = 1.4426950408889634f;
 
 template <int HD, int NR>
 struct Shape {
-  static constexpr int SOFT_WARPS = 8 * NR, MMA_WARP = SOFT_WARPS, CONV_WARP = MMA_WARP + 1;
+  static constexpr int NB = NR == 1 ? 2 : 1;                       // score buffers of a row tile
+  static constexpr int SOFT_WARPS = 4 * NR, MMA_WARP = SOFT_WARPS, CONV_WARP = MMA_WARP + 1;
   static constexpr int THREADS = (SOFT_WARPS + 1 + CONV_WARPS) * 32;
   static constexpr uint32_t Q_BYTES = TQ * HD * 2, KV_BYTES = TK * HD * 2, HALF_Q = TQ * 128, HALF_K = TK * 128;
-  static constexpr uint32_t ROW_COLS = 2 * TK + HD;                // tensor-memory columns of a row tile: two score buffers, O
+  static constexpr uint32_t O_COL = NB * TK, ROW_COLS = O_COL + HD; // tensor-memory columns of a row tile: scores, O
   static constexpr uint32_t TMEM_COLS = ROW_COLS * NR <= 256 ? 256 : 512;
-  // behind the tiles: barriers, the tensor memory's address, the abort flag, maxima [NR][2][128], scales [4][4] float4
-  static constexpr int BARS = 4 * STAGES + NR * (2 + 2 + 1 + 1 + 4 + 4);
-  static constexpr size_t TILES = NR * Q_BYTES + 2 * STAGES * KV_BYTES;
-  static constexpr size_t SMEM = TILES + BARS * 8 + 16 + NR * 2 * TQ * 4 + SCALE_STAGES * 4 * 16 + 16;
+  static constexpr int BARS = 4 * STAGES + NR * (2 * NB + 2) + 1;
+  // rows on their way from the pages: so many times 64 ahead of the conversion
+  static constexpr int AHEAD = NR == 2 && HD == 128 ? 2 : 4;
+  static constexpr uint32_t RAW_BYTES = UNIT * HD;
+  static constexpr size_t TILES = NR * Q_BYTES + 2 * STAGES * KV_BYTES + 2 * AHEAD * RAW_BYTES;
+  // behind the tiles: scales [4][8] float4, scales on their way [AHEAD][2][4], barriers, the tensor memory's address, the abort flag
+  static constexpr size_t SMEM = TILES + SCALE_STAGES * (TK / 16) * 16 + AHEAD * 32 + BARS * 8 + 16;
 };
 
 struct PreArgs {
@@ -64,63 +73,66 @@ __host__ __device__ constexpr uint32_t instr_half(int n, bool b_mn) {
   return (1u << 4) | ((b_mn ? 1u : 0u) << 16) | ((uint32_t)(n >> 3) << 17) | ((uint32_t)(128 >> 4) << 24);
 }
 
+// The largest of three.
+__device__ __forceinline__ float max3(float x, float y, float z) {
+  float r;
+  asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(x), "f"(y), "f"(z));
+  return r;
+}
+
 template <int HD, int NR>
 __global__ void __launch_bounds__(Shape<HD, NR>::THREADS, 1) attention_q8_prefill_kernel(const PreArgs a) {
   using SH = Shape<HD, NR>;
-  constexpr uint32_t KV_BYTES = SH::KV_BYTES, HALF_K = SH::HALF_K, HALF_Q = SH::HALF_Q, ROW_COLS = SH::ROW_COLS, O_COL = 2 * TK;
-  constexpr int HC = HD / 2, ROWS = NR * TQ, KT = TK / 2;
+  constexpr uint32_t KV_BYTES = SH::KV_BYTES, HALF_K = SH::HALF_K, HALF_Q = SH::HALF_Q, ROW_COLS = SH::ROW_COLS, O_COL = SH::O_COL;
+  constexpr int ROWS = NR * TQ, NB = SH::NB, GROUPS = TK / 16;
   pdl_launch_dependents();
   extern __shared__ __align__(1024) unsigned char smem[];
   unsigned char* q_s = smem;                                       // [NR][HD / 64][128][128 B]
-  unsigned char* k_s = q_s + NR * SH::Q_BYTES;                     // [STAGES][HD / 64][64][128 B]
+  unsigned char* k_s = q_s + NR * SH::Q_BYTES;                     // [STAGES][HD / 64][128][128 B]
   unsigned char* v_s = k_s + STAGES * KV_BYTES;
-  uint64_t* full_k = reinterpret_cast<uint64_t*>(v_s + STAGES * KV_BYTES);
+  unsigned char* raw_s = v_s + STAGES * KV_BYTES;                  // [2][AHEAD][pieces a thread][64 threads][16 B]
+  float4* scale_s = reinterpret_cast<float4*>(raw_s + 2 * SH::AHEAD * SH::RAW_BYTES);      // [SCALE_STAGES][GROUPS]
+  float* raw_scale = reinterpret_cast<float*>(scale_s + SCALE_STAGES * GROUPS);            // [AHEAD][2][4]
+  uint64_t* full_k = reinterpret_cast<uint64_t*>(raw_scale + SH::AHEAD * 8);
   uint64_t* empty_k = full_k + STAGES;
   uint64_t* full_v = empty_k + STAGES;
   uint64_t* empty_v = full_v + STAGES;
-  uint64_t* bar_s = empty_v + STAGES;                              // [NR][2]: that score buffer is complete
-  uint64_t* bar_p = bar_s + 2 * NR;                                // [NR][2]: all rows have read S(t) and written P(t)
-  uint64_t* bar_pv = bar_p + 2 * NR;                               // [NR]: an O product is complete
+  uint64_t* bar_s = empty_v + STAGES;                              // [NR][NB]: that score buffer is complete
+  uint64_t* bar_p = bar_s + NB * NR;                               // [NR][NB]: all rows have read S(t) and written P(t)
+  uint64_t* bar_pv = bar_p + NB * NR;                              // [NR]: an O product is complete
   uint64_t* bar_o = bar_pv + NR;                                   // [NR]: the last one
-  uint64_t* bar_x = bar_o + NR;                                    // [NR][4]: both threads of the rows have left their maxima
-  uint64_t* bar_r = bar_x + 4 * NR;                                // [NR][4]: both have read the other's
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bar_r + 4 * NR);
+  uint64_t* bar_q = bar_o + NR;                                    // the queries are in place
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bar_q + 1);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
-  float* max_x = reinterpret_cast<float*>(tmem_slot + 4);          // [NR][2][128]
-  float4* scale_s = reinterpret_cast<float4*>(smem + ((SH::TILES + SH::BARS * 8 + 16 + NR * 2 * TQ * 4 + 15) & ~(size_t)15));
 
   const int b = blockIdx.z, kvh = blockIdx.y, G = a.H / a.KVH;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  if ((smem_u32(smem) & 1023u) != 0) {                             // the swizzled tiles need 1024-byte alignment
+    if (tid == 0) atomicCAS(a.status, 0, 29);
+    return;
+  }
   pdl_wait();                                                      // what it reads is written by kernels before
   const int qs = a.q_start[b], q_len = a.q_start[b + 1] - qs, seq_len = a.seq_lens[b];
   const int n_rows = q_len * G, n_blocks = (n_rows + ROWS - 1) / ROWS;
   if ((int)blockIdx.x >= n_blocks) return;
   const int row0 = (n_blocks - 1 - blockIdx.x) * ROWS;             // longest blocks first
   const int prefix = seq_len - q_len;
-
-  if ((smem_u32(smem) & 1023u) != 0) {                             // the swizzled tiles need 1024-byte alignment
-    if (tid == 0) atomicCAS(a.status, 0, 29);
-    return;
-  }
   if (tid == 0) {
     for (int s = 0; s < STAGES; ++s) {
-      mbar_init(&full_k[s], CONV_WARPS / 2);
+      mbar_init(&full_k[s], CONV_WARPS / 2 * (TK / UNIT));
       mbar_init(&empty_k[s], 1);
-      mbar_init(&full_v[s], CONV_WARPS / 2);
+      mbar_init(&full_v[s], CONV_WARPS / 2 * (TK / UNIT));
       mbar_init(&empty_v[s], 1);
     }
     for (int r = 0; r < NR; ++r) {
-      for (int i = 0; i < 2; ++i) {
-        mbar_init(&bar_s[2 * r + i], 2);                           // the product's end, and the issuing thread, which saw the scales
-        mbar_init(&bar_p[2 * r + i], 2 * TQ);
+      for (int i = 0; i < NB; ++i) {
+        mbar_init(&bar_s[NB * r + i], 2);                          // the product's end, and the issuing thread, which saw the scales
+        mbar_init(&bar_p[NB * r + i], TQ);
       }
       mbar_init(&bar_pv[r], 1);
       mbar_init(&bar_o[r], 1);
-      for (int i = 0; i < 4; ++i) {
-        mbar_init(&bar_x[4 * r + i], 64);
-        mbar_init(&bar_r[4 * r + i], 64);
-      }
     }
+    mbar_init(bar_q, SH::SOFT_WARPS * 32);
     *abort_flag = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
@@ -128,6 +140,10 @@ __global__ void __launch_bounds__(Shape<HD, NR>::THREADS, 1) attention_q8_prefil
     asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(tmem_slot)), "r"(SH::TMEM_COLS) : "memory");
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
   }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = *tmem_slot;
 
   const int last_row = min(row0 + ROWS, n_rows) - 1;
   const int j_hi = prefix + last_row / G;                          // the last key that any row sees, and the first
@@ -135,112 +151,80 @@ __global__ void __launch_bounds__(Shape<HD, NR>::THREADS, 1) attention_q8_prefil
   const int j_lo = key_lo & ~15;
   const int n_tiles = (seq_len > 0 && j_hi >= key_lo) ? (j_hi - j_lo) / TK + 1 : 0;
 
-  // a softmax thread's row tile, row, and which half of a turn's keys (and of the head's columns) it takes
-  const int rt = warp >> 3, lane_row = tid & (TQ - 1), hh = (warp >> 2) & 1;
+  const int rt = warp >> 2, lane_row = tid & (TQ - 1);             // a softmax thread's row tile and row
   const bool softmax = warp < SH::SOFT_WARPS;
-  const int row = row0 + rt * TQ + lane_row;
+  const int row = row0 + tid;
   const bool row_ok = softmax && row < n_rows;
   const int tok = row_ok ? row / G : 0, g = row_ok ? row % G : 0;
   const int pos = row_ok ? prefix + tok : -1;
 
-  // Q rows -> shared memory as half floats, K-major with the 128-byte swizzle (16-byte piece c of row r at c ^ (r & 7))
-  float factor = 0.f;
-  uint4 qv[HC / 8];
-  if (softmax) {
-    const bf16* src = a.q + (size_t)(qs + tok) * a.q_ts + (size_t)(kvh * G + g) * HD + hh * HC;
-    float amax = 0.f;
-#pragma unroll
-    for (int cc = 0; cc < HC / 8; ++cc) {
-      qv[cc] = row_ok ? *reinterpret_cast<const uint4*>(src + cc * 8) : make_uint4(0u, 0u, 0u, 0u);
-      const unsigned w[4] = {qv[cc].x, qv[cc].y, qv[cc].z, qv[cc].w};
-#pragma unroll
-      for (int i = 0; i < 4; ++i)
-        amax = fmaxf(amax, fmaxf(q8::abs_or_inf(__uint_as_float(w[i] << 16)), q8::abs_or_inf(__uint_as_float(w[i] & 0xffff0000u))));
-    }
-    max_x[(rt * 2 + hh) * TQ + lane_row] = amax;
-  }
-  __syncthreads();
-  if (softmax) {
-    const float amax = fmaxf(max_x[rt * 2 * TQ + lane_row], max_x[(rt * 2 + 1) * TQ + lane_row]);
-    const float to_half = q8::query_to_half(amax, a.scale * LOG2E_P, factor);
-#pragma unroll
-    for (int cc = 0; cc < HC / 8; ++cc) {
-      const unsigned w[4] = {qv[cc].x, qv[cc].y, qv[cc].z, qv[cc].w};
-      unsigned h[4];
-#pragma unroll
-      for (int i = 0; i < 4; ++i)
-        h[i] = q8::pack_half(__uint_as_float(w[i] << 16) * to_half, __uint_as_float(w[i] & 0xffff0000u) * to_half);
-      const int c = hh * (HC / 8) + cc;
-      *reinterpret_cast<uint4*>(q_s + rt * SH::Q_BYTES + (c >> 3) * HALF_Q + lane_row * 128 + (((c & 7) ^ (lane_row & 7)) << 4)) =
-          make_uint4(h[0], h[1], h[2], h[3]);
-    }
-  }
-  fence_async_smem();
-  tc_fence_before();
-  __syncthreads();
-  tc_fence_after();
-  const uint32_t tmem = *tmem_slot;
-
   if (warp >= SH::CONV_WARP) {
     // ================= converters: warps 0 and 1 the keys (and the scales), 2 and 3 the values =================
-    constexpr int CPR = HD / 16, NP = TK * CPR / 64;               // 16-byte pieces of a row; pieces a thread takes of a tile
-    constexpr int RPP = 64 / CPR;                                  // rows a turn of 64 threads covers
+    constexpr int CPR = HD / 16, NP = UNIT * CPR / 64;             // 16-byte pieces of a row; pieces a thread takes of 64 rows
+    constexpr int RPP = 64 / CPR;                                  // rows that 64 threads cover with a piece each
     const bool keys = warp < SH::CONV_WARP + 2;
     const int ct = (tid - SH::CONV_WARP * 32) & 63, c16 = ct % CPR, r0 = ct / CPR;
     const unsigned char* cache = keys ? a.cache[0] : a.cache[1];
     const int* table = a.block_tables + (size_t)b * a.table_width;
-    // the page of 16 keys (lane & 3) of tile t, -1 outside; fetched two tiles ahead, for lanes 0 to 3's sake by all of them
-    auto page_of = [&](int t) {
-      const int j = j_lo + t * TK + (lane & 3) * 16, lp = j / a.page;
-      return (t < n_tiles && j <= j_hi && lp < a.table_width) ? table[lp] : -1;
+    const int n_units = n_tiles * (TK / UNIT);
+    // the page and the place in it of 16 keys, a lane, of 512 rows: -1 outside; fetched that many rows ahead
+    int pg = -1, in_page = 0, pg_next, in_next;
+    auto fetch_pages = [&](int block) {
+      const int j = j_lo + block * 512 + lane * 16, lp = j / a.page;
+      in_next = j - lp * a.page;
+      pg_next = (j <= j_hi && lp < a.table_width) ? table[lp] : -1;
     };
-    uint4 piece[NP];
-    float ks = 0.f, vs = 0.f;
-    auto load_scales = [&](int pg) {
-      const size_t at = (size_t)max(pg, 0) * a.KVH + kvh;
-      ks = pg >= 0 ? a.scales[0][at] : 0.f;
-      vs = pg >= 0 ? a.scales[1][at] : 1.f;
-    };
-    auto load = [&](int t, int pg, int in_page, int i) {
-      const int r = r0 + i * RPP, grp = r >> 4, j = j_lo + t * TK + r;
-      const int p = __shfl_sync(0xffffffffu, pg, grp), in = __shfl_sync(0xffffffffu, in_page, grp);
-      const bool there = p >= 0 && j >= key_lo && j <= j_hi;
-      const unsigned char* src = cache + (((size_t)max(p, 0) * a.KVH + kvh) * a.page + in + (r & 15)) * HD + c16 * 16;
-      piece[i] = there ? __ldg(reinterpret_cast<const uint4*>(src)) : make_uint4(0u, 0u, 0u, 0u);
-    };
-    auto in_page_of = [&](int t) { return (j_lo + t * TK + (lane & 3) * 16) % a.page; };
-    int pg_next = page_of(1);
-    if (n_tiles > 0) {
-      const int pg = page_of(0), in_page = in_page_of(0);
+    fetch_pages(0);
+    // 64 rows from the pages, asynchronously: a thread's pieces go to a place of its own, which it alone reads
+    unsigned char* raw = raw_s + (keys ? 0 : SH::AHEAD * SH::RAW_BYTES) + ct * 16;
+    auto issue = [&](int u) {
+      if (u < n_units) {
+        if (u % 8 == 0) {
+          pg = pg_next;
+          in_page = in_next;
+          fetch_pages(u / 8 + 1);
+        }
+        unsigned char* dst = raw + (u % SH::AHEAD) * SH::RAW_BYTES;
 #pragma unroll
-      for (int i = 0; i < NP; ++i) load(0, pg, in_page, i);
-      if (keys) load_scales(pg);
-    }
+        for (int grp = 0; grp < 4; ++grp) {
+          const int p = __shfl_sync(0xffffffffu, pg, (u % 8) * 4 + grp), in = __shfl_sync(0xffffffffu, in_page, (u % 8) * 4 + grp);
+          const unsigned char* src = cache + (((size_t)max(p, 0) * a.KVH + kvh) * a.page + in + (r0 & 15)) * HD + c16 * 16;
+#pragma unroll
+          for (int i = 0; i < NP / 4; ++i) {
+            const int j = j_lo + u * UNIT + grp * 16 + (r0 & 15) + i * RPP;
+            cp_async_16(dst + (grp * (NP / 4) + i) * 1024, src + i * RPP * HD, p >= 0 && j >= key_lo && j <= j_hi);
+          }
+        }
+        if (warp == SH::CONV_WARP) {
+          const int p = __shfl_sync(0xffffffffu, pg, (u % 8) * 4 + (lane & 3));
+          const size_t at = (size_t)max(p, 0) * a.KVH + kvh;
+          if (lane < 8) cp_async_4(raw_scale + (u % SH::AHEAD) * 8 + lane, (lane < 4 ? a.scales[0] : a.scales[1]) + at, p >= 0);
+        }
+      }
+      cp_async_commit();
+    };
+#pragma unroll 1
+    for (int u = 0; u < SH::AHEAD; ++u) issue(u);
     bool ok = true;
-    for (int t = 0; t < n_tiles; ++t) {
-      const int st = t % STAGES;
-      if (t >= STAGES) {
+    for (int u = 0; u < n_units; ++u) {
+      const int t = u / (TK / UNIT), half = u % (TK / UNIT), st = t % STAGES;
+      if (half == 0 && t >= STAGES) {
         ok = mbar_wait(keys ? &empty_k[st] : &empty_v[st], (uint32_t)((t / STAGES - 1) & 1), a.status, keys ? 24 : 27, abort_flag);
         ok = __all_sync(0xffffffffu, ok);
         if (!ok) break;
       }
-      unsigned char* tile = (keys ? k_s : v_s) + st * KV_BYTES;
-      if (keys && warp == SH::CONV_WARP && lane < 4)
-        // (score factor, log2 of the value's scale, its inverse) of 16 keys
-        scale_s[(t % SCALE_STAGES) * 4 + lane] = make_float4(vs != vs ? vs : ks, (float)((int)(__float_as_uint(vs) >> 23) - 127),
-                                                             q8::inverse_scale(vs), 0.f);
-      const int pg = pg_next, in_page = in_page_of(t + 1);
-      pg_next = page_of(t + 2);
-      if (keys) load_scales(pg);
+      cp_async_wait<SH::AHEAD - 1>();
+      unsigned char* tile = (keys ? k_s : v_s) + st * KV_BYTES + half * UNIT * 128;
+      const unsigned char* src = raw + (u % SH::AHEAD) * SH::RAW_BYTES;
 #pragma unroll
       for (int i = 0; i < NP; ++i) {
         const int r = r0 + i * RPP, odd = c16 >> 2 & (HD == 128 ? 1 : 0);
+        const uint4 piece = *reinterpret_cast<const uint4*>(src + i * 1024);
         uint4 lo, hi;
-        q8::halves_of(piece[i].x, lo.x, lo.y);
-        q8::halves_of(piece[i].y, lo.z, lo.w);
-        q8::halves_of(piece[i].z, hi.x, hi.y);
-        q8::halves_of(piece[i].w, hi.z, hi.w);
-        load(t + 1, pg, in_page, i);                               // (nothing behind the last tile: its pages are -1)
+        q8::halves_of(piece.x, lo.x, lo.y);
+        q8::halves_of(piece.y, lo.z, lo.w);
+        q8::halves_of(piece.z, hi.x, hi.y);
+        q8::halves_of(piece.w, hi.z, hi.w);
         // columns 16 c16 .. of the row: half c16 / 4 of the head, pieces 2 (c16 & 3) and the next; the second half's lanes begin with
         // the second piece, so that a row's eight lanes write to eight different places of a line
         unsigned char* line = tile + (c16 >> 2) * HALF_K + r * 128;
@@ -248,10 +232,21 @@ __global__ void __launch_bounds__(Shape<HD, NR>::THREADS, 1) attention_q8_prefil
         *reinterpret_cast<uint4*>(line + (((first + odd) ^ (r & 7)) << 4)) = odd ? hi : lo;
         *reinterpret_cast<uint4*>(line + (((first + 1 - odd) ^ (r & 7)) << 4)) = odd ? lo : hi;
       }
+      if (warp == SH::CONV_WARP) {
+        __syncwarp();                                              // (lanes 4 to 7 brought the values' scales)
+        if (lane < 4) {
+          const float ks = raw_scale[(u % SH::AHEAD) * 8 + lane], vs = raw_scale[(u % SH::AHEAD) * 8 + 4 + lane];
+          // (score factor, log2 of the value's scale, its inverse) of 16 keys
+          scale_s[(t % SCALE_STAGES) * GROUPS + half * 4 + lane] =
+              make_float4(vs != vs ? vs : ks, (float)((int)(__float_as_uint(vs) >> 23) - 127), q8::inverse_scale(vs), 0.f);
+        }
+      }
       fence_async_smem();
       __syncwarp();
       if (lane == 0) mbar_arrive(keys ? &full_k[st] : &full_v[st]);
+      issue(u + SH::AHEAD);
     }
+    cp_async_wait<0>();
   } else if (warp == SH::MMA_WARP) {
     // ================= product issue, one lane =================
     if (lane == 0 && n_tiles > 0) {
@@ -260,10 +255,10 @@ __global__ void __launch_bounds__(Shape<HD, NR>::THREADS, 1) attention_q8_prefil
         const uint32_t qa = smem_u32(q_s + r * SH::Q_BYTES), ka = smem_u32(k_s + (t % STAGES) * KV_BYTES);
 #pragma unroll
         for (int ks = 0; ks < HD / 16; ++ks)
-          umma(tmem + r * ROW_COLS + (t & 1) * TK, smem_desc(qa + (ks >> 2) * HALF_Q + (ks & 3) * 32),
+          umma(tmem + r * ROW_COLS + (t % NB) * TK, smem_desc(qa + (ks >> 2) * HALF_Q + (ks & 3) * 32),
                smem_desc(ka + (ks >> 2) * HALF_K + (ks & 3) * 32), idesc, ks > 0 ? 1u : 0u);
-        umma_commit(&bar_s[2 * r + (t & 1)]);
-        mbar_arrive(&bar_s[2 * r + (t & 1)]);
+        umma_commit(&bar_s[NB * r + t % NB]);
+        mbar_arrive(&bar_s[NB * r + t % NB]);
         if (r == NR - 1) umma_commit(&empty_k[t % STAGES]);
       };
       auto issue_o = [&](int r, int t) {
@@ -271,108 +266,169 @@ __global__ void __launch_bounds__(Shape<HD, NR>::THREADS, 1) attention_q8_prefil
         const uint32_t va = smem_u32(v_s + (t % STAGES) * KV_BYTES), d = tmem + r * ROW_COLS + O_COL;
 #pragma unroll
         for (int kk = 0; kk < TK / 16; ++kk)
-          umma_ts(d, tmem + r * ROW_COLS + (t & 1) * TK + kk * 8, smem_desc_mn(va + kk * 16 * 128, HALF_K), idesc, (t > 0 || kk > 0) ? 1u : 0u);
+          umma_ts(d, tmem + r * ROW_COLS + (t % NB) * TK + kk * 8, smem_desc_mn(va + kk * 16 * 128, HALF_K), idesc, (t > 0 || kk > 0) ? 1u : 0u);
         if (r == NR - 1) umma_commit(&empty_v[t % STAGES]);
         umma_commit(&bar_pv[r]);
         if (t + 1 == n_tiles) umma_commit(&bar_o[r]);
       };
-      bool ok = true;
-      for (int t = 0; t < 2 && t < n_tiles && ok; ++t) {
-        ok = mbar_wait(&full_k[t], 0, a.status, 21, abort_flag);
+      bool ok = mbar_wait(bar_q, 0, a.status, 20, abort_flag);
+      for (int t = 0; t < NB && t < n_tiles && ok; ++t) {
+        ok = mbar_wait(&full_k[t % STAGES], 0, a.status, 21, abort_flag);
         if (!ok) break;
         tc_fence_after();
         for (int r = 0; r < NR; ++r) issue_s(r, t);
       }
       for (int t = 0; t < n_tiles && ok; ++t)
         for (int r = 0; r < NR && ok; ++r) {
-          ok = mbar_wait_spin(&bar_p[2 * r + (t & 1)], (uint32_t)((t >> 1) & 1), a.status, 26, abort_flag);
+          ok = mbar_wait_spin(&bar_p[NB * r + t % NB], (uint32_t)((t / NB) & 1), a.status, 26, abort_flag);
           if (ok && r == 0) ok = mbar_wait(&full_v[t % STAGES], (uint32_t)((t / STAGES) & 1), a.status, 23, abort_flag);
           if (!ok) break;
           tc_fence_after();
           issue_o(r, t);
-          if (t + 2 < n_tiles) {
-            if (r == 0) ok = mbar_wait(&full_k[t % STAGES], (uint32_t)(((t + 2) / STAGES) & 1), a.status, 28, abort_flag);
+          if (t + NB < n_tiles) {
+            if (r == 0) ok = mbar_wait(&full_k[(t + NB) % STAGES], (uint32_t)(((t + NB) / STAGES) & 1), a.status, 28, abort_flag);
             if (!ok) break;
             tc_fence_after();
-            issue_s(r, t + 2);                                     // over P(t), behind the product that reads it
+            issue_s(r, t + NB);                                    // over P(t), behind the product that reads it
           }
         }
     }
   } else {
-    // ================= softmax: two threads per row = tensor-memory lane =================
+    // ================= softmax: a thread a row = tensor-memory lane =================
+    // Q rows -> shared memory as half floats, K-major with the 128-byte swizzle (16-byte piece c of row r at c ^ (r & 7))
+    float factor = 0.f;
+    {
+      const uint4* src = reinterpret_cast<const uint4*>(a.q + (size_t)(qs + tok) * a.q_ts + (size_t)(kvh * G + g) * HD);
+      uint4 v[HD / 8];
+      float amax = 0.f;
+#pragma unroll
+      for (int c = 0; c < HD / 8; ++c) v[c] = row_ok ? src[c] : make_uint4(0u, 0u, 0u, 0u);
+#pragma unroll
+      for (int c = 0; c < HD / 8; ++c) {
+        const unsigned w[4] = {v[c].x, v[c].y, v[c].z, v[c].w};
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+          amax = fmaxf(amax, fmaxf(q8::abs_or_inf(__uint_as_float(w[i] << 16)), q8::abs_or_inf(__uint_as_float(w[i] & 0xffff0000u))));
+      }
+      // (the factor is positive: a negative scale turns the queries)
+      float to_half = q8::query_to_half(amax, fabsf(a.scale) * LOG2E_P, factor);
+      if (a.scale < 0.f) to_half = -to_half;
+#pragma unroll
+      for (int c = 0; c < HD / 8; ++c) {
+        const unsigned w[4] = {v[c].x, v[c].y, v[c].z, v[c].w};
+        unsigned h[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+          h[i] = q8::pack_half(__uint_as_float(w[i] << 16) * to_half, __uint_as_float(w[i] & 0xffff0000u) * to_half);
+        *reinterpret_cast<uint4*>(q_s + rt * SH::Q_BYTES + (c >> 3) * HALF_Q + lane_row * 128 + (((c & 7) ^ (lane_row & 7)) << 4)) =
+            make_uint4(h[0], h[1], h[2], h[3]);
+      }
+      fence_async_smem();
+      mbar_arrive(bar_q);
+    }
     float m_ref = -INFINITY, l_run = 0.f;
-    const int pair = warp & 3;                                     // warps `pair` and `pair + 4` of the row tile share 32 rows
-    const uint32_t lane_addr = tmem + ((uint32_t)(pair * 32) << 16) + rt * ROW_COLS;
-    uint64_t* const my_x = &bar_x[4 * rt + pair];
-    uint64_t* const my_r = &bar_r[4 * rt + pair];
-    float* const max_mine = max_x + (rt * 2 + hh) * TQ + lane_row;
-    const float* const max_other = max_x + (rt * 2 + (hh ^ 1)) * TQ + lane_row;
+    const uint32_t lane_addr = tmem + ((uint32_t)((warp & 3) * 32) << 16) + rt * ROW_COLS;
     bool ok = true;
     for (int t = 0; t < n_tiles; ++t) {
-      const uint32_t s_addr = lane_addr + (t & 1) * TK;
-      ok = mbar_wait_spin(&bar_s[2 * rt + (t & 1)], (uint32_t)((t >> 1) & 1), a.status, 22, abort_flag);
+      const uint32_t s_addr = lane_addr + (t % NB) * TK;
+      ok = mbar_wait_spin(&bar_s[NB * rt + t % NB], (uint32_t)((t / NB) & 1), a.status, 22, abort_flag);
       ok = __all_sync(0xffffffffu, ok);
       if (!ok) break;
       tc_fence_after();
-      const int j0 = j_lo + t * TK + hh * KT;                      // this thread's first key of the turn
-      uint32_t sv[KT];
-      tmem_ld32(s_addr + hh * KT, sv);
-      const float4 sc0 = scale_s[(t % SCALE_STAGES) * 4 + 2 * hh], sc1 = scale_s[(t % SCALE_STAGES) * 4 + 2 * hh + 1];
-      const float f0 = sc0.x * factor, f1 = sc1.x * factor;
-      tmem_wait_ld();
-      float mx = -INFINITY;
-      const bool all_visible = __all_sync(0xffffffffu, (j0 + KT - 1 <= pos) && (a.window <= 0 || j0 > pos - a.window));
+      const int j0 = j_lo + t * TK;
+      const float4* sc = scale_s + (t % SCALE_STAGES) * GROUPS;
+      // keys wholly before every row of the warp (the common case away from the diagonal) need no mask
+      const bool all_visible = __all_sync(0xffffffffu, (j0 + TK - 1 <= pos) && (a.window <= 0 || j0 > pos - a.window));
+      const int see_lo = a.window > 0 ? max(0, pos - a.window + 1 - j0) : 0;       // the row sees keys see_lo .. see_lo + see_n of the turn
+      const unsigned see_n = (unsigned)max(0, min(TK, pos + 1 - j0) - see_lo);
+      bool move = false;
+      float corr = 1.f, rs = 0.f;
+      // Both passes go over 64 scores a turn of their loops, which stay loops: unrolled whole they are more instructions than the caches
+      // near the schedulers hold.  32 scores come while the 32 before are worked on.
+      auto turn = [&](auto masked) {
+        constexpr bool MASK = decltype(masked)::value;
+        uint32_t buf[2][32];
+        float mx = -INFINITY;
+        auto largest = [&](const uint32_t(&sv)[32], int c) {
 #pragma unroll
-      for (int i = 0; i < KT; ++i) {
-        float v = i < 16 ? fmaf(__uint_as_float(sv[i]), f0, sc0.y) : fmaf(__uint_as_float(sv[i]), f1, sc1.y);
-        if (!all_visible) v = (j0 + i <= pos && (a.window <= 0 || j0 + i > pos - a.window)) ? v : -INFINITY;
-        sv[i] = __float_as_uint(v);
-        mx = fmaxf(mx, v);
-      }
-      if (t > 0) {
-        ok = mbar_wait_spin(my_r, (uint32_t)((t - 1) & 1), a.status, 31, abort_flag);      // the last one has been read
-        ok = __all_sync(0xffffffffu, ok);
-        if (!ok) break;
-      }
-      *max_mine = mx;
-      mbar_arrive(my_x);
-      // P as pairs of half floats, and this half's share of the denominator
-      uint32_t pw[KT / 2];
-      auto exponentials = [&](float m_use) {
-        float rs0 = 0.f, rs1 = 0.f;
+          for (int h = 0; h < 2; ++h) {
+            float top[2] = {-INFINITY, -INFINITY};
 #pragma unroll
-        for (int i = 0; i < KT / 2; ++i) {
-          const float p0 = ex2(__uint_as_float(sv[2 * i]) - m_use), p1 = ex2(__uint_as_float(sv[2 * i + 1]) - m_use);
-          if (i < 8) rs0 += p0 + p1;
-          else rs1 += p0 + p1;
-          pw[i] = q8::pack_half(p0, p1);
+            for (int i = 0; i < 16; i += 2) {
+              float s0 = __uint_as_float(sv[h * 16 + i]), s1 = __uint_as_float(sv[h * 16 + i + 1]);
+              if (MASK) {
+                s0 = (unsigned)(c * 32 + h * 16 + i - see_lo) < see_n ? s0 : -INFINITY;
+                s1 = (unsigned)(c * 32 + h * 16 + i + 1 - see_lo) < see_n ? s1 : -INFINITY;
+              }
+              top[i >> 1 & 1] = max3(top[i >> 1 & 1], s0, s1);
+            }
+            const float4 x = sc[2 * c + h];
+            const float best = fmaxf(top[0], top[1]);
+            // (nothing seen: no maximum, whatever the factor)
+            mx = fmaxf(mx, MASK && best == -INFINITY ? -INFINITY : fmaf(best, x.x * factor, x.y));
+          }
+        };
+        tmem_ld32(s_addr, buf[0]);
+#pragma unroll 1
+        for (int c = 0; c < TK / 32; c += 2) {
+          tmem_wait_ld();
+          tmem_ld32(s_addr + (c + 1) * 32, buf[1]);
+          largest(buf[0], c);
+          tmem_wait_ld();
+          tmem_ld32(s_addr + (c + 2) % (TK / 32) * 32, buf[0]);    // (at last the first ones again, for the weights)
+          largest(buf[1], c + 1);
         }
-        return fmaf(rs0, sc0.z, rs1 * sc1.z);
+        move = mx > m_ref + RESCALE_STEP || (m_ref == -INFINITY && mx > -INFINITY);
+        if (move) {
+          corr = ex2(m_ref - mx);                                  // 0 when there was no reference yet
+          m_ref = mx;
+        }
+        const float m_use = m_ref == -INFINITY ? 0.f : m_ref;
+        auto weights = [&](const uint32_t(&sv)[32], int c) {
+          uint32_t pw[16];
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {
+            const float4 x = sc[2 * c + h];
+            const float f = x.x * factor, add = x.y - m_use;
+            float part[2] = {0.f, 0.f};
+#pragma unroll
+            for (int i = 0; i < 16; i += 2) {
+              float p0 = ex2(fmaf(__uint_as_float(sv[h * 16 + i]), f, add));
+              float p1 = ex2(fmaf(__uint_as_float(sv[h * 16 + i + 1]), f, add));
+              if (MASK) {
+                p0 = (unsigned)(c * 32 + h * 16 + i - see_lo) < see_n ? p0 : 0.f;
+                p1 = (unsigned)(c * 32 + h * 16 + i + 1 - see_lo) < see_n ? p1 : 0.f;
+              }
+              part[0] += p0;
+              part[1] += p1;
+              pw[h * 8 + i / 2] = q8::pack_half(p0, p1);
+            }
+            rs = fmaf(part[0] + part[1], x.z, rs);
+          }
+          tmem_st16(s_addr + c * 16, pw);                          // over scores that have been read
+        };
+#pragma unroll 1
+        for (int c = 0; c < TK / 32; c += 2) {
+          tmem_wait_ld();
+          tmem_ld32(s_addr + (c + 1) * 32, buf[1]);
+          weights(buf[0], c);
+          tmem_wait_ld();
+          if (c + 2 < TK / 32) tmem_ld32(s_addr + (c + 2) * 32, buf[0]);
+          weights(buf[1], c + 1);
+        }
       };
-      // taken against the present reference while the other thread's maximum is on its way, and again for rows whose reference moves
-      const bool ahead = __all_sync(0xffffffffu, m_ref != -INFINITY);
-      float rs = 0.f;
-      if (ahead) rs = exponentials(m_ref);
-      ok = mbar_wait_spin(my_x, (uint32_t)(t & 1), a.status, 32, abort_flag);
-      ok = __all_sync(0xffffffffu, ok);
-      if (!ok) break;
-      mx = fmaxf(mx, *max_other);
-      mbar_arrive(my_r);
-      const bool move = mx > m_ref + RESCALE_STEP || (m_ref == -INFINITY && mx > -INFINITY);
-      float corr = 1.f;
-      if (move) {
-        corr = ex2(m_ref - mx);                                    // 0 when there was no reference yet
-        m_ref = mx;
-      }
-      if (!ahead || move) rs = exponentials((m_ref == -INFINITY) ? 0.f : m_ref);
+      if (all_visible) turn(std::false_type());
+      else turn(std::true_type());
       l_run = l_run * corr + rs;
       if (t > 0 && __any_sync(0xffffffffu, move)) {
-        ok = mbar_wait_spin(&bar_pv[rt], (uint32_t)((t - 1) & 1), a.status, 30, abort_flag);
-        ok = __all_sync(0xffffffffu, ok);
-        if (!ok) break;
-        tc_fence_after();
+        if (NB == 2) {                                             // (one buffer: S(t) was issued behind the product before, and is complete)
+          ok = mbar_wait_spin(&bar_pv[rt], (uint32_t)((t - 1) & 1), a.status, 30, abort_flag);
+          ok = __all_sync(0xffffffffu, ok);
+          if (!ok) break;
+          tc_fence_after();
+        }
 #pragma unroll 1
-        for (int c = hh * HC; c < hh * HC + HC; c += 32) {
+        for (int c = 0; c < HD; c += 32) {
           uint32_t ov[32];
           tmem_ld32(lane_addr + O_COL + c, ov);
           tmem_wait_ld();
@@ -381,35 +437,20 @@ __global__ void __launch_bounds__(Shape<HD, NR>::THREADS, 1) attention_q8_prefil
           tmem_st32(lane_addr + O_COL + c, ov);
         }
       }
-      // over the first half of S(t): the second thread's words lie over scores of the FIRST thread of the row, which has them in
-      // registers since before it left its maximum
-      tmem_st16(s_addr + hh * 16, pw);
       tmem_wait_st();
       tc_fence_before();
-      mbar_arrive(&bar_p[2 * rt + (t & 1)]);
+      mbar_arrive(&bar_p[NB * rt + t % NB]);
     }
     if (ok && n_tiles > 0) {
       ok = mbar_wait(&bar_o[rt], 0, a.status, 25, abort_flag);
       ok = __all_sync(0xffffffffu, ok);
-    }
-    // the row's denominator is the two halves' (same reference): through the maxima's places, once the last ones have been read
-    if (ok && n_tiles > 0) {
-      ok = mbar_wait_spin(my_r, (uint32_t)((n_tiles - 1) & 1), a.status, 33, abort_flag);
-      ok = __all_sync(0xffffffffu, ok);
-      if (ok) {
-        *max_mine = l_run;
-        mbar_arrive(my_x);
-        ok = mbar_wait_spin(my_x, (uint32_t)(n_tiles & 1), a.status, 34, abort_flag);
-        ok = __all_sync(0xffffffffu, ok);
-        if (ok) l_run += *max_other;
-      }
     }
     if (ok) {
       tc_fence_after();
       bf16* dst = a.out + (size_t)(qs + tok) * a.o_ts + (size_t)(kvh * G + g) * HD;
       const float inv = l_run > 0.f ? 1.f / l_run : l_run;         // nothing seen: 0; NaN stays
 #pragma unroll 1
-      for (int c = hh * HC; c < hh * HC + HC; c += 32) {
+      for (int c = 0; c < HD; c += 32) {
         uint32_t ov[32];
         if (n_tiles > 0) {
           tmem_ld32(lane_addr + O_COL + c, ov);                    // the whole warp loads; rows without a query store nothing
