@@ -7,10 +7,10 @@
 // without them, and a sum one more for 16 weights.
 //
 // One block = NR tiles of 128 query rows (a row is a (token, head-in-group) pair of one kv head) over the same keys, 128 a turn.
-// Softmax: four warps a row tile, a thread a row = tensor-memory lane.  It reads its scores twice: for the maximum (the scale of 16 keys is
-// one factor, so that is the maximum of the products, three at a time, and one multiply-add), then 32 at a time for the weights, which
-// go back over scores already read as pairs of half floats.  One warp issues the products (one lane): S(t) = Q K(t)^T, O += P(t) V(t) with
-// P read from tensor memory.  Four warps turn the pages' bytes into half floats, two the keys and two the values: 16 bytes a piece, brought
+// Softmax: four warps a row tile, a thread a row = tensor-memory lane, which holds a turn's 128 scores in registers: their maximum (the
+// scale of 16 keys is one factor, so that is the maximum of the products, three an instruction, and one multiply-add), then the weights, which
+// go back over the scores as pairs of half floats.  One warp issues the products (one lane): S(t) = Q K(t)^T, O += P(t) V(t) with
+// P read from tensor memory.  Four warps (eight where NR = 1) turn the pages' bytes into half floats, half of them the keys: 16 bytes a piece, brought
 // by cp.async to a place that its thread alone reads, 128 rows and more ahead of the conversion, stored with the 128-byte swizzle that the products read (values with keys along
 // the rows: MN-major).  Rows outside the visible range are zeros.
 // NR = 2: a score buffer each, so that the softmax of one row tile runs beside the products of the other; a converted tile serves 256 rows;
@@ -31,15 +31,17 @@ namespace {
 
 using namespace tc;
 
-constexpr int TQ = 128, TK = 128, UNIT = 64, STAGES = 2, SCALE_STAGES = 4, CONV_WARPS = 4;
+constexpr int TQ = 128, TK = 128, UNIT = 64, STAGES = 2, SCALE_STAGES = 4;
 constexpr float RESCALE_STEP = 8.f;
 constexpr float LOG2E_P = 1.4426950408889634f;
 
 template <int HD, int NR>
 struct Shape {
   static constexpr int NB = NR == 1 ? 2 : 1;                       // score buffers of a row tile
-  static constexpr int SOFT_WARPS = 4 * NR, MMA_WARP = SOFT_WARPS, CONV_WARP = MMA_WARP + 1;
-  static constexpr int THREADS = (SOFT_WARPS + 1 + CONV_WARPS) * 32;
+  // four warpgroups, each with its own number of registers a thread: softmax (one or two), conversion, and the one whose first warp issues
+  // the products.  128 a thread are there; what the others give back the softmax takes: 256 x 200 + 256 x 56, 128 x 232 + 384 x 88.
+  static constexpr int SOFT_WARPS = 4 * NR, CONV_WARPS = NR == 1 ? 8 : 4, CONV_WARP = SOFT_WARPS, MMA_WARP = CONV_WARP + CONV_WARPS;
+  static constexpr int THREADS = 512, SOFT_REGS = NR == 1 ? 232 : 200, OTHER_REGS = NR == 1 ? 88 : 56;
   static constexpr uint32_t Q_BYTES = TQ * HD * 2, KV_BYTES = TK * HD * 2, HALF_Q = TQ * 128, HALF_K = TK * 128;
   static constexpr uint32_t O_COL = NB * TK, ROW_COLS = O_COL + HD; // tensor-memory columns of a row tile: scores, O
   static constexpr uint32_t TMEM_COLS = ROW_COLS * NR <= 256 ? 256 : 512;
@@ -73,6 +75,9 @@ __host__ __device__ constexpr uint32_t instr_half(int n, bool b_mn) {
   return (1u << 4) | ((b_mn ? 1u : 0u) << 16) | ((uint32_t)(n >> 3) << 17) | ((uint32_t)(128 >> 4) << 24);
 }
 
+// Registers a thread of the warpgroup gives back, or takes out of what others gave back.
+template <int N> __device__ __forceinline__ void give_registers() { asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(N)); }
+template <int N> __device__ __forceinline__ void take_registers() { asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(N)); }
 // The largest of three.
 __device__ __forceinline__ float max3(float x, float y, float z) {
   float r;
@@ -90,7 +95,7 @@ __global__ void __launch_bounds__(Shape<HD, NR>::THREADS, 1) attention_q8_prefil
   unsigned char* q_s = smem;                                       // [NR][HD / 64][128][128 B]
   unsigned char* k_s = q_s + NR * SH::Q_BYTES;                     // [STAGES][HD / 64][128][128 B]
   unsigned char* v_s = k_s + STAGES * KV_BYTES;
-  unsigned char* raw_s = v_s + STAGES * KV_BYTES;                  // [2][AHEAD][pieces a thread][64 threads][16 B]
+  unsigned char* raw_s = v_s + STAGES * KV_BYTES;                  // [2][AHEAD][pieces a thread][threads][16 B]
   float4* scale_s = reinterpret_cast<float4*>(raw_s + 2 * SH::AHEAD * SH::RAW_BYTES);      // [SCALE_STAGES][GROUPS]
   float* raw_scale = reinterpret_cast<float*>(scale_s + SCALE_STAGES * GROUPS);            // [AHEAD][2][4]
   uint64_t* full_k = reinterpret_cast<uint64_t*>(raw_scale + SH::AHEAD * 8);
@@ -119,9 +124,9 @@ __global__ void __launch_bounds__(Shape<HD, NR>::THREADS, 1) attention_q8_prefil
   const int prefix = seq_len - q_len;
   if (tid == 0) {
     for (int s = 0; s < STAGES; ++s) {
-      mbar_init(&full_k[s], CONV_WARPS / 2 * (TK / UNIT));
+      mbar_init(&full_k[s], SH::CONV_WARPS / 2 * (TK / UNIT));
       mbar_init(&empty_k[s], 1);
-      mbar_init(&full_v[s], CONV_WARPS / 2 * (TK / UNIT));
+      mbar_init(&full_v[s], SH::CONV_WARPS / 2 * (TK / UNIT));
       mbar_init(&empty_v[s], 1);
     }
     for (int r = 0; r < NR; ++r) {
@@ -158,12 +163,14 @@ __global__ void __launch_bounds__(Shape<HD, NR>::THREADS, 1) attention_q8_prefil
   const int tok = row_ok ? row / G : 0, g = row_ok ? row % G : 0;
   const int pos = row_ok ? prefix + tok : -1;
 
-  if (warp >= SH::CONV_WARP) {
-    // ================= converters: warps 0 and 1 the keys (and the scales), 2 and 3 the values =================
-    constexpr int CPR = HD / 16, NP = UNIT * CPR / 64;             // 16-byte pieces of a row; pieces a thread takes of 64 rows
-    constexpr int RPP = 64 / CPR;                                  // rows that 64 threads cover with a piece each
-    const bool keys = warp < SH::CONV_WARP + 2;
-    const int ct = (tid - SH::CONV_WARP * 32) & 63, c16 = ct % CPR, r0 = ct / CPR;
+  if (warp >= SH::CONV_WARP && warp < SH::MMA_WARP) {
+    // ================= converters: the first half of the warps the keys (and the scales), the others the values =================
+    give_registers<SH::OTHER_REGS>();
+    constexpr int CT = SH::CONV_WARPS * 16;                        // threads of each half
+    constexpr int CPR = HD / 16, NP = UNIT * CPR / CT;             // 16-byte pieces of a row; pieces a thread takes of 64 rows
+    constexpr int RPP = CT / CPR, SAME = RPP < 16 ? 16 / RPP : 1;  // rows that they cover with a piece each; pieces within 16 rows
+    const bool keys = warp < SH::CONV_WARP + SH::CONV_WARPS / 2;
+    const int ct = (tid - SH::CONV_WARP * 32) % CT, c16 = ct % CPR, r0 = ct / CPR;
     const unsigned char* cache = keys ? a.cache[0] : a.cache[1];
     const int* table = a.block_tables + (size_t)b * a.table_width;
     const int n_units = n_tiles * (TK / UNIT);
@@ -185,15 +192,17 @@ __global__ void __launch_bounds__(Shape<HD, NR>::THREADS, 1) attention_q8_prefil
           fetch_pages(u / 8 + 1);
         }
         unsigned char* dst = raw + (u % SH::AHEAD) * SH::RAW_BYTES;
+        const unsigned char* src = cache;
+        bool page = false;
 #pragma unroll
-        for (int grp = 0; grp < 4; ++grp) {
-          const int p = __shfl_sync(0xffffffffu, pg, (u % 8) * 4 + grp), in = __shfl_sync(0xffffffffu, in_page, (u % 8) * 4 + grp);
-          const unsigned char* src = cache + (((size_t)max(p, 0) * a.KVH + kvh) * a.page + in + (r0 & 15)) * HD + c16 * 16;
-#pragma unroll
-          for (int i = 0; i < NP / 4; ++i) {
-            const int j = j_lo + u * UNIT + grp * 16 + (r0 & 15) + i * RPP;
-            cp_async_16(dst + (grp * (NP / 4) + i) * 1024, src + i * RPP * HD, p >= 0 && j >= key_lo && j <= j_hi);
+        for (int i = 0; i < NP; ++i) {
+          const int r = r0 + i * RPP, j = j_lo + u * UNIT + r;
+          if (i % SAME == 0) {
+            const int p = __shfl_sync(0xffffffffu, pg, (u % 8) * 4 + (r >> 4)), in = __shfl_sync(0xffffffffu, in_page, (u % 8) * 4 + (r >> 4));
+            src = cache + (((size_t)max(p, 0) * a.KVH + kvh) * a.page + in + (r & 15)) * HD + c16 * 16;
+            page = p >= 0;
           }
+          cp_async_16(dst + i * (CT * 16), src + (i % SAME) * RPP * HD, page && j >= key_lo && j <= j_hi);
         }
         if (warp == SH::CONV_WARP) {
           const int p = __shfl_sync(0xffffffffu, pg, (u % 8) * 4 + (lane & 3));
@@ -219,7 +228,7 @@ __global__ void __launch_bounds__(Shape<HD, NR>::THREADS, 1) attention_q8_prefil
 #pragma unroll
       for (int i = 0; i < NP; ++i) {
         const int r = r0 + i * RPP, odd = c16 >> 2 & (HD == 128 ? 1 : 0);
-        const uint4 piece = *reinterpret_cast<const uint4*>(src + i * 1024);
+        const uint4 piece = *reinterpret_cast<const uint4*>(src + i * (CT * 16));
         uint4 lo, hi;
         q8::halves_of(piece.x, lo.x, lo.y);
         q8::halves_of(piece.y, lo.z, lo.w);
@@ -247,9 +256,10 @@ __global__ void __launch_bounds__(Shape<HD, NR>::THREADS, 1) attention_q8_prefil
       issue(u + SH::AHEAD);
     }
     cp_async_wait<0>();
-  } else if (warp == SH::MMA_WARP) {
+  } else if (warp >= SH::MMA_WARP) {
     // ================= product issue, one lane =================
-    if (lane == 0 && n_tiles > 0) {
+    give_registers<SH::OTHER_REGS>();
+    if (warp == SH::MMA_WARP && lane == 0 && n_tiles > 0) {
       auto issue_s = [&](int r, int t) {
         constexpr uint32_t idesc = instr_half(TK, false);
         const uint32_t qa = smem_u32(q_s + r * SH::Q_BYTES), ka = smem_u32(k_s + (t % STAGES) * KV_BYTES);
@@ -295,6 +305,7 @@ __global__ void __launch_bounds__(Shape<HD, NR>::THREADS, 1) attention_q8_prefil
     }
   } else {
     // ================= softmax: a thread a row = tensor-memory lane =================
+    take_registers<SH::SOFT_REGS>();
     // Q rows -> shared memory as half floats, K-major with the 128-byte swizzle (16-byte piece c of row r at c ^ (r & 7))
     float factor = 0.f;
     {
@@ -343,40 +354,28 @@ __global__ void __launch_bounds__(Shape<HD, NR>::THREADS, 1) attention_q8_prefil
       const unsigned see_n = (unsigned)max(0, min(TK, pos + 1 - j0) - see_lo);
       bool move = false;
       float corr = 1.f, rs = 0.f;
-      // Both passes go over 64 scores a turn of their loops, which stay loops: unrolled whole they are more instructions than the caches
-      // near the schedulers hold.  32 scores come while the 32 before are worked on.
       auto turn = [&](auto masked) {
         constexpr bool MASK = decltype(masked)::value;
-        uint32_t buf[2][32];
+        uint32_t sv[TK];
+#pragma unroll
+        for (int c = 0; c < TK / 32; ++c) tmem_ld32(s_addr + c * 32, *reinterpret_cast<uint32_t(*)[32]>(sv + c * 32));
+        tmem_wait_ld();
         float mx = -INFINITY;
-        auto largest = [&](const uint32_t(&sv)[32], int c) {
 #pragma unroll
-          for (int h = 0; h < 2; ++h) {
-            float top[2] = {-INFINITY, -INFINITY};
+        for (int h = 0; h < GROUPS; ++h) {
+          float top[2] = {-INFINITY, -INFINITY};
 #pragma unroll
-            for (int i = 0; i < 16; i += 2) {
-              float s0 = __uint_as_float(sv[h * 16 + i]), s1 = __uint_as_float(sv[h * 16 + i + 1]);
-              if (MASK) {
-                s0 = (unsigned)(c * 32 + h * 16 + i - see_lo) < see_n ? s0 : -INFINITY;
-                s1 = (unsigned)(c * 32 + h * 16 + i + 1 - see_lo) < see_n ? s1 : -INFINITY;
-              }
-              top[i >> 1 & 1] = max3(top[i >> 1 & 1], s0, s1);
+          for (int i = 0; i < 16; i += 2) {
+            if (MASK) {
+              if ((unsigned)(h * 16 + i - see_lo) >= see_n) sv[h * 16 + i] = 0xff800000u;
+              if ((unsigned)(h * 16 + i + 1 - see_lo) >= see_n) sv[h * 16 + i + 1] = 0xff800000u;
             }
-            const float4 x = sc[2 * c + h];
-            const float best = fmaxf(top[0], top[1]);
-            // (nothing seen: no maximum, whatever the factor)
-            mx = fmaxf(mx, MASK && best == -INFINITY ? -INFINITY : fmaf(best, x.x * factor, x.y));
+            top[i >> 1 & 1] = max3(top[i >> 1 & 1], __uint_as_float(sv[h * 16 + i]), __uint_as_float(sv[h * 16 + i + 1]));
           }
-        };
-        tmem_ld32(s_addr, buf[0]);
-#pragma unroll 1
-        for (int c = 0; c < TK / 32; c += 2) {
-          tmem_wait_ld();
-          tmem_ld32(s_addr + (c + 1) * 32, buf[1]);
-          largest(buf[0], c);
-          tmem_wait_ld();
-          tmem_ld32(s_addr + (c + 2) % (TK / 32) * 32, buf[0]);    // (at last the first ones again, for the weights)
-          largest(buf[1], c + 1);
+          const float4 x = sc[h];
+          const float best = fmaxf(top[0], top[1]);
+          // (nothing seen: no maximum, whatever the factor)
+          mx = fmaxf(mx, MASK && best == -INFINITY ? -INFINITY : fmaf(best, x.x * factor, x.y));
         }
         move = mx > m_ref + RESCALE_STEP || (m_ref == -INFINITY && mx > -INFINITY);
         if (move) {
@@ -384,37 +383,25 @@ __global__ void __launch_bounds__(Shape<HD, NR>::THREADS, 1) attention_q8_prefil
           m_ref = mx;
         }
         const float m_use = m_ref == -INFINITY ? 0.f : m_ref;
-        auto weights = [&](const uint32_t(&sv)[32], int c) {
-          uint32_t pw[16];
 #pragma unroll
-          for (int h = 0; h < 2; ++h) {
-            const float4 x = sc[2 * c + h];
-            const float f = x.x * factor, add = x.y - m_use;
-            float part[2] = {0.f, 0.f};
+        for (int h = 0; h < GROUPS; ++h) {
+          const float4 x = sc[h];
+          const float f = x.x * factor, add = x.y - m_use;
+          float part[2] = {0.f, 0.f};
 #pragma unroll
-            for (int i = 0; i < 16; i += 2) {
-              float p0 = ex2(fmaf(__uint_as_float(sv[h * 16 + i]), f, add));
-              float p1 = ex2(fmaf(__uint_as_float(sv[h * 16 + i + 1]), f, add));
-              if (MASK) {
-                p0 = (unsigned)(c * 32 + h * 16 + i - see_lo) < see_n ? p0 : 0.f;
-                p1 = (unsigned)(c * 32 + h * 16 + i + 1 - see_lo) < see_n ? p1 : 0.f;
-              }
-              part[0] += p0;
-              part[1] += p1;
-              pw[h * 8 + i / 2] = q8::pack_half(p0, p1);
+          for (int i = 0; i < 16; i += 2) {
+            float p0 = ex2(fmaf(__uint_as_float(sv[h * 16 + i]), f, add));
+            float p1 = ex2(fmaf(__uint_as_float(sv[h * 16 + i + 1]), f, add));
+            if (MASK) {                                            // (a factor of 0 would make a NaN of it)
+              p0 = sv[h * 16 + i] == 0xff800000u ? 0.f : p0;
+              p1 = sv[h * 16 + i + 1] == 0xff800000u ? 0.f : p1;
             }
-            rs = fmaf(part[0] + part[1], x.z, rs);
+            part[0] += p0;
+            part[1] += p1;
+            sv[h * 8 + i / 2] = q8::pack_half(p0, p1);             // (its place has been read)
           }
-          tmem_st16(s_addr + c * 16, pw);                          // over scores that have been read
-        };
-#pragma unroll 1
-        for (int c = 0; c < TK / 32; c += 2) {
-          tmem_wait_ld();
-          tmem_ld32(s_addr + (c + 1) * 32, buf[1]);
-          weights(buf[0], c);
-          tmem_wait_ld();
-          if (c + 2 < TK / 32) tmem_ld32(s_addr + (c + 2) * 32, buf[0]);
-          weights(buf[1], c + 1);
+          rs = fmaf(part[0] + part[1], x.z, rs);
+          if (h % 4 == 3) tmem_st32(s_addr + (h / 4) * 32, *reinterpret_cast<const uint32_t(*)[32]>(sv + (h / 4) * 32));
         }
       };
       if (all_visible) turn(std::false_type());
@@ -485,8 +472,16 @@ int g_row_tiles = 0;
 template <int HD, int NR>
 cudaError_t launch(const PreArgs& a, int B, int max_q_len, cudaStream_t s) {
   using SH = Shape<HD, NR>;
-  static const cudaError_t configured =
-      cudaFuncSetAttribute(attention_q8_prefill_kernel<HD, NR>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)SH::SMEM);
+  constexpr int SOFT = SH::SOFT_WARPS * 32;
+  static_assert(SOFT * SH::SOFT_REGS + (SH::THREADS - SOFT) * SH::OTHER_REGS <= SH::THREADS * 128, "more registers than the block has");
+  static const cudaError_t configured = [] {
+    // the split of registers counts on 128 a thread at launch: with fewer a warpgroup would wait for what nobody gives
+    cudaFuncAttributes attr;
+    const cudaError_t e = cudaFuncGetAttributes(&attr, attention_q8_prefill_kernel<HD, NR>);
+    if (e != cudaSuccess) return e;
+    if (attr.numRegs != 128) return cudaErrorLaunchOutOfResources;
+    return cudaFuncSetAttribute(attention_q8_prefill_kernel<HD, NR>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)SH::SMEM);
+  }();
   if (configured != cudaSuccess) return configured;
   const dim3 grid(ceil_div(max_q_len * (a.H / a.KVH), NR * TQ), a.KVH, B);
   return ts_launch(attention_q8_prefill_kernel<HD, NR>, grid, dim3(SH::THREADS), SH::SMEM, s, a);
