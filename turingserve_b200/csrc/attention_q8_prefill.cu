@@ -75,6 +75,31 @@ __host__ __device__ constexpr uint32_t instr_half(int n, bool b_mn) {
   return (1u << 4) | ((b_mn ? 1u : 0u) << 16) | ((uint32_t)(n >> 3) << 17) | ((uint32_t)(128 >> 4) << 24);
 }
 
+// One lane of the warp.
+__device__ __forceinline__ bool elect_one() {
+  uint32_t p;
+  asm volatile("{\n .reg .pred p;\n elect.sync _|p, 0xffffffff;\n selp.u32 %0, 1, 0, p;\n}\n" : "=r"(p));
+  return p != 0;
+}
+// Shared-memory descriptors of tiles with the 128-byte swizzle: the address (and, MN-major, the distance of 64 elements along that dimension)
+// in the lower half (K-major: 1, unused); 8-row groups 1,024 bytes apart, the version and the swizzle in the upper one.
+constexpr uint32_t DESC_HI = (1024u >> 4) | (1u << 14) | (2u << 29);
+__device__ __forceinline__ uint32_t desc_lo(uint32_t addr) { return (addr & 0x3FFFF) >> 4; }
+template <int ACC>
+__device__ __forceinline__ void mma_ss(uint32_t d, uint32_t a_lo, uint32_t b_lo, uint32_t idesc) {
+  asm volatile(
+      "{\n .reg .pred p;\n .reg .b64 a, b;\n setp.ne.b32 p, %5, 0;\n mov.b64 a, {%1, %3};\n mov.b64 b, {%2, %3};\n"
+      " tcgen05.mma.cta_group::1.kind::f16 [%0], a, b, %4, p;\n}\n"
+      ::"r"(d), "r"(a_lo), "r"(b_lo), "r"(DESC_HI), "r"(idesc), "n"(ACC) : "memory");
+}
+template <int ACC>
+__device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint32_t b_lo, uint32_t idesc) {
+  asm volatile(
+      "{\n .reg .pred p;\n .reg .b64 b;\n setp.ne.b32 p, %5, 0;\n mov.b64 b, {%2, %3};\n"
+      " tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], b, %4, p;\n}\n"
+      ::"r"(d), "r"(a), "r"(b_lo), "r"(DESC_HI), "r"(idesc), "n"(ACC) : "memory");
+}
+
 // Registers a thread of the warpgroup gives back, or takes out of what others gave back.
 template <int N> __device__ __forceinline__ void give_registers() { asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(N)); }
 template <int N> __device__ __forceinline__ void take_registers() { asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(N)); }
@@ -259,31 +284,42 @@ __global__ void __launch_bounds__(Shape<HD, NR>::THREADS, 1) attention_q8_prefil
   } else if (warp >= SH::MMA_WARP) {
     // ================= product issue, one lane =================
     give_registers<SH::OTHER_REGS>();
-    if (warp == SH::MMA_WARP && lane == 0 && n_tiles > 0) {
+    if (warp == SH::MMA_WARP && n_tiles > 0) {
+      // The whole warp walks the loop and waits; one elected lane issues.  (Descriptors stay uniform values that way: their upper halves are
+      // constants, the lower ones advance by constants.)
+      const bool one = elect_one();
+      const uint32_t q_lo = desc_lo(smem_u32(q_s)) | 1u << 16, k_lo = desc_lo(smem_u32(k_s)) | 1u << 16, v_lo = desc_lo(smem_u32(v_s)) | ((HALF_K >> 4) << 16);
       auto issue_s = [&](int r, int t) {
         constexpr uint32_t idesc = instr_half(TK, false);
-        const uint32_t qa = smem_u32(q_s + r * SH::Q_BYTES), ka = smem_u32(k_s + (t % STAGES) * KV_BYTES);
+        const uint32_t qa = q_lo + r * (SH::Q_BYTES >> 4), ka = k_lo + (t % STAGES) * (KV_BYTES >> 4), d = tmem + r * ROW_COLS + (t % NB) * TK;
+        if (one) {
 #pragma unroll
-        for (int ks = 0; ks < HD / 16; ++ks)
-          umma(tmem + r * ROW_COLS + (t % NB) * TK, smem_desc(qa + (ks >> 2) * HALF_Q + (ks & 3) * 32),
-               smem_desc(ka + (ks >> 2) * HALF_K + (ks & 3) * 32), idesc, ks > 0 ? 1u : 0u);
-        umma_commit(&bar_s[NB * r + t % NB]);
-        mbar_arrive(&bar_s[NB * r + t % NB]);
-        if (r == NR - 1) umma_commit(&empty_k[t % STAGES]);
+          for (int ks = 0; ks < HD / 16; ++ks) {
+            const uint32_t aq = qa + ((ks >> 2) * HALF_Q + (ks & 3) * 32 >> 4), ak = ka + ((ks >> 2) * HALF_K + (ks & 3) * 32 >> 4);
+            if (ks == 0) mma_ss<0>(d, aq, ak, idesc);
+            else mma_ss<1>(d, aq, ak, idesc);
+          }
+          umma_commit(&bar_s[NB * r + t % NB]);
+          mbar_arrive(&bar_s[NB * r + t % NB]);
+          if (r == NR - 1) umma_commit(&empty_k[t % STAGES]);
+        }
       };
       auto issue_o = [&](int r, int t) {
         constexpr uint32_t idesc = instr_half(HD, true);
-        const uint32_t va = smem_u32(v_s + (t % STAGES) * KV_BYTES), d = tmem + r * ROW_COLS + O_COL;
+        const uint32_t va = v_lo + (t % STAGES) * (KV_BYTES >> 4), d = tmem + r * ROW_COLS + O_COL, pa = tmem + r * ROW_COLS + (t % NB) * TK;
+        if (one) {
+          if (t == 0) mma_ts<0>(d, pa, va, idesc);
+          else mma_ts<1>(d, pa, va, idesc);
 #pragma unroll
-        for (int kk = 0; kk < TK / 16; ++kk)
-          umma_ts(d, tmem + r * ROW_COLS + (t % NB) * TK + kk * 8, smem_desc_mn(va + kk * 16 * 128, HALF_K), idesc, (t > 0 || kk > 0) ? 1u : 0u);
-        if (r == NR - 1) umma_commit(&empty_v[t % STAGES]);
-        umma_commit(&bar_pv[r]);
-        if (t + 1 == n_tiles) umma_commit(&bar_o[r]);
+          for (int kk = 1; kk < TK / 16; ++kk) mma_ts<1>(d, pa + kk * 8, va + (kk * 16 * 128 >> 4), idesc);
+          if (r == NR - 1) umma_commit(&empty_v[t % STAGES]);
+          umma_commit(&bar_pv[r]);
+          if (t + 1 == n_tiles) umma_commit(&bar_o[r]);
+        }
       };
       bool ok = mbar_wait(bar_q, 0, a.status, 20, abort_flag);
       for (int t = 0; t < NB && t < n_tiles && ok; ++t) {
-        ok = mbar_wait(&full_k[t % STAGES], 0, a.status, 21, abort_flag);
+        ok = __all_sync(0xffffffffu, mbar_wait(&full_k[t % STAGES], 0, a.status, 21, abort_flag));
         if (!ok) break;
         tc_fence_after();
         for (int r = 0; r < NR; ++r) issue_s(r, t);
@@ -292,11 +328,12 @@ __global__ void __launch_bounds__(Shape<HD, NR>::THREADS, 1) attention_q8_prefil
         for (int r = 0; r < NR && ok; ++r) {
           ok = mbar_wait_spin(&bar_p[NB * r + t % NB], (uint32_t)((t / NB) & 1), a.status, 26, abort_flag);
           if (ok && r == 0) ok = mbar_wait(&full_v[t % STAGES], (uint32_t)((t / STAGES) & 1), a.status, 23, abort_flag);
+          ok = __all_sync(0xffffffffu, ok);
           if (!ok) break;
           tc_fence_after();
           issue_o(r, t);
           if (t + NB < n_tiles) {
-            if (r == 0) ok = mbar_wait(&full_k[(t + NB) % STAGES], (uint32_t)(((t + NB) / STAGES) & 1), a.status, 28, abort_flag);
+            if (r == 0) ok = __all_sync(0xffffffffu, mbar_wait(&full_k[(t + NB) % STAGES], (uint32_t)(((t + NB) / STAGES) & 1), a.status, 28, abort_flag));
             if (!ok) break;
             tc_fence_after();
             issue_s(r, t + NB);                                    // over P(t), behind the product that reads it
