@@ -10,8 +10,9 @@
 // Softmax: four warps a row tile, a thread a row = tensor-memory lane, which holds a turn's 128 scores in registers: their maximum (the
 // scale of 16 keys is one factor, so that is the maximum of the products, three an instruction, and one multiply-add), then the weights, which
 // go back over the scores as pairs of half floats.  One warp issues the products (one lane): S(t) = Q K(t)^T, O += P(t) V(t) with
-// P read from tensor memory.  Four warps (eight where NR = 1) turn the pages' bytes into half floats, half of them the keys: 16 bytes a piece, brought
-// by cp.async to a place that its thread alone reads, 128 rows and more ahead of the conversion, stored with the 128-byte swizzle that the products read (values with keys along
+// P read from tensor memory.  Seven
+// warps (eleven where NR = 1) turn the pages' bytes into half floats, 16 rows of keys or values a job: 16 bytes a piece, brought by
+// cp.async to a place that its lane alone reads while other rows are converted, stored with the 128-byte swizzle that the products read (values with keys along
 // the rows: MN-major).  Rows outside the visible range are zeros.
 // NR = 2: a score buffer each, so that the softmax of one row tile runs beside the products of the other; a converted tile serves 256 rows;
 // tensor memory is full and a block fills an SM.  NR = 1, for launches of few row tiles, which are as slow as their longest block: two score
@@ -31,27 +32,27 @@ namespace {
 
 using namespace tc;
 
-constexpr int TQ = 128, TK = 128, UNIT = 64, STAGES = 2, SCALE_STAGES = 4;
+constexpr int TQ = 128, TK = 128, STAGES = 2, SCALE_STAGES = 4;
 constexpr float RESCALE_STEP = 8.f;
 constexpr float LOG2E_P = 1.4426950408889634f;
 
 template <int HD, int NR>
 struct Shape {
   static constexpr int NB = NR == 1 ? 2 : 1;                       // score buffers of a row tile
-  // four warpgroups, each with its own number of registers a thread: softmax (one or two), conversion, and the one whose first warp issues
-  // the products.  128 a thread are there; what the others give back the softmax takes: 256 x 200 + 256 x 56, 128 x 232 + 384 x 88.
-  static constexpr int SOFT_WARPS = 4 * NR, CONV_WARPS = NR == 1 ? 8 : 4, CONV_WARP = SOFT_WARPS, MMA_WARP = CONV_WARP + CONV_WARPS;
-  static constexpr int THREADS = 512, SOFT_REGS = NR == 1 ? 232 : 200, OTHER_REGS = NR == 1 ? 88 : 56;
+  // 16 warps in four warpgroups: softmax (one or two), then the converters and, the last warp, the one that issues the products.  128 registers a
+  // thread are there; what the others give back the softmax takes: 256 x 200 + 256 x 56, 128 x 232 + 384 x 88.
+  static constexpr int THREADS = 512, SOFT_WARPS = 4 * NR, MMA_WARP = 15, CONV_WARPS = MMA_WARP - SOFT_WARPS;
+  static constexpr int SOFT_REGS = NR == 1 ? 232 : 200, OTHER_REGS = NR == 1 ? 88 : 56;
   static constexpr uint32_t Q_BYTES = TQ * HD * 2, KV_BYTES = TK * HD * 2, HALF_Q = TQ * 128, HALF_K = TK * 128;
   static constexpr uint32_t O_COL = NB * TK, ROW_COLS = O_COL + HD; // tensor-memory columns of a row tile: scores, O
   static constexpr uint32_t TMEM_COLS = ROW_COLS * NR <= 256 ? 256 : 512;
   static constexpr int BARS = 4 * STAGES + NR * (2 * NB + 2) + 1;
-  // rows on their way from the pages: so many times 64 ahead of the conversion
-  static constexpr int AHEAD = NR == 2 && HD == 128 ? 2 : 4;
-  static constexpr uint32_t RAW_BYTES = UNIT * HD;
-  static constexpr size_t TILES = NR * Q_BYTES + 2 * STAGES * KV_BYTES + 2 * AHEAD * RAW_BYTES;
-  // behind the tiles: scales [4][8] float4, scales on their way [AHEAD][2][4], barriers, the tensor memory's address, the abort flag
-  static constexpr size_t SMEM = TILES + SCALE_STAGES * (TK / 16) * 16 + AHEAD * 32 + BARS * 8 + 16;
+  // 16 rows of keys or of values are a converter's job; so many jobs of its are on their way from the pages
+  static constexpr int AHEAD = 2;
+  static constexpr uint32_t JOB_BYTES = 16 * HD;
+  static constexpr size_t TILES = NR * Q_BYTES + 2 * STAGES * KV_BYTES + CONV_WARPS * AHEAD * JOB_BYTES;
+  // behind the tiles: scales [4][8] float4, scales on their way [converters][AHEAD][2], barriers, the tensor memory's address, the abort flag
+  static constexpr size_t SMEM = TILES + SCALE_STAGES * (TK / 16) * 16 + CONV_WARPS * AHEAD * 8 + BARS * 8 + 16;
 };
 
 struct PreArgs {
@@ -120,10 +121,10 @@ __global__ void __launch_bounds__(Shape<HD, NR>::THREADS, 1) attention_q8_prefil
   unsigned char* q_s = smem;                                       // [NR][HD / 64][128][128 B]
   unsigned char* k_s = q_s + NR * SH::Q_BYTES;                     // [STAGES][HD / 64][128][128 B]
   unsigned char* v_s = k_s + STAGES * KV_BYTES;
-  unsigned char* raw_s = v_s + STAGES * KV_BYTES;                  // [2][AHEAD][pieces a thread][threads][16 B]
-  float4* scale_s = reinterpret_cast<float4*>(raw_s + 2 * SH::AHEAD * SH::RAW_BYTES);      // [SCALE_STAGES][GROUPS]
-  float* raw_scale = reinterpret_cast<float*>(scale_s + SCALE_STAGES * GROUPS);            // [AHEAD][2][4]
-  uint64_t* full_k = reinterpret_cast<uint64_t*>(raw_scale + SH::AHEAD * 8);
+  unsigned char* raw_s = v_s + STAGES * KV_BYTES;                  // [converters][AHEAD][pieces a lane][32 lanes][16 B]
+  float4* scale_s = reinterpret_cast<float4*>(raw_s + SH::CONV_WARPS * SH::AHEAD * SH::JOB_BYTES);        // [SCALE_STAGES][GROUPS]
+  float* raw_scale = reinterpret_cast<float*>(scale_s + SCALE_STAGES * GROUPS);                           // [converters][AHEAD][2]
+  uint64_t* full_k = reinterpret_cast<uint64_t*>(raw_scale + SH::CONV_WARPS * SH::AHEAD * 2);
   uint64_t* empty_k = full_k + STAGES;
   uint64_t* full_v = empty_k + STAGES;
   uint64_t* empty_v = full_v + STAGES;
@@ -149,9 +150,9 @@ __global__ void __launch_bounds__(Shape<HD, NR>::THREADS, 1) attention_q8_prefil
   const int prefix = seq_len - q_len;
   if (tid == 0) {
     for (int s = 0; s < STAGES; ++s) {
-      mbar_init(&full_k[s], SH::CONV_WARPS / 2 * (TK / UNIT));
+      mbar_init(&full_k[s], GROUPS);
       mbar_init(&empty_k[s], 1);
-      mbar_init(&full_v[s], SH::CONV_WARPS / 2 * (TK / UNIT));
+      mbar_init(&full_v[s], GROUPS);
       mbar_init(&empty_v[s], 1);
     }
     for (int r = 0; r < NR; ++r) {
@@ -188,161 +189,12 @@ __global__ void __launch_bounds__(Shape<HD, NR>::THREADS, 1) attention_q8_prefil
   const int tok = row_ok ? row / G : 0, g = row_ok ? row % G : 0;
   const int pos = row_ok ? prefix + tok : -1;
 
-  if (warp >= SH::CONV_WARP && warp < SH::MMA_WARP) {
-    // ================= converters: the first half of the warps the keys (and the scales), the others the values =================
-    give_registers<SH::OTHER_REGS>();
-    constexpr int CT = SH::CONV_WARPS * 16;                        // threads of each half
-    constexpr int CPR = HD / 16, NP = UNIT * CPR / CT;             // 16-byte pieces of a row; pieces a thread takes of 64 rows
-    constexpr int RPP = CT / CPR, SAME = RPP < 16 ? 16 / RPP : 1;  // rows that they cover with a piece each; pieces within 16 rows
-    const bool keys = warp < SH::CONV_WARP + SH::CONV_WARPS / 2;
-    const int ct = (tid - SH::CONV_WARP * 32) % CT, c16 = ct % CPR, r0 = ct / CPR;
-    const unsigned char* cache = keys ? a.cache[0] : a.cache[1];
-    const int* table = a.block_tables + (size_t)b * a.table_width;
-    const int n_units = n_tiles * (TK / UNIT);
-    // the page and the place in it of 16 keys, a lane, of 512 rows: -1 outside; fetched that many rows ahead
-    int pg = -1, in_page = 0, pg_next, in_next;
-    auto fetch_pages = [&](int block) {
-      const int j = j_lo + block * 512 + lane * 16, lp = j / a.page;
-      in_next = j - lp * a.page;
-      pg_next = (j <= j_hi && lp < a.table_width) ? table[lp] : -1;
-    };
-    fetch_pages(0);
-    // 64 rows from the pages, asynchronously: a thread's pieces go to a place of its own, which it alone reads
-    unsigned char* raw = raw_s + (keys ? 0 : SH::AHEAD * SH::RAW_BYTES) + ct * 16;
-    auto issue = [&](int u) {
-      if (u < n_units) {
-        if (u % 8 == 0) {
-          pg = pg_next;
-          in_page = in_next;
-          fetch_pages(u / 8 + 1);
-        }
-        unsigned char* dst = raw + (u % SH::AHEAD) * SH::RAW_BYTES;
-        const unsigned char* src = cache;
-        bool page = false;
-#pragma unroll
-        for (int i = 0; i < NP; ++i) {
-          const int r = r0 + i * RPP, j = j_lo + u * UNIT + r;
-          if (i % SAME == 0) {
-            const int p = __shfl_sync(0xffffffffu, pg, (u % 8) * 4 + (r >> 4)), in = __shfl_sync(0xffffffffu, in_page, (u % 8) * 4 + (r >> 4));
-            src = cache + (((size_t)max(p, 0) * a.KVH + kvh) * a.page + in + (r & 15)) * HD + c16 * 16;
-            page = p >= 0;
-          }
-          cp_async_16(dst + i * (CT * 16), src + (i % SAME) * RPP * HD, page && j >= key_lo && j <= j_hi);
-        }
-        if (warp == SH::CONV_WARP) {
-          const int p = __shfl_sync(0xffffffffu, pg, (u % 8) * 4 + (lane & 3));
-          const size_t at = (size_t)max(p, 0) * a.KVH + kvh;
-          if (lane < 8) cp_async_4(raw_scale + (u % SH::AHEAD) * 8 + lane, (lane < 4 ? a.scales[0] : a.scales[1]) + at, p >= 0);
-        }
-      }
-      cp_async_commit();
-    };
-#pragma unroll 1
-    for (int u = 0; u < SH::AHEAD; ++u) issue(u);
-    bool ok = true;
-    for (int u = 0; u < n_units; ++u) {
-      const int t = u / (TK / UNIT), half = u % (TK / UNIT), st = t % STAGES;
-      if (half == 0 && t >= STAGES) {
-        ok = mbar_wait(keys ? &empty_k[st] : &empty_v[st], (uint32_t)((t / STAGES - 1) & 1), a.status, keys ? 24 : 27, abort_flag);
-        ok = __all_sync(0xffffffffu, ok);
-        if (!ok) break;
-      }
-      cp_async_wait<SH::AHEAD - 1>();
-      unsigned char* tile = (keys ? k_s : v_s) + st * KV_BYTES + half * UNIT * 128;
-      const unsigned char* src = raw + (u % SH::AHEAD) * SH::RAW_BYTES;
-#pragma unroll
-      for (int i = 0; i < NP; ++i) {
-        const int r = r0 + i * RPP, odd = c16 >> 2 & (HD == 128 ? 1 : 0);
-        const uint4 piece = *reinterpret_cast<const uint4*>(src + i * (CT * 16));
-        uint4 lo, hi;
-        q8::halves_of(piece.x, lo.x, lo.y);
-        q8::halves_of(piece.y, lo.z, lo.w);
-        q8::halves_of(piece.z, hi.x, hi.y);
-        q8::halves_of(piece.w, hi.z, hi.w);
-        // columns 16 c16 .. of the row: half c16 / 4 of the head, pieces 2 (c16 & 3) and the next; the second half's lanes begin with
-        // the second piece, so that a row's eight lanes write to eight different places of a line
-        unsigned char* line = tile + (c16 >> 2) * HALF_K + r * 128;
-        const int first = 2 * (c16 & 3);
-        *reinterpret_cast<uint4*>(line + (((first + odd) ^ (r & 7)) << 4)) = odd ? hi : lo;
-        *reinterpret_cast<uint4*>(line + (((first + 1 - odd) ^ (r & 7)) << 4)) = odd ? lo : hi;
-      }
-      if (warp == SH::CONV_WARP) {
-        __syncwarp();                                              // (lanes 4 to 7 brought the values' scales)
-        if (lane < 4) {
-          const float ks = raw_scale[(u % SH::AHEAD) * 8 + lane], vs = raw_scale[(u % SH::AHEAD) * 8 + 4 + lane];
-          // (score factor, log2 of the value's scale, its inverse) of 16 keys
-          scale_s[(t % SCALE_STAGES) * GROUPS + half * 4 + lane] =
-              make_float4(vs != vs ? vs : ks, (float)((int)(__float_as_uint(vs) >> 23) - 127), q8::inverse_scale(vs), 0.f);
-        }
-      }
-      fence_async_smem();
-      __syncwarp();
-      if (lane == 0) mbar_arrive(keys ? &full_k[st] : &full_v[st]);
-      issue(u + SH::AHEAD);
-    }
-    cp_async_wait<0>();
-  } else if (warp >= SH::MMA_WARP) {
-    // ================= product issue, one lane =================
-    give_registers<SH::OTHER_REGS>();
-    if (warp == SH::MMA_WARP && n_tiles > 0) {
-      // The whole warp walks the loop and waits; one elected lane issues.  (Descriptors stay uniform values that way: their upper halves are
-      // constants, the lower ones advance by constants.)
-      const bool one = elect_one();
-      const uint32_t q_lo = desc_lo(smem_u32(q_s)) | 1u << 16, k_lo = desc_lo(smem_u32(k_s)) | 1u << 16, v_lo = desc_lo(smem_u32(v_s)) | ((HALF_K >> 4) << 16);
-      auto issue_s = [&](int r, int t) {
-        constexpr uint32_t idesc = instr_half(TK, false);
-        const uint32_t qa = q_lo + r * (SH::Q_BYTES >> 4), ka = k_lo + (t % STAGES) * (KV_BYTES >> 4), d = tmem + r * ROW_COLS + (t % NB) * TK;
-        if (one) {
-#pragma unroll
-          for (int ks = 0; ks < HD / 16; ++ks) {
-            const uint32_t aq = qa + ((ks >> 2) * HALF_Q + (ks & 3) * 32 >> 4), ak = ka + ((ks >> 2) * HALF_K + (ks & 3) * 32 >> 4);
-            if (ks == 0) mma_ss<0>(d, aq, ak, idesc);
-            else mma_ss<1>(d, aq, ak, idesc);
-          }
-          umma_commit(&bar_s[NB * r + t % NB]);
-          mbar_arrive(&bar_s[NB * r + t % NB]);
-          if (r == NR - 1) umma_commit(&empty_k[t % STAGES]);
-        }
-      };
-      auto issue_o = [&](int r, int t) {
-        constexpr uint32_t idesc = instr_half(HD, true);
-        const uint32_t va = v_lo + (t % STAGES) * (KV_BYTES >> 4), d = tmem + r * ROW_COLS + O_COL, pa = tmem + r * ROW_COLS + (t % NB) * TK;
-        if (one) {
-          if (t == 0) mma_ts<0>(d, pa, va, idesc);
-          else mma_ts<1>(d, pa, va, idesc);
-#pragma unroll
-          for (int kk = 1; kk < TK / 16; ++kk) mma_ts<1>(d, pa + kk * 8, va + (kk * 16 * 128 >> 4), idesc);
-          if (r == NR - 1) umma_commit(&empty_v[t % STAGES]);
-          umma_commit(&bar_pv[r]);
-          if (t + 1 == n_tiles) umma_commit(&bar_o[r]);
-        }
-      };
-      bool ok = mbar_wait(bar_q, 0, a.status, 20, abort_flag);
-      for (int t = 0; t < NB && t < n_tiles && ok; ++t) {
-        ok = __all_sync(0xffffffffu, mbar_wait(&full_k[t % STAGES], 0, a.status, 21, abort_flag));
-        if (!ok) break;
-        tc_fence_after();
-        for (int r = 0; r < NR; ++r) issue_s(r, t);
-      }
-      for (int t = 0; t < n_tiles && ok; ++t)
-        for (int r = 0; r < NR && ok; ++r) {
-          ok = mbar_wait_spin(&bar_p[NB * r + t % NB], (uint32_t)((t / NB) & 1), a.status, 26, abort_flag);
-          if (ok && r == 0) ok = mbar_wait(&full_v[t % STAGES], (uint32_t)((t / STAGES) & 1), a.status, 23, abort_flag);
-          ok = __all_sync(0xffffffffu, ok);
-          if (!ok) break;
-          tc_fence_after();
-          issue_o(r, t);
-          if (t + NB < n_tiles) {
-            if (r == 0) ok = __all_sync(0xffffffffu, mbar_wait(&full_k[(t + NB) % STAGES], (uint32_t)(((t + NB) / STAGES) & 1), a.status, 28, abort_flag));
-            if (!ok) break;
-            tc_fence_after();
-            issue_s(r, t + NB);                                    // over P(t), behind the product that reads it
-          }
-        }
-    }
-  } else {
+  // (a warpgroup takes or gives as one: its four warps at the same instruction)
+  if (softmax) take_registers<SH::SOFT_REGS>();
+  else give_registers<SH::OTHER_REGS>();
+
+  if (softmax) {
     // ================= softmax: a thread a row = tensor-memory lane =================
-    take_registers<SH::SOFT_REGS>();
     // Q rows -> shared memory as half floats, K-major with the 128-byte swizzle (16-byte piece c of row r at c ^ (r & 7))
     float factor = 0.f;
     {
@@ -496,6 +348,145 @@ __global__ void __launch_bounds__(Shape<HD, NR>::THREADS, 1) attention_q8_prefil
           }
         }
       }
+    }
+  } else if (warp != SH::MMA_WARP) {
+    // ================= converters: each warp takes every CONV_WARPS-th job, 16 rows of keys (and their scales) or of values =================
+    constexpr int CPR = HD / 16, NP = CPR / 2, RPP = 32 / CPR;     // 16-byte pieces of a row; pieces a lane takes; rows the lanes cover with one each
+    // A lane's piece c16 of rows r0, r0 + RPP, ...: eight neighbouring lanes have four pieces of two rows, whose stores (every other piece of a
+    // line of the converted tile, swapped by the row's number) then go to eight different places of a line.
+    const int cw = warp - SH::SOFT_WARPS;
+    const int c16 = HD == 128 ? (lane & 3) + (lane >> 1 & 4) : lane & 3, r0 = HD == 128 ? (lane >> 2 & 1) + (lane >> 4) * 2 : lane >> 2;
+    const int* table = a.block_tables + (size_t)b * a.table_width;
+    const int n_jobs = n_tiles * 2 * GROUPS;
+    // the page and the place in it of 16 keys, a lane, of 512 rows: -1 outside; fetched that many rows ahead
+    int pg = -1, in_page = 0, pg_next, in_next, block = -1;
+    auto fetch_pages = [&](int blk) {
+      const int j = j_lo + blk * 512 + lane * 16, lp = j / a.page;
+      in_next = j - lp * a.page;
+      pg_next = (j <= j_hi && lp < a.table_width) ? table[lp] : -1;
+    };
+    fetch_pages(0);
+    // a job's rows from its page, asynchronously: a lane's pieces go to a place of its own, which it alone reads
+    unsigned char* raw = raw_s + cw * SH::AHEAD * SH::JOB_BYTES + lane * 16;
+    float* raw_sc = raw_scale + cw * SH::AHEAD * 2;
+    auto issue = [&](int job, int slot) {
+      if (job < n_jobs) {
+        const int t = job / (2 * GROUPS), kv = job / GROUPS & 1, grp = job % GROUPS;
+        if (t / 4 != block) {
+          block = t / 4;
+          pg = pg_next;
+          in_page = in_next;
+          fetch_pages(block + 1);
+        }
+        const int p = __shfl_sync(0xffffffffu, pg, (t & 3) * GROUPS + grp), in = __shfl_sync(0xffffffffu, in_page, (t & 3) * GROUPS + grp);
+        const size_t at = (size_t)max(p, 0) * a.KVH + kvh;
+        const unsigned char* src = (kv ? a.cache[1] : a.cache[0]) + (at * a.page + in + r0) * HD + c16 * 16;
+        const int j0 = j_lo + t * TK + grp * 16 + r0;
+#pragma unroll
+        for (int i = 0; i < NP; ++i)
+          cp_async_16(raw + slot * SH::JOB_BYTES + i * 512, src + i * RPP * HD, p >= 0 && j0 + i * RPP >= key_lo && j0 + i * RPP <= j_hi);
+        if (kv == 0 && lane < 2) cp_async_4(raw_sc + slot * 2 + lane, (lane == 0 ? a.scales[0] : a.scales[1]) + at, p >= 0);
+      }
+      cp_async_commit();
+    };
+#pragma unroll 1
+    for (int i = 0; i < SH::AHEAD; ++i) issue(cw + i * SH::CONV_WARPS, i);
+    bool ok = true;
+    for (int job = cw, slot = 0; job < n_jobs; job += SH::CONV_WARPS, slot = (slot + 1) % SH::AHEAD) {
+      const int t = job / (2 * GROUPS), kv = job / GROUPS & 1, grp = job % GROUPS, st = t % STAGES;
+      if (t >= STAGES) {
+        ok = mbar_wait(kv ? &empty_v[st] : &empty_k[st], (uint32_t)((t / STAGES - 1) & 1), a.status, kv ? 27 : 24, abort_flag);
+        ok = __all_sync(0xffffffffu, ok);
+        if (!ok) break;
+      }
+      cp_async_wait<SH::AHEAD - 1>();
+      // columns 16 c16 .. of the row: half c16 / 4 of the head, pieces 2 (c16 & 3) and the next
+      unsigned char* line = (kv ? v_s : k_s) + st * KV_BYTES + (c16 >> 2) * HALF_K + (grp * 16 + r0) * 128;
+      const int lo_at = (2 * (c16 & 3) ^ (r0 & 7)) << 4;           // (the next piece's is this one's last bit turned; four rows on, the third)
+#pragma unroll
+      for (int i = 0; i < NP; ++i) {
+        const uint4 piece = *reinterpret_cast<const uint4*>(raw + slot * SH::JOB_BYTES + i * 512);
+        uint4 lo, hi;
+        q8::halves_of(piece.x, lo.x, lo.y);
+        q8::halves_of(piece.y, lo.z, lo.w);
+        q8::halves_of(piece.z, hi.x, hi.y);
+        q8::halves_of(piece.w, hi.z, hi.w);
+        const int swap = lo_at ^ (i * RPP % 8 << 4);
+        *reinterpret_cast<uint4*>(line + i * RPP * 128 + swap) = lo;
+        *reinterpret_cast<uint4*>(line + i * RPP * 128 + (swap ^ 16)) = hi;
+      }
+      if (kv == 0) {
+        __syncwarp();                                              // (lane 1 brought the values' scale)
+        if (lane == 0) {
+          const float ks = raw_sc[slot * 2], vs = raw_sc[slot * 2 + 1];
+          // (score factor, log2 of the value's scale, its inverse) of the 16 keys
+          scale_s[(t % SCALE_STAGES) * GROUPS + grp] =
+              make_float4(vs != vs ? vs : ks, (float)((int)(__float_as_uint(vs) >> 23) - 127), q8::inverse_scale(vs), 0.f);
+        }
+      }
+      fence_async_smem();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(kv ? &full_v[st] : &full_k[st]);
+      issue(job + SH::AHEAD * SH::CONV_WARPS, slot);
+    }
+    cp_async_wait<0>();
+  } else {
+    // ================= product issue, one lane =================
+    if (n_tiles > 0) {
+      // The whole warp walks the loop and waits; one elected lane issues.  (Descriptors stay uniform values that way: their upper halves are
+      // constants, the lower ones advance by constants.)
+      const bool one = elect_one();
+      const uint32_t q_lo = desc_lo(smem_u32(q_s)) | 1u << 16, k_lo = desc_lo(smem_u32(k_s)) | 1u << 16, v_lo = desc_lo(smem_u32(v_s)) | ((HALF_K >> 4) << 16);
+      auto issue_s = [&](int r, int t) {
+        constexpr uint32_t idesc = instr_half(TK, false);
+        const uint32_t qa = q_lo + r * (SH::Q_BYTES >> 4), ka = k_lo + (t % STAGES) * (KV_BYTES >> 4), d = tmem + r * ROW_COLS + (t % NB) * TK;
+        if (one) {
+#pragma unroll
+          for (int ks = 0; ks < HD / 16; ++ks) {
+            const uint32_t aq = qa + ((ks >> 2) * HALF_Q + (ks & 3) * 32 >> 4), ak = ka + ((ks >> 2) * HALF_K + (ks & 3) * 32 >> 4);
+            if (ks == 0) mma_ss<0>(d, aq, ak, idesc);
+            else mma_ss<1>(d, aq, ak, idesc);
+          }
+          umma_commit(&bar_s[NB * r + t % NB]);
+          mbar_arrive(&bar_s[NB * r + t % NB]);
+          if (r == NR - 1) umma_commit(&empty_k[t % STAGES]);
+        }
+      };
+      auto issue_o = [&](int r, int t) {
+        constexpr uint32_t idesc = instr_half(HD, true);
+        const uint32_t va = v_lo + (t % STAGES) * (KV_BYTES >> 4), d = tmem + r * ROW_COLS + O_COL, pa = tmem + r * ROW_COLS + (t % NB) * TK;
+        if (one) {
+          if (t == 0) mma_ts<0>(d, pa, va, idesc);
+          else mma_ts<1>(d, pa, va, idesc);
+#pragma unroll
+          for (int kk = 1; kk < TK / 16; ++kk) mma_ts<1>(d, pa + kk * 8, va + (kk * 16 * 128 >> 4), idesc);
+          if (r == NR - 1) umma_commit(&empty_v[t % STAGES]);
+          umma_commit(&bar_pv[r]);
+          if (t + 1 == n_tiles) umma_commit(&bar_o[r]);
+        }
+      };
+      bool ok = mbar_wait(bar_q, 0, a.status, 20, abort_flag);
+      for (int t = 0; t < NB && t < n_tiles && ok; ++t) {
+        ok = __all_sync(0xffffffffu, mbar_wait(&full_k[t % STAGES], 0, a.status, 21, abort_flag));
+        if (!ok) break;
+        tc_fence_after();
+        for (int r = 0; r < NR; ++r) issue_s(r, t);
+      }
+      for (int t = 0; t < n_tiles && ok; ++t)
+        for (int r = 0; r < NR && ok; ++r) {
+          ok = mbar_wait_spin(&bar_p[NB * r + t % NB], (uint32_t)((t / NB) & 1), a.status, 26, abort_flag);
+          if (ok && r == 0) ok = mbar_wait(&full_v[t % STAGES], (uint32_t)((t / STAGES) & 1), a.status, 23, abort_flag);
+          ok = __all_sync(0xffffffffu, ok);
+          if (!ok) break;
+          tc_fence_after();
+          issue_o(r, t);
+          if (t + NB < n_tiles) {
+            if (r == 0) ok = __all_sync(0xffffffffu, mbar_wait(&full_k[(t + NB) % STAGES], (uint32_t)(((t + NB) / STAGES) & 1), a.status, 28, abort_flag));
+            if (!ok) break;
+            tc_fence_after();
+            issue_s(r, t + NB);                                    // over P(t), behind the product that reads it
+          }
+        }
     }
   }
   tc_fence_before();
