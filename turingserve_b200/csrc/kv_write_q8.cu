@@ -114,7 +114,7 @@ __global__ void kv_write_q8_kernel(const WriteArgs a) {
 //   sides until the first and the last run end: their largest values then are every block's that shares a run, no block waits for
 //   another, and all compute the same scale (the scale that a page had is a lower bound: reading it after the run's first
 //   block has put the new one there gives the same).  The run's first block brings the page's other rows to a larger scale.
-// What bounds it: a few tokens the chain of loads (slots, rows, scale: three trips), thousands the bytes of qkv once and of the
+// What bounds it: a few tokens the chain of loads (slots and rows, then the scale: two trips), thousands the bytes of qkv once and of the
 // outputs, at 64 tokens a block the rows read twice come out of L1 or L2.
 constexpr int FAST_THREADS = 128, SPAN_MAX = 64;
 
@@ -221,12 +221,35 @@ __global__ void __launch_bounds__(FAST_THREADS) kv_write_q8_fast_kernel(const Fa
   __shared__ int slot_s[SPAN_MAX], lead_s[SPAN_MAX], edge_s[2], fresh_s[SPAN_MAX];
   __shared__ unsigned mask_s[2][2], amax_s[SPAN_MAX];             // leaders, live tokens
   __shared__ float inv_s[SPAN_MAX];
+  const int col = (a.H + kv * a.KVH + kvh) * D + 8 * j;
+  auto load_row = [&](int t, float (&x)[16]) {
+    load16<PART>(f, t, row_elems, col, col + HALF, x);
+    if (kv == 0 && a.rot) {
+      float c[8], s[8];
+      load_table(a, t, HALF, j, c, s);
+      turn(x, c, s);
+    }
+  };
+  // All that the first trip to memory can bring: the span's slots, 128 slots to either side (its first and last run may go on there), and
+  // the span's rows, if it is no more of them than the block takes in one turn.
+  const bool back = tid < 32;
+  int around[4];
+  if (tid < 64) {
+#pragma unroll
+    for (int u = 0; u < 4; ++u) {
+      const int t = back ? w0 - 1 - (u * 32 + lane) : w1 + u * 32 + lane;
+      around[u] = t >= 0 && t < a.T ? a.slots[t] : -2;
+    }
+  }
   if (tid < SPAN_MAX) {
     const int t = w0 + tid;
     slot_s[tid] = t < w1 ? a.slots[t] : -1;
     fresh_s[tid] = 0;
     amax_s[tid] = 0;
   }
+  float x[16];
+  const bool short_span = f.span <= ROWS;
+  if (short_span && w0 + r < w1) load_row(w0 + r, x);
   __syncthreads();
   if (tid < SPAN_MAX) {
     const int s = slot_s[tid];
@@ -245,24 +268,22 @@ __global__ void __launch_bounds__(FAST_THREADS) kv_write_q8_fast_kernel(const Fa
   if (live == 0) return;
   const int n_runs = __popcll(leads);
   auto run_at = [&](int i) { return __popcll(leads & (~0ull >> (63 - i))) - 1; };
-  if (tid < SPAN_MAX && (leads >> tid & 1)) lead_s[run_at(tid)] = tid;
+  // the scales that the runs' pages have: on their way while the rows' maxima are found
+  float held = 0.f;
+  if (tid < SPAN_MAX && (leads >> tid & 1)) {
+    lead_s[run_at(tid)] = tid;
+    held = a.scale[kv][(size_t)(slot_s[tid] / a.page) * a.KVH + kvh];
+  }
   if (tid < 64) {
     // where the first run begins (warp 0) and the last one ends (warp 1): 128 tokens a turn
-    const bool back = tid < 32;
     const int pg = slot_s[back ? __ffsll((long long)live) - 1 : 63 - __clzll((long long)live)] / a.page;
     int edge = back ? w0 : w1, at = back ? w0 - 1 : w1;           // tokens [edge of the run]; next token to look at
     for (;;) {
-      int s[4];
-#pragma unroll
-      for (int u = 0; u < 4; ++u) {
-        const int t = back ? at - (u * 32 + lane) : at + u * 32 + lane;
-        s[u] = t >= 0 && t < a.T ? a.slots[t] : -2;
-      }
       bool ended = false;
 #pragma unroll
       for (int u = 0; u < 4 && !ended; ++u) {
-        const unsigned other = __ballot_sync(0xffffffffu, s[u] == -2 || (s[u] >= 0 && s[u] / a.page != pg));
-        unsigned same = __ballot_sync(0xffffffffu, s[u] >= 0 && s[u] / a.page == pg);
+        const unsigned other = __ballot_sync(0xffffffffu, around[u] == -2 || (around[u] >= 0 && around[u] / a.page != pg));
+        unsigned same = __ballot_sync(0xffffffffu, around[u] >= 0 && around[u] / a.page == pg);
         if (other) same &= (other & (~other + 1)) - 1;            // only those before the first that is not of the run
         if (same) {
           const int far = u * 32 + 31 - __clz(same);
@@ -272,28 +293,24 @@ __global__ void __launch_bounds__(FAST_THREADS) kv_write_q8_fast_kernel(const Fa
       }
       if (ended) break;
       at += back ? -128 : 128;
+#pragma unroll
+      for (int u = 0; u < 4; ++u) {
+        const int t = back ? at - (u * 32 + lane) : at + u * 32 + lane;
+        around[u] = t >= 0 && t < a.T ? a.slots[t] : -2;
+      }
     }
     if (lane == 0) edge_s[back ? 0 : 1] = edge;
   }
   __syncthreads();
   const int e0 = edge_s[0], e1 = edge_s[1];
-  const int col = (a.H + kv * a.KVH + kvh) * D + 8 * j;
   auto slot_of = [&](int t) { return t >= w0 && t < w1 ? slot_s[t - w0] : a.slots[t]; };
   auto run_of = [&](int t) { return t < w0 ? 0 : (t >= w1 ? n_runs - 1 : run_at(t - w0)); };
-  auto load_row = [&](int t, float (&x)[16]) {
-    load16<PART>(f, t, row_elems, col, col + HALF, x);
-    if (kv == 0 && a.rot) {
-      float c[8], s[8];
-      load_table(a, t, HALF, j, c, s);
-      turn(x, c, s);
-    }
-  };
-  float x[16];
-  for (int base = e0; base < e1; base += ROWS) {                  // (every lane of a warp takes every turn: the maxima are shuffled)
+  const bool own = short_span && e0 >= w0 && e1 <= w1;            // the runs lie in the span, whose rows are in registers
+  for (int base = own ? w0 : e0; base < e1; base += ROWS) {       // (every lane of a warp takes every turn: the maxima are shuffled)
     const int t = base + r, s = t < e1 ? slot_of(t) : -1;
     unsigned amax = 0;
     if (s >= 0) {
-      load_row(t, x);
+      if (!own) load_row(t, x);
 #pragma unroll
       for (int i = 0; i < 16; ++i) amax = max(amax, __float_as_uint(fabsf(x[i])));
     }
@@ -309,12 +326,12 @@ __global__ void __launch_bounds__(FAST_THREADS) kv_write_q8_fast_kernel(const Fa
   // (a run belongs to the block that has its first token)
   auto begins_here = [&](int run) { return run > 0 || e0 >= w0; };
   __shared__ float held_s[SPAN_MAX], now_s[SPAN_MAX];
-  if (tid < n_runs) {
-    const float* sp = a.scale[kv] + (size_t)(slot_s[lead_s[tid]] / a.page) * a.KVH + kvh;
-    const float held = *sp, need = scale_for(amax_s[tid]), now = fresh_s[tid] ? need : larger_scale(held, need);
-    held_s[tid] = held;
-    now_s[tid] = now;
-    inv_s[tid] = inverse_scale(now);
+  if (tid < SPAN_MAX && (leads >> tid & 1)) {
+    const int run = run_at(tid);
+    const float need = scale_for(amax_s[run]), now = fresh_s[run] ? need : larger_scale(held, need);
+    held_s[run] = held;
+    now_s[run] = now;
+    inv_s[run] = inverse_scale(now);
   }
   __syncthreads();
   auto page_rows = [&](int slot) { return a.cache[kv] + ((size_t)(slot / a.page) * a.KVH + kvh) * a.page * D; };
@@ -340,11 +357,10 @@ __global__ void __launch_bounds__(FAST_THREADS) kv_write_q8_fast_kernel(const Fa
       *p = v;
     }
   }
-  const bool once = e1 - e0 <= ROWS;                              // the rows are still in registers
-  for (int t = once ? e0 + r : w0 + r; t < w1; t += ROWS) {
-    const int s = t >= w0 ? slot_s[t - w0] : -1;
+  for (int t = w0 + r; t < w1; t += ROWS) {
+    const int s = slot_s[t - w0];
     if (s < 0) continue;
-    if (!once) load_row(t, x);
+    if (!own) load_row(t, x);
     const float inv = inv_s[run_at(t - w0)];
     unsigned w[4] = {0, 0, 0, 0};
     if (inv != 0.f) {

@@ -7,15 +7,17 @@
 //   block_tables[g, b, i] = tables[g, r, i] for i < ceil(seq_lens[b] / page), else 0, the page that nobody owns
 // after `updates` (group, row, index, page) have gone into the tables; of updates of the same place the last one holds.
 //
-// One block a request, which sums the lengths before its own, puts its row's updates in place and writes its tokens and its
-// table rows; one more block for the updates of rows that are not in the step.  One launch whatever the step: 8 requests of 2,048
-// tokens are bound by its latency; 129 requests with tables of 2,048 entries move 3 MB.  The kernel does not let kernels behind
-// it start early: they may read the maps before they wait.
+// One block a request (several where tables are wide or portions long), which sums the lengths before its own, puts its row's updates in
+// place and writes its tokens and its table rows; one more block puts all updates in place, for rows that are not in the step.
+// Only the update that holds in the end is ever written, so blocks that write the same place write the same value.  One launch
+// whatever the step: 8 requests of 2,048 tokens are bound by its latency (2.0 us in a graph, of which a launch is most); 129 requests
+// with two tables of 2,048 entries and a portion of 1,920 tokens move 3 MB.  The kernel does not let kernels behind it start early: they
+// may read the maps before they wait.
 #include "common.cuh"
 
 namespace {
 
-constexpr int THREADS = 256;
+constexpr int THREADS = 256, UPDATES = 512;
 
 struct MapArgs {
   const int* requests;                 // [3][B]: table row, tokens before, tokens brought
@@ -30,7 +32,9 @@ __global__ void __launch_bounds__(THREADS) step_maps_kernel(const MapArgs a) {
   pdl_wait();
   const int b = blockIdx.x, tid = threadIdx.x;
   const bool extra = b == a.B;
+  if (extra && blockIdx.y > 0) return;
   __shared__ int sums[THREADS / 32];
+  __shared__ int4 up_s[UPDATES];
   const int upto = extra ? a.B : b;
   int mine = 0;
   for (int i = tid; i < upto; i += THREADS) mine += max(0, a.requests[2 * a.B + i]);
@@ -39,15 +43,23 @@ __global__ void __launch_bounds__(THREADS) step_maps_kernel(const MapArgs a) {
   if ((tid & 31) == 0) sums[tid >> 5] = mine;
   const int row = extra ? -1 : a.requests[b], start = extra ? 0 : a.requests[a.B + b], n = extra ? 0 : max(0, a.requests[2 * a.B + b]);
   const bool real = row >= 0 && row < a.R;
-  for (int u = tid; u < a.U; u += THREADS) {
-    const int4 up = a.updates[u];
-    if ((!extra && up.y != row) || up.x < 0 || up.x >= a.G || up.y < 0 || up.y >= a.R || up.z < 0 || up.z >= a.P) continue;
-    bool holds = true;
-    for (int w = u + 1; w < a.U && holds; ++w) {
-      const int4 later = a.updates[w];
-      holds = later.x != up.x || later.y != up.y || later.z != up.z;
+  for (int base = 0; base < a.U; base += UPDATES) {
+    const int count = min(UPDATES, a.U - base);
+    __syncthreads();
+    for (int i = tid; i < count; i += THREADS) up_s[i] = a.updates[base + i];
+    __syncthreads();
+    for (int i = tid; i < count; i += THREADS) {
+      const int4 up = up_s[i];
+      if ((!extra && up.y != row) || up.x < 0 || up.x >= a.G || up.y < 0 || up.y >= a.R || up.z < 0 || up.z >= a.P) continue;
+      bool holds = true;                                           // no later one of the same place
+#pragma unroll 4
+      for (int w = i + 1; w < count; ++w) holds = holds && (up_s[w].x != up.x || up_s[w].y != up.y || up_s[w].z != up.z);
+      for (int w = base + count; w < a.U && holds; ++w) {
+        const int4 later = a.updates[w];
+        holds = later.x != up.x || later.y != up.y || later.z != up.z;
+      }
+      if (holds) a.tables[((size_t)up.x * a.R + up.y) * a.P + up.z] = up.w;
     }
-    if (holds) a.tables[((size_t)up.x * a.R + up.y) * a.P + up.z] = up.w;
   }
   __syncthreads();
   int first = 0;
@@ -62,21 +74,38 @@ __global__ void __launch_bounds__(THREADS) step_maps_kernel(const MapArgs a) {
     }
     return;
   }
-  const int len = real ? start + n : 0, live = len > 0 ? (len + a.page - 1) / a.page : 0;
-  if (tid == 0) {
+  const int len = real ? start + n : 0, live = min(len > 0 ? (len + a.page - 1) / a.page : 0, a.P);
+  if (tid == 0 && blockIdx.y == 0) {
     a.q_start[b + 1] = first + n;
     a.seq_lens[b] = len;
   }
+  const int at = blockIdx.y * THREADS + tid, step = gridDim.y * THREADS, tokens = min(n, a.T - first);
   for (int g = 0; g < a.G; ++g) {
     const int* tab = a.tables + ((size_t)g * a.R + (real ? row : 0)) * a.P;
     int* bt = a.block_tables + g * a.tables_g + (size_t)b * a.W;
-    for (int i = tid; i < a.W; i += THREADS) bt[i] = (i < live && i < a.P) ? tab[i] : 0;
-    for (int i = tid; i < n && first + i < a.T; i += THREADS) {
-      const int p = start + i, lp = p / a.page;
-      a.slots[g * a.slots_g + first + i] = (real && p >= 0 && lp < a.P) ? tab[lp] * a.page + p % a.page : -1;
+    for (int i0 = at; i0 < a.W; i0 += 4 * step) {                  // four entries at a time on their way
+      int v[4];
+#pragma unroll
+      for (int u = 0; u < 4; ++u) v[u] = i0 + u * step < live ? tab[i0 + u * step] : 0;
+#pragma unroll
+      for (int u = 0; u < 4; ++u)
+        if (i0 + u * step < a.W) bt[i0 + u * step] = v[u];
+    }
+    int* slots = a.slots + g * a.slots_g + first;
+    for (int i0 = at; i0 < tokens; i0 += 4 * step) {
+      int v[4];
+#pragma unroll
+      for (int u = 0; u < 4; ++u) {
+        const int p = start + i0 + u * step, lp = p / a.page;
+        const bool there = i0 + u * step < tokens && real && p >= 0 && lp < a.P;
+        v[u] = there ? tab[lp] * a.page + p % a.page : -1;
+      }
+#pragma unroll
+      for (int u = 0; u < 4; ++u)
+        if (i0 + u * step < tokens) slots[i0 + u * step] = v[u];
     }
   }
-  for (int i = tid; i < n && first + i < a.T; i += THREADS) {
+  for (int i = at; i < tokens; i += step) {
     a.token_request[first + i] = b;
     a.positions[first + i] = start + i;
   }
@@ -93,6 +122,10 @@ TS_API int ts_step_maps(const int* requests, const int* updates, int* tables, in
   if (((uintptr_t)updates & 15) != 0) TS_REFUSE(TS_ERR_ALIGN, "ts_step_maps: updates must be 16-byte aligned");
   MapArgs a = {requests, (const int4*)updates, tables, q_start, seq_lens, token_request, positions, slots, block_tables,
                slots_g, tables_g, B, T, U, G, R, P, W, page};
-  ts_launch(step_maps_kernel, dim3(B + 1), dim3(THREADS), 0, (cudaStream_t)stream, a);
+  // blocks a request: one for every 1,024 entries of its tables, or tokens, at most (one block a request with two tables of 2,048
+  // entries: 24 us for 129 requests)
+  const long long most = (long long)W * G > T - B ? (long long)W * G : T - B;
+  const int parts = most <= 1024 ? 1 : (most >= 8192 ? 8 : (int)((most + 1023) / 1024));
+  ts_launch(step_maps_kernel, dim3(B + 1, parts), dim3(THREADS), 0, (cudaStream_t)stream, a);
   TS_LAUNCH_CHECK();
 }
