@@ -58,6 +58,17 @@ def test_a_later_update_of_the_same_place_holds(ops):
     assert on[0, 1, 2].item() == 12 and on[0, 0, 0].item() == 5
 
 
+@pytest.mark.parametrize("n", [40, 513, 1300])
+def test_updates_in_any_order(ops, n):
+    """Many updates, places twice and more among them, a row's far from each other, rows in the step and not; more than a block holds at once."""
+    g = torch.Generator().manual_seed(n)
+    updates = torch.stack([torch.randint(0, 2, (n,), generator=g), torch.randint(0, 6, (n,), generator=g), torch.randint(0, 50, (n,), generator=g),
+                           torch.randint(1, 9999, (n,), generator=g)], 1)
+    run(ops, [[4, 1, -1], [300, 17, 0], [90, 1, 1]], updates.tolist(), tables_of(2, 6, 50), 8, 92, 50)
+    ascending = sorted(updates.tolist(), key=lambda u: (u[1], u[0], u[2]))
+    run(ops, [[4, 1, -1], [300, 17, 0], [90, 1, 1]], ascending, tables_of(2, 6, 50), 8, 92, 50)
+
+
 def test_narrow_and_wide_block_tables(ops):
     for W in (1, 3, 8, 20):
         run(ops, [[1, 0], [20, 0], [12, 5]], [], tables_of(3, 2, 8), 8, 17, W)

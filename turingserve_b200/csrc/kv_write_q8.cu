@@ -252,19 +252,20 @@ __global__ void __launch_bounds__(FAST_THREADS) kv_write_q8_fast_kernel(const Fa
   if (short_span && w0 + r < w1) load_row(w0 + r, x);
   __syncthreads();
   if (tid < SPAN_MAX) {
-    const int s = slot_s[tid];
-    int before = tid - 1;
-    while (before >= 0 && slot_s[before] < 0) --before;
-    const bool lead = s >= 0 && (before < 0 || slot_s[before] / a.page != s / a.page);
-    const unsigned leads = __ballot_sync(0xffffffffu, lead), live = __ballot_sync(0xffffffffu, s >= 0);
-    if (lane == 0) {
-      mask_s[0][tid >> 5] = leads;
-      mask_s[1][tid >> 5] = live;
-    }
+    const unsigned m = __ballot_sync(0xffffffffu, slot_s[tid] >= 0);
+    if (lane == 0) mask_s[1][tid >> 5] = m;
+  }
+  __syncthreads();
+  const unsigned long long live = mask_s[1][0] | (unsigned long long)mask_s[1][1] << 32;
+  if (tid < SPAN_MAX) {
+    const unsigned long long below = live & ((1ull << tid) - 1);
+    const int s = slot_s[tid], pg = s / a.page;
+    const bool lead = s >= 0 && (below == 0 || slot_s[63 - __clzll((long long)below)] / a.page != pg);
+    const unsigned m = __ballot_sync(0xffffffffu, lead);
+    if (lane == 0) mask_s[0][tid >> 5] = m;
   }
   __syncthreads();
   const unsigned long long leads = mask_s[0][0] | (unsigned long long)mask_s[0][1] << 32;
-  const unsigned long long live = mask_s[1][0] | (unsigned long long)mask_s[1][1] << 32;
   if (live == 0) return;
   const int n_runs = __popcll(leads);
   auto run_at = [&](int i) { return __popcll(leads & (~0ull >> (63 - i))) - 1; };

@@ -8,7 +8,7 @@
 // after `updates` (group, row, index, page) have gone into the tables; of updates of the same place the last one holds.
 //
 // One block a request (several where tables are wide or portions long), which sums the lengths before its own, puts its row's updates in
-// place and writes its tokens and its table rows; one more block puts all updates in place, for rows that are not in the step.
+// place and writes its tokens and its table rows; one more block puts the others in place, of rows that are not in the step.
 // Only the update that holds in the end is ever written, so blocks that write the same place write the same value.  One launch
 // whatever the step: 8 requests of 2,048 tokens are bound by its latency (2.0 us in a graph, of which a launch is most); 129 requests
 // with two tables of 2,048 entries and a portion of 1,920 tokens move 3 MB.  The kernel does not let kernels behind it start early: they
@@ -17,7 +17,7 @@
 
 namespace {
 
-constexpr int THREADS = 256, UPDATES = 512;
+constexpr int THREADS = 256, UPDATES = 512, ROWS_HELD = 1024;
 
 struct MapArgs {
   const int* requests;                 // [3][B]: table row, tokens before, tokens brought
@@ -35,6 +35,9 @@ __global__ void __launch_bounds__(THREADS) step_maps_kernel(const MapArgs a) {
   if (extra && blockIdx.y > 0) return;
   __shared__ int sums[THREADS / 32];
   __shared__ int4 up_s[UPDATES];
+  __shared__ int rows_s[ROWS_HELD];
+  if (extra)
+    for (int i = tid; i < min(a.B, ROWS_HELD); i += THREADS) rows_s[i] = a.requests[i];
   const int upto = extra ? a.B : b;
   int mine = 0;
   for (int i = tid; i < upto; i += THREADS) mine += max(0, a.requests[2 * a.B + i]);
@@ -43,20 +46,54 @@ __global__ void __launch_bounds__(THREADS) step_maps_kernel(const MapArgs a) {
   if ((tid & 31) == 0) sums[tid >> 5] = mine;
   const int row = extra ? -1 : a.requests[b], start = extra ? 0 : a.requests[a.B + b], n = extra ? 0 : max(0, a.requests[2 * a.B + b]);
   const bool real = row >= 0 && row < a.R;
-  for (int base = 0; base < a.U; base += UPDATES) {
-    const int count = min(UPDATES, a.U - base);
+  __shared__ int segments, doubt;
+  if (tid == 0) segments = doubt = 0;
+  auto fetch = [&](int base, int count) {
     __syncthreads();
     for (int i = tid; i < count; i += THREADS) up_s[i] = a.updates[base + i];
     __syncthreads();
+  };
+  // Which updates this block puts in place: its row's; the extra block those of rows that no request has.
+  auto mine_too = [&](const int4& up) {
+    if (up.x < 0 || up.x >= a.G || up.y < 0 || up.y >= a.R || up.z < 0 || up.z >= a.P) return false;
+    if (!extra) return up.y == row;
+    bool owned = false;
+    const int here = min(a.B, ROWS_HELD);
+#pragma unroll 8
+    for (int i = 0; i < here; ++i) owned |= rows_s[i] == up.y;
+    for (int i = here; i < a.B; ++i) owned |= a.requests[i] == up.y;
+    return !owned;
+  };
+  // One place twice?  Not if a row's updates stand next to each other, in ascending order; only otherwise every one is held against those
+  // behind it (120 of one row: 12 us of 16).
+  if (!extra)
+    for (int base = 0; base < a.U; base += UPDATES) {
+      const int count = min(UPDATES, a.U - base);
+      fetch(base, count);
+      for (int i = tid; i < count; i += THREADS) {
+        const int4 up = up_s[i];
+        if (up.y != row) continue;
+        const int4 prev = i > 0 ? up_s[i - 1] : (base > 0 ? a.updates[base - 1] : make_int4(0, -2, 0, 0));
+        if (prev.y != row) atomicAdd(&segments, 1);
+        else if (prev.x > up.x || (prev.x == up.x && prev.z >= up.z)) doubt = 1;
+      }
+    }
+  for (int base = 0; base < a.U; base += UPDATES) {
+    const int count = min(UPDATES, a.U - base);
+    if (extra || a.U > UPDATES) fetch(base, count);
+    else __syncthreads();
+    const bool look = extra || doubt || segments > 1;
     for (int i = tid; i < count; i += THREADS) {
       const int4 up = up_s[i];
-      if ((!extra && up.y != row) || up.x < 0 || up.x >= a.G || up.y < 0 || up.y >= a.R || up.z < 0 || up.z >= a.P) continue;
+      if (!mine_too(up)) continue;
       bool holds = true;                                           // no later one of the same place
+      if (look) {
 #pragma unroll 4
-      for (int w = i + 1; w < count; ++w) holds = holds && (up_s[w].x != up.x || up_s[w].y != up.y || up_s[w].z != up.z);
-      for (int w = base + count; w < a.U && holds; ++w) {
-        const int4 later = a.updates[w];
-        holds = later.x != up.x || later.y != up.y || later.z != up.z;
+        for (int w = i + 1; w < count; ++w) holds = holds && (up_s[w].x != up.x || up_s[w].y != up.y || up_s[w].z != up.z);
+        for (int w = base + count; w < a.U && holds; ++w) {
+          const int4 later = a.updates[w];
+          holds = later.x != up.x || later.y != up.y || later.z != up.z;
+        }
       }
       if (holds) a.tables[((size_t)up.x * a.R + up.y) * a.P + up.z] = up.w;
     }
