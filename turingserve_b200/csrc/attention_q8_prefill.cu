@@ -515,6 +515,18 @@ cudaError_t launch(const PreArgs& a, int B, int max_q_len, cudaStream_t s) {
   return ts_launch(attention_q8_prefill_kernel<HD, NR>, grid, dim3(SH::THREADS), SH::SMEM, s, a);
 }
 
+// About how many times the longest block's time a launch of n blocks takes, whose lengths fall evenly from 1 to `least`: the work over the
+// SMs, or r + 1 of the blocks that are the longest left when an SM takes its (r + 1)th.
+double launch_time(long long n, double least) {
+  const double sms = ts_sm_count();
+  double t = n * (1.0 + least) / 2.0 / sms;
+  for (int r = 0; r < n / sms && r < 64; ++r) {
+    const double v = (r + 1) * (1.0 - (1.0 - least) * (r * sms / n));
+    if (v > t) t = v;
+  }
+  return t;
+}
+
 }  // namespace
 
 TS_API void ts_set_q8_prefill(int row_tiles) { g_row_tiles = row_tiles == 1 || row_tiles == 2 ? row_tiles : 0; }   // for measurements
@@ -522,8 +534,8 @@ TS_API void ts_set_q8_prefill(int row_tiles) { g_row_tiles = row_tiles == 1 || r
 // Requests of any number of tokens (rows q_start[b] ..).  q, out: rows [H, D] q_ts / o_ts elements apart.
 TS_API int ts_attention_q8_prefill(void* out, long long o_ts, const void* q, long long q_ts, const void* k_cache, const void* v_cache,
                                    const float* k_scale, const float* v_scale, const int* block_tables, const int* q_start,
-                                   const int* seq_lens, int B, int table_width, int max_q_len, int H, int KVH, int D, int page,
-                                   float scale, int window, void* stream) {
+                                   const int* seq_lens, int B, int table_width, int max_q_len, int max_seq_len, int H, int KVH, int D,
+                                   int page, float scale, int window, void* stream) {
   if (B <= 0 || max_q_len <= 0) return 0;
   if (KVH <= 0 || H % KVH != 0 || (D != 64 && D != 128) || page < 16 || page % 16 != 0)
     TS_REFUSE(TS_ERR_UNSUPPORTED, "ts_attention_q8_prefill: H=%d KVH=%d D=%d page=%d is not taken by this kernel", H, KVH, D, page);
@@ -536,8 +548,14 @@ TS_API int ts_attention_q8_prefill(void* out, long long o_ts, const void* q, lon
   const PreArgs a = {(bf16*)out, o_ts, (const bf16*)q, q_ts, {(const unsigned char*)k_cache, (const unsigned char*)v_cache},
                      {k_scale, v_scale}, block_tables, q_start, seq_lens, table_width, H, KVH, page, scale, window, status};
   cudaStream_t s = (cudaStream_t)stream;
-  const long long pairs = (long long)ceil_div(max_q_len * (H / KVH), 2 * TQ) * KVH * B;
-  const bool two = g_row_tiles ? g_row_tiles == 2 : pairs > ts_sm_count();
+  // Two row tiles a block or one: a turn of 128 keys takes a block of two 1.64 times as long (4,750 against 2,900 cycles), so it is two where half
+  // the blocks more than make up for that (us, one / two: 28 heads over 4, 4,096 tokens 194 / 169, 2,048 63 / 71, 1,024 30 / 32, 2,048 behind
+  // 4,000 225 / 215; 40 over 8, 512 behind 4,000 109 / 98; 12 over 2, 2,048 31 / 49).
+  const int rows = max_q_len * (H / KVH);
+  const double reach = max_seq_len < 1 ? 1 : max_seq_len, sees = window > 0 && window < reach ? window : reach;
+  const double before = max_q_len < reach ? reach - max_q_len : 0, least = (before < sees ? before : sees) / sees;
+  const bool two = g_row_tiles ? g_row_tiles == 2
+                               : launch_time((long long)ceil_div(rows, 2 * TQ) * KVH * B, least) * 1.64 < launch_time((long long)ceil_div(rows, TQ) * KVH * B, least);
   const cudaError_t e = D == 64 ? (two ? launch<64, 2>(a, B, max_q_len, s) : launch<64, 1>(a, B, max_q_len, s))
                                 : (two ? launch<128, 2>(a, B, max_q_len, s) : launch<128, 1>(a, B, max_q_len, s));
   if (e != cudaSuccess) TS_REFUSE((int)e, "ts_attention_q8_prefill: %s", cudaGetErrorString(e));

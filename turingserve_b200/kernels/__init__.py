@@ -110,7 +110,7 @@ class CudaOps:
             "ts_attention_q8_decode": [P, L, P, L, P, P, P, P, P, P, P, P, I, I, I, I, I, I, I, I, I, F, I, I, P],
             "ts_attention_q8_decode_blocks_per_sm": [I, I],
             "ts_attention_q8_decode_clusters": [I, I, I],
-            "ts_attention_q8_prefill": [P, L, P, L, P, P, P, P, P, P, P, I, I, I, I, I, I, I, F, I, P],
+            "ts_attention_q8_prefill": [P, L, P, L, P, P, P, P, P, P, P, I, I, I, I, I, I, I, I, F, I, P],
             "ts_step_maps": [P, P, P, P, P, P, P, P, L, P, L, I, I, I, I, I, I, I, I, P],
             "ts_sample": [P, P, P, P, I, I, P, P],
             "ts_penalize": [P, P, P, P, I, I, P],
@@ -771,7 +771,9 @@ class CudaOps:
         if plan is None:
             fits = [0, 0] + [self.lib.ts_attention_q8_decode_clusters(G, D, n) for n in range(2, 9)]
             plan = self._q8_plans[key] = (self.num_sms * self.lib.ts_attention_q8_decode_blocks_per_sm(G, D), fits)
-        n = self.q8_splits or max(1, min(plan[0] // pairs, -(-reach // 256), 128))
+        # (us, 12 heads over 2: 1 request of 512 keys on 1 / 2 / 4 blocks 5.5 / 5.5 / 4.7; of 2,048 on 4 / 8 / 16 7.0 / 5.9 / 6.4; of 32,000
+        # on 32 / 64 / 125 14.1 / 13.7 / 18.8)
+        n = self.q8_splits or max(1, min(plan[0] // pairs, max(min(-(-reach // 128), 8), -(-reach // 512)), 128))
         return n, 2 <= n <= 8 and self.q8_clusters and plan[1][n] >= pairs
 
     def attention_q8(self, out, q, k_cache, v_cache, k_scale, v_scale, block_tables, step, KVH: int, page_size: int, scale: float,
@@ -816,8 +818,8 @@ class CudaOps:
                     return
         where = (tables + 4 * nd * width, q_start + 4 * nd, seq_lens + 4 * nd)
         if fast and self.use_tc_attention and page_size % 16 == 0:
-            rc = self.lib.ts_attention_q8_prefill(o_ptr, o_ts, q_ptr, q_ts, *pages, *where, B - nd, width, step.max_q_len, H, KVH, D,
-                                                  page_size, scale, w, stream)
+            rc = self.lib.ts_attention_q8_prefill(o_ptr, o_ts, q_ptr, q_ts, *pages, *where, B - nd, width, step.max_q_len, step.max_seq_len,
+                                                  H, KVH, D, page_size, scale, w, stream)
             if rc != self.UNSUPPORTED:
                 self._check(rc, "attention_q8_prefill")
                 return
