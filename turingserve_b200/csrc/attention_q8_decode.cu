@@ -19,6 +19,12 @@
 // stages filled by its own cp.async (16 bytes a lane, rows outside the visible range filled with zeros): no barrier and
 // no other warp in the loop.  The warps' sums meet in shared memory; the splits' in a cluster's distributed shared memory
 // where the blocks of a request and kv head form one, else a second kernel sums what they left in scratch.
+//
+// What bounds it: long contexts the memory (1 request of 100,001 keys over 8 kv heads of 128 38 us, 5.4 TB/s; 128 of 3,000..4,096 over
+// 4 85 us, 5.5 TB/s; 64 of 4,100..8,192 81 us, 5.0 TB/s, the SMs with two of its 256 blocks being the last), short ones the chain launch,
+// table, rows, a tile or two, merge (1 request of 57 keys 3.3 us, 8 of 2,048 over 2 kv heads 6.8).  Measured beside it: two stages (twelve
+// warps an SM instead of eight) 105 us at one block a pair of the 64 requests and 77 to 80 at three and more, but 28 against 23 for 64 of
+// 1,024..2,048; boxes by TMA, whose rows a lane issues for all, 89 against 81.
 #include "mma_utils.cuh"
 #include "q8_cache.cuh"
 
@@ -73,7 +79,7 @@ __device__ __forceinline__ int piece_off(int row, int c) {
   return line * 128 + ((at ^ (line & 7)) << 4);
 }
 
-template <int D, int NG>
+template <int D, int NG, bool PAGES16>
 __global__ void __launch_bounds__(THREADS) attention_q8_decode_kernel(const DecArgs a) {
   pdl_launch_dependents();
   using ST = Stage<D>;
@@ -93,12 +99,31 @@ __global__ void __launch_bounds__(THREADS) attention_q8_decode_kernel(const DecA
 
   unsigned char* ring = smem + warp * ST::WARP_BYTES;
   const int* table = a.block_tables + (size_t)b * a.table_width;
-  // the cache row of key my_first * TILE + lane + 32 i, or -1 outside the visible range
-  auto row_of = [&](int i) {
-    const int j = (my_first + i) * TILE + lane, lp = j / a.page;
-    if (i >= n_tiles || j < lo || j >= seq_len || lp >= a.table_width) return -1;
-    return (table[lp] * a.KVH + kvh) * a.page + (j - lp * a.page);
+  // The cache row of key (my_first + i) * TILE + lane, or -1 outside the visible range; asked for i = 0, 1, 2, ...  Table entries take longer than
+  // a tile's work while the memory is busy: of pages of a multiple of 16 a lane holds the entry of 16 keys, 512 keys in all, and the
+  // next 512 are on their way; of others a key's, one tile ahead.
+  int pg = -1, in_page = 0, pg_next = -1, in_next = 0;
+  auto fetch_pages = [&](int block) {
+    const int j = (my_first + block * 16) * TILE + lane * 16, lp = j / a.page;
+    in_next = j - lp * a.page;
+    pg_next = (j < seq_len && j + 16 > lo && lp < a.table_width) ? table[lp] : -1;
   };
+  auto row_of = [&](int i) {
+    const int j = (my_first + i) * TILE + lane;
+    const bool seen = i < n_tiles && j >= lo && j < seq_len;
+    if (PAGES16) {
+      if (i % 16 == 0) {
+        pg = pg_next;
+        in_page = in_next;
+        fetch_pages(i / 16 + 1);
+      }
+      const int p = __shfl_sync(0xffffffffu, pg, i % 16 * 2 + (lane >> 4)), in = __shfl_sync(0xffffffffu, in_page, i % 16 * 2 + (lane >> 4));
+      return seen && p >= 0 ? (p * a.KVH + kvh) * a.page + in + (lane & 15) : -1;
+    }
+    const int lp = j / a.page;
+    return seen && lp < a.table_width ? (table[lp] * a.KVH + kvh) * a.page + (j - lp * a.page) : -1;
+  };
+  if (PAGES16) fetch_pages(0);
   auto fetch = [&](int i, int row) {                             // this lane's key's row; i < n_tiles
     unsigned char* st = ring + (i % STAGES) * ST::BYTES;
     const int c16 = lane % CPR;
@@ -441,15 +466,15 @@ __global__ void __launch_bounds__(D / 4 * 4) attention_q8_merge_kernel(const Dec
   *reinterpret_cast<uint2*>(dst) = make_uint2(pack_bf16(acc.x * inv, acc.y * inv), pack_bf16(acc.z * inv, acc.w * inv));
 }
 
-template <int D, int NG>
+template <int D, int NG, bool PAGES16>
 int prepare_kernel() {
   static const int slots = [] {
-    if (cudaFuncSetAttribute(attention_q8_decode_kernel<D, NG>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)Stage<D>::SMEM) != cudaSuccess) {
+    if (cudaFuncSetAttribute(attention_q8_decode_kernel<D, NG, PAGES16>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)Stage<D>::SMEM) != cudaSuccess) {
       cudaGetLastError();
       return 0;
     }
     int n = 0;
-    if (cudaOccupancyMaxActiveBlocksPerMultiprocessor(&n, attention_q8_decode_kernel<D, NG>, THREADS, Stage<D>::SMEM) != cudaSuccess) {
+    if (cudaOccupancyMaxActiveBlocksPerMultiprocessor(&n, attention_q8_decode_kernel<D, NG, PAGES16>, THREADS, Stage<D>::SMEM) != cudaSuccess) {
       cudaGetLastError();
       return 0;
     }
@@ -459,7 +484,7 @@ int prepare_kernel() {
 }
 
 // How many clusters of n blocks the chip holds at once.
-template <int D, int NG>
+template <int D, int NG, bool PAGES16>
 int clusters_that_fit(int n) {
   static int known[9];
   int& k = known[n];
@@ -477,16 +502,16 @@ int clusters_that_fit(int n) {
     cfg.attrs = attr;
     cfg.numAttrs = 1;
     int clusters = 0;
-    if (cudaOccupancyMaxActiveClusters(&clusters, attention_q8_decode_kernel<D, NG>, &cfg) == cudaSuccess && clusters >= 1) k = clusters;
+    if (cudaOccupancyMaxActiveClusters(&clusters, attention_q8_decode_kernel<D, NG, PAGES16>, &cfg) == cudaSuccess && clusters >= 1) k = clusters;
     cudaGetLastError();                                          // a refusal is an answer, not an error
   }
   return k;
 }
 
-template <int D, int NG>
+template <int D, int NG, bool PAGES16>
 int launch(const DecArgs& a, cudaStream_t s) {
-  if (prepare_kernel<D, NG>() == 0) TS_REFUSE(TS_ERR_UNSUPPORTED, "ts_attention_q8_decode: the device does not hold a block");
-  cudaError_t e = ts_launch_cluster(attention_q8_decode_kernel<D, NG>, dim3(a.cluster ? a.nsplit : 1, 1, 1), dim3(a.nsplit, a.KVH, a.B),
+  if (prepare_kernel<D, NG, PAGES16>() == 0) TS_REFUSE(TS_ERR_UNSUPPORTED, "ts_attention_q8_decode: the device does not hold a block");
+  cudaError_t e = ts_launch_cluster(attention_q8_decode_kernel<D, NG, PAGES16>, dim3(a.cluster ? a.nsplit : 1, 1, 1), dim3(a.nsplit, a.KVH, a.B),
                                     dim3(THREADS), Stage<D>::SMEM, s, a);
   if (e != cudaSuccess) TS_REFUSE((int)e, "ts_attention_q8_decode: %s", cudaGetErrorString(e));
   if (a.nsplit > 1 && !a.cluster) {
@@ -503,15 +528,15 @@ static bool decode_takes(int H, int KVH, int D) { return KVH > 0 && H % KVH == 0
 // Blocks of the kernel that an SM holds at once, for groups of G heads of D.
 TS_API int ts_attention_q8_decode_blocks_per_sm(int G, int D) {
   if (!decode_takes(G, 1, D)) return 0;
-  if (D == 64) return G <= 8 ? prepare_kernel<64, 1>() : prepare_kernel<64, 2>();
-  return G <= 8 ? prepare_kernel<128, 1>() : prepare_kernel<128, 2>();
+  if (D == 64) return G <= 8 ? prepare_kernel<64, 1, true>() : prepare_kernel<64, 2, true>();
+  return G <= 8 ? prepare_kernel<128, 1, true>() : prepare_kernel<128, 2, true>();
 }
 
 // Clusters of n blocks (2 to 8) that the device holds at once; 0: none.
 TS_API int ts_attention_q8_decode_clusters(int G, int D, int n) {
   if (n < 2 || n > 8 || !ts_clusters_enabled() || ts_attention_q8_decode_blocks_per_sm(G, D) == 0) return 0;
-  const int k = D == 64 ? (G <= 8 ? clusters_that_fit<64, 1>(n) : clusters_that_fit<64, 2>(n))
-                        : (G <= 8 ? clusters_that_fit<128, 1>(n) : clusters_that_fit<128, 2>(n));
+  const int k = D == 64 ? (G <= 8 ? clusters_that_fit<64, 1, true>(n) : clusters_that_fit<64, 2, true>(n))
+                        : (G <= 8 ? clusters_that_fit<128, 1, true>(n) : clusters_that_fit<128, 2, true>(n));
   return k < 0 ? 0 : k;
 }
 
@@ -535,6 +560,11 @@ TS_API int ts_attention_q8_decode(void* out, long long o_ts, const void* q, long
   DecArgs a = {(bf16*)out, o_ts, (const bf16*)q, q_ts, {(const unsigned char*)k_cache, (const unsigned char*)v_cache},
                {k_scale, v_scale}, block_tables, q_start, seq_lens, scratch, B, table_width, H, KVH, page, scale, window, nsplit, cluster, early};
   cudaStream_t s = (cudaStream_t)stream;
-  if (D == 64) return H / KVH <= 8 ? launch<64, 1>(a, s) : launch<64, 2>(a, s);
-  return H / KVH <= 8 ? launch<128, 1>(a, s) : launch<128, 2>(a, s);
+  const int G = H / KVH;
+  if (page % 16 == 0) {
+    if (D == 64) return G <= 8 ? launch<64, 1, true>(a, s) : launch<64, 2, true>(a, s);
+    return G <= 8 ? launch<128, 1, true>(a, s) : launch<128, 2, true>(a, s);
+  }
+  if (D == 64) return G <= 8 ? launch<64, 1, false>(a, s) : launch<64, 2, false>(a, s);
+  return G <= 8 ? launch<128, 1, false>(a, s) : launch<128, 2, false>(a, s);
 }
