@@ -395,6 +395,95 @@ def test_scales_over_the_whole_range(ops, case):
     assert fits
 
 
+@pytest.fixture
+def forced(ops):
+    """Sets the instance of the portions' kernel and the splits of the single tokens'; the rules hold again afterwards."""
+    def force(row_tiles=0, splits=0, clusters=True):
+        ops.lib.ts_set_q8_prefill(row_tiles)
+        ops.q8_splits, ops.q8_clusters = splits, clusters
+    yield force
+    force()
+
+
+@pytest.mark.parametrize("row_tiles", [1, 2])
+@pytest.mark.parametrize("case", [c for c in ATTENDS if max(c[0]) > 1] + [([513, 2, 700], [1025, 2, 5000], 12, 2, 128, 16, 0),
+                                                                            ([400], [400], 34, 2, 64, 48, 0)],
+                         ids=lambda c: f"{len(c[0])}x{max(c[0])}of{max(c[1])}-{c[4]}-w{c[6]}")
+def test_one_and_two_row_tiles(ops, forced, case, row_tiles):
+    forced(row_tiles=row_tiles)
+    for std in (1.0, 4.0):
+        a = Attend(*case, std=std)
+        a.run(ops)
+        a.check()
+
+
+@pytest.mark.parametrize("splits,clusters", [(1, False), (2, True), (3, False), (5, True), (8, True), (8, False), (29, False), (128, False)])
+@pytest.mark.parametrize("case", [ATTENDS[2], ATTENDS[3], ATTENDS[4], ATTENDS[6], ATTENDS[8], ATTENDS[9], ATTENDS[10], ATTENDS[14]],
+                         ids=lambda c: f"{len(c[0])}of{max(c[1])}-{c[2]}-{c[4]}-p{c[5]}-w{c[6]}")
+def test_single_tokens_cut_over_blocks(ops, forced, case, splits, clusters):
+    """More blocks than tiles among them: blocks and warps without a key."""
+    forced(splits=splits, clusters=clusters)
+    a = Attend(*case)
+    if len(a.lens) > 2:
+        a.vs[a.tables[0, 0].long(), 0] = math.nan                  # (a part that is all NaN, beside parts without keys)
+    a.run(ops)
+    a.check()
+
+
+def test_a_cache_of_more_than_2_32_bytes(ops):
+    """Its last pages: written, and read by single tokens and by a portion."""
+    H, KVH, D, page = 8, 8, 128, 64
+    total = (1 << 32) // (KVH * page * D) + 2000
+    k, v = (torch.empty((total, KVH, page, D), dtype=F8, device=DEV) for _ in range(2))
+    ks, vs = torch.ones((total, KVH), device=DEV), torch.ones((total, KVH), device=DEV)
+    assert k.numel() > 1 << 32
+    a = Attend([1, 1, 150], [700, 65, 333], H, KVH, D, page)
+    moved = a.tables + (total - 1 - a.k.shape[0])
+    for b, n in enumerate(a.lens):
+        held = -(-n // page)
+        for big, small in ((k, a.k), (v, a.v), (ks, a.ks), (vs, a.vs)):
+            big[moved[b, :held].long()] = small[a.tables[b, :held].long()]
+    want = a.run(ops).clone()
+    a.k, a.v, a.ks, a.vs, a.tables = k, v, ks, vs, moved.contiguous()
+    assert torch.equal(a.run(ops), want)
+    w = Write([70, 1], [10, 40], H, KVH, D, D, page, BF16)
+    w.run(ops)
+    w_slots, shift = w.slots, (total - 10) * page
+    outs = [t.clone() for t in (w.k, w.v, w.ks, w.vs)]
+    for big, small in ((k, w.k0), (v, w.v0), (ks, w.ks0), (vs, w.vs0)):
+        big[total - 10:total - 10 + small.shape[0]] = small
+    w.slots = w_slots + shift
+    ops.rope_kv_write_q8(w.q, w.x, w.positions, w.cos, w.sin, H, KVH, D, D, k, v, ks, vs, w.slots, page)
+    for big, small in zip((k, v, ks, vs), outs):
+        got = big[total - 10:total - 10 + small.shape[0]]
+        assert torch.equal(got.reshape(-1).view(torch.uint8), small.reshape(-1).view(torch.uint8))
+
+
+def test_a_negative_scale_and_none(ops):
+    for scale in (-0.09, 0.0):
+        for case in (ATTENDS[3], ATTENDS[24], ATTENDS[22]):
+            a = Attend(*case)
+            a.scale = scale
+            a.run(ops)
+            plus = Attend(*case)
+            plus.scale, plus.q = abs(scale), -plus.q if scale < 0 else plus.q
+            want, size, mags = plain.attend(plus.q, a.k, a.v, a.ks, a.vs, a.tables, a.q_lens, a.lens, a.page, abs(scale), a.window)
+            bound = 2.0 ** -8 * want.abs() + (2 * 132 * 2.0 ** -24 * mags + 2.0 ** -17 + 2100 * 2.0 ** -24 + 2.0 ** -11) * size
+            fits = bool(((a.out.double().view(a.q.shape) - want).abs() <= bound + 2100 * 2.0 ** -25 * float(a.vs.max()) * 448).all())
+            assert fits
+
+
+def test_portions_with_caches_in_any_order_in_memory(ops):
+    """Values before keys, keys and values far apart."""
+    for case in (ATTENDS[3], ATTENDS[24]):
+        a = Attend(*case)
+        want = a.run(ops).clone()
+        both = torch.empty((2, *a.k.shape), dtype=F8, device=DEV)
+        both[0], both[1] = a.v, a.k
+        a.v, a.k = both[0], both[1]
+        assert torch.equal(a.run(ops), want)
+
+
 def test_strides(ops):
     """Queries and outputs as columns of wider tensors."""
     for case in (ATTENDS[3], ATTENDS[24]):
