@@ -131,9 +131,8 @@ attention_q8_kernel(T* __restrict__ out, long long o_ts, const T* __restrict__ q
 }
 
 template <typename T>
-int launch(void* out, long long o_ts, const void* q, long long q_ts, const void* k, const void* v, const float* ks, const float* vs,
-           const int* tables, const int* q_start, const int* seq_lens, int B, int width, int max_q_len, int H, int KVH, int D,
-           int page, float scale, int window, cudaStream_t s) {
+int launch(const q8::AttendCall& c, cudaStream_t s) {
+  const int D = c.D;
   const size_t smem = sizeof(float) * ((size_t)ROWS * D + (size_t)KT * (D + 1) + (size_t)KT * D);
   static size_t configured = 0;
   if (smem > 48 * 1024 && smem > configured) {
@@ -141,30 +140,30 @@ int launch(void* out, long long o_ts, const void* q, long long q_ts, const void*
     if (e != cudaSuccess) TS_REFUSE((int)e, "ts_attention_q8: shared memory %zu: %s", smem, cudaGetErrorString(e));
     configured = smem;
   }
-  const long long tiles = ((long long)max_q_len * (H / KVH) + ROWS - 1) / ROWS;
-  if (tiles > 0x7fffffffLL) TS_REFUSE(TS_ERR_LIMIT, "ts_attention_q8: portions of %d tokens", max_q_len);
-  ts_launch(attention_q8_kernel<T>, dim3((unsigned)tiles, KVH, B), dim3(NWARPS * 32), smem, s, (T*)out, o_ts, (const T*)q, q_ts,
-            (const unsigned char*)k, (const unsigned char*)v, ks, vs, tables, q_start, seq_lens, width, H, KVH, D, page, scale, window);
+  const long long tiles = ((long long)c.max_q_len * (c.H / c.KVH) + ROWS - 1) / ROWS;
+  if (tiles > 0x7fffffffLL) TS_REFUSE(TS_ERR_LIMIT, "ts_attention_q8: portions of %d tokens", c.max_q_len);
+  ts_launch(attention_q8_kernel<T>, dim3((unsigned)tiles, c.KVH, c.B), dim3(NWARPS * 32), smem, s, (T*)c.out, c.o_ts, (const T*)c.q, c.q_ts,
+            (const unsigned char*)c.k_cache, (const unsigned char*)c.v_cache, c.k_scale, c.v_scale, c.block_tables, c.q_start, c.seq_lens,
+            c.table_width, c.H, c.KVH, D, c.page, c.scale, c.window);
   TS_LAUNCH_CHECK();
 }
 
 }  // namespace
 
 // q, out: rows [H, D] o_ts / q_ts elements apart.  window <= 0: none.
-TS_API int ts_attention_q8(void* out, long long o_ts, const void* q, long long q_ts, const void* k_cache, const void* v_cache,
-                           const float* k_scale, const float* v_scale, const int* block_tables, const int* q_start,
-                           const int* seq_lens, int B, int table_width, int max_q_len, int H, int KVH, int D, int page,
-                           float scale, int window, int dtype, void* stream) {
+TS_API int ts_attention_q8_record() { return (int)sizeof(q8::AttendCall); }
+
+TS_API int ts_attention_q8(const void* record, void* stream) {
+  const q8::AttendCall& c = *(const q8::AttendCall*)record;
+  const int B = c.B, max_q_len = c.max_q_len, H = c.H, KVH = c.KVH, D = c.D, page = c.page, dtype = c.dtype;
   if (B <= 0 || max_q_len <= 0) return 0;
   if (KVH <= 0 || H % KVH || page <= 0) TS_REFUSE(TS_ERR_SHAPE, "ts_attention_q8: %d heads over %d kv heads, pages of %d", H, KVH, page);
   if (D <= 0 || D > 32 * MAX_DPL) TS_REFUSE(TS_ERR_LIMIT, "ts_attention_q8: head_dim %d (limit %d)", D, 32 * MAX_DPL);
   if (B > 65535 || KVH > 65535) TS_REFUSE(TS_ERR_LIMIT, "ts_attention_q8: %d requests / %d kv heads per launch", B, KVH);
   cudaStream_t s = (cudaStream_t)stream;
   if (dtype == TS_F32)
-    return launch<float>(out, o_ts, q, q_ts, k_cache, v_cache, k_scale, v_scale, block_tables, q_start, seq_lens, B, table_width,
-                         max_q_len, H, KVH, D, page, scale, window, s);
+    return launch<float>(c, s);
   if (dtype == TS_BF16)
-    return launch<bf16>(out, o_ts, q, q_ts, k_cache, v_cache, k_scale, v_scale, block_tables, q_start, seq_lens, B, table_width,
-                        max_q_len, H, KVH, D, page, scale, window, s);
+    return launch<bf16>(c, s);
   TS_REFUSE(TS_ERR_DTYPE, "ts_attention_q8: dtype %d", dtype);
 }

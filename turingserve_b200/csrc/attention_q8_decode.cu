@@ -543,10 +543,13 @@ TS_API int ts_attention_q8_decode_clusters(int G, int D, int n) {
 // One query token per request (rows q_start[b]).  nsplit: blocks that cut the keys of a (request, kv head) among themselves; cluster: as one
 // cluster (2 to 8 of them), else with B * H * nsplit * (D + 2) floats of scratch.  early: index arrays and cache rows before
 // each request's last page are in place already and are read before the wait for the kernels before.
-TS_API int ts_attention_q8_decode(void* out, long long o_ts, const void* q, long long q_ts, const void* k_cache, const void* v_cache,
-                                  const float* k_scale, const float* v_scale, const int* block_tables, const int* q_start,
-                                  const int* seq_lens, float* scratch, int B, int table_width, int nsplit, int cluster, int H, int KVH, int D,
-                                  int page, int num_pages, float scale, int window, int early, void* stream) {
+TS_API int ts_attention_q8_decode(const void* record, void* stream) {
+  const AttendCall& c = *(const AttendCall*)record;
+  const int B = c.B, H = c.H, KVH = c.KVH, D = c.D, page = c.page, num_pages = c.num_pages, nsplit = c.nsplit, cluster = c.cluster;
+  const long long o_ts = c.o_ts, q_ts = c.q_ts;
+  const void *const k_cache = c.k_cache, *const v_cache = c.v_cache, *const q = c.q;
+  void* const out = c.out;
+  float* const scratch = c.scratch;
   if (B <= 0) return 0;
   if (!decode_takes(H, KVH, D) || page <= 0)
     TS_REFUSE(TS_ERR_UNSUPPORTED, "ts_attention_q8_decode: H=%d KVH=%d D=%d page=%d is not taken by this kernel", H, KVH, D, page);
@@ -558,7 +561,8 @@ TS_API int ts_attention_q8_decode(void* out, long long o_ts, const void* q, long
     TS_REFUSE(TS_ERR_UNSUPPORTED, "ts_attention_q8_decode: pages on 16 bytes, rows of queries and outputs on 8");
   if ((long long)num_pages * KVH * page > 0x7fffffffLL) TS_REFUSE(TS_ERR_UNSUPPORTED, "ts_attention_q8_decode: a cache of more than 2^31 rows");
   DecArgs a = {(bf16*)out, o_ts, (const bf16*)q, q_ts, {(const unsigned char*)k_cache, (const unsigned char*)v_cache},
-               {k_scale, v_scale}, block_tables, q_start, seq_lens, scratch, B, table_width, H, KVH, page, scale, window, nsplit, cluster, early};
+               {c.k_scale, c.v_scale}, c.block_tables, c.q_start, c.seq_lens, scratch, B, c.table_width, H, KVH, page, c.scale, c.window, nsplit,
+               cluster, c.early};
   cudaStream_t s = (cudaStream_t)stream;
   const int G = H / KVH;
   if (page % 16 == 0) {

@@ -532,10 +532,12 @@ double launch_time(long long n, double least) {
 TS_API void ts_set_q8_prefill(int row_tiles) { g_row_tiles = row_tiles == 1 || row_tiles == 2 ? row_tiles : 0; }   // for measurements
 
 // Requests of any number of tokens (rows q_start[b] ..).  q, out: rows [H, D] q_ts / o_ts elements apart.
-TS_API int ts_attention_q8_prefill(void* out, long long o_ts, const void* q, long long q_ts, const void* k_cache, const void* v_cache,
-                                   const float* k_scale, const float* v_scale, const int* block_tables, const int* q_start,
-                                   const int* seq_lens, int B, int table_width, int max_q_len, int max_seq_len, int H, int KVH, int D,
-                                   int page, float scale, int window, void* stream) {
+TS_API int ts_attention_q8_prefill(const void* record, void* stream) {
+  const q8::AttendCall& c = *(const q8::AttendCall*)record;
+  const int B = c.B, max_q_len = c.max_q_len, max_seq_len = c.max_seq_len, H = c.H, KVH = c.KVH, D = c.D, page = c.page, window = c.window;
+  const long long o_ts = c.o_ts, q_ts = c.q_ts;
+  const void *const k_cache = c.k_cache, *const v_cache = c.v_cache, *const q = c.q;
+  void* const out = c.out;
   if (B <= 0 || max_q_len <= 0) return 0;
   if (KVH <= 0 || H % KVH != 0 || (D != 64 && D != 128) || page < 16 || page % 16 != 0)
     TS_REFUSE(TS_ERR_UNSUPPORTED, "ts_attention_q8_prefill: H=%d KVH=%d D=%d page=%d is not taken by this kernel", H, KVH, D, page);
@@ -546,7 +548,7 @@ TS_API int ts_attention_q8_prefill(void* out, long long o_ts, const void* q, lon
   int* status = ts_attn_status_word();
   if (status == nullptr) TS_REFUSE(TS_ERR_LIMIT, "ts_attention_q8_prefill: no status word");
   const PreArgs a = {(bf16*)out, o_ts, (const bf16*)q, q_ts, {(const unsigned char*)k_cache, (const unsigned char*)v_cache},
-                     {k_scale, v_scale}, block_tables, q_start, seq_lens, table_width, H, KVH, page, scale, window, status};
+                     {c.k_scale, c.v_scale}, c.block_tables, c.q_start, c.seq_lens, c.table_width, H, KVH, page, c.scale, window, status};
   cudaStream_t s = (cudaStream_t)stream;
   // Two row tiles a block or one: a turn of 128 keys takes a block of two 1.64 times as long (4,750 against 2,900 cycles), so it is two where half
   // the blocks more than make up for that (us, one / two: 28 heads over 4, 4,096 tokens 194 / 169, 2,048 63 / 71, 1,024 30 / 32, 2,048 behind

@@ -71,4 +71,19 @@ __device__ __forceinline__ float query_to_half(float amax, float scale, float& f
 }
 __device__ __forceinline__ float abs_or_inf(float x) { return x != x ? INFINITY : fabsf(x); }
 
+// What the kernels of attention over this cache are called with: see attention_q8.cu, attention_q8_decode.cu, attention_q8_prefill.cu.  One
+// record for all three; each reads what it needs.
+struct AttendCall {
+  void* out;
+  const void* q;
+  const void *k_cache, *v_cache;
+  const float *k_scale, *v_scale;
+  const int *block_tables, *q_start, *seq_lens;
+  float* scratch;
+  long long o_ts, q_ts;
+  int B, table_width, max_q_len, max_seq_len, H, KVH, D, page, num_pages, window, dtype;
+  int nsplit, cluster, early;
+  float scale;
+};
+
 }  // namespace q8

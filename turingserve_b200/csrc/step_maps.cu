@@ -150,15 +150,25 @@ __global__ void __launch_bounds__(THREADS) step_maps_kernel(const MapArgs a) {
 
 }  // namespace
 
-TS_API int ts_step_maps(const int* requests, const int* updates, int* tables, int* q_start, int* seq_lens, int* token_request,
-                        int* positions, int* slots, long long slots_g, int* block_tables, long long tables_g, int B, int T, int U,
-                        int G, int R, int P, int W, int page, void* stream) {
+struct MapCall {
+  const int *requests, *updates;
+  int *tables, *q_start, *seq_lens, *token_request, *positions, *slots, *block_tables;
+  long long slots_g, tables_g;
+  int B, T, U, G, R, P, W, page;
+};
+
+TS_API int ts_step_maps_record() { return (int)sizeof(MapCall); }
+
+// (the arguments as one record: see kv_write_q8.cu)
+TS_API int ts_step_maps(const void* record, void* stream) {
+  const MapCall& c = *(const MapCall*)record;
+  const int B = c.B, T = c.T, U = c.U, G = c.G, R = c.R, P = c.P, W = c.W, page = c.page;
   if (B <= 0) return 0;
   if (T < 0 || U < 0 || G < 0 || R <= 0 || P <= 0 || W < 0 || page <= 0)
     TS_REFUSE(TS_ERR_SHAPE, "ts_step_maps: T=%d U=%d G=%d R=%d P=%d W=%d page=%d", T, U, G, R, P, W, page);
-  if (((uintptr_t)updates & 15) != 0) TS_REFUSE(TS_ERR_ALIGN, "ts_step_maps: updates must be 16-byte aligned");
-  MapArgs a = {requests, (const int4*)updates, tables, q_start, seq_lens, token_request, positions, slots, block_tables,
-               slots_g, tables_g, B, T, U, G, R, P, W, page};
+  if (((uintptr_t)c.updates & 15) != 0) TS_REFUSE(TS_ERR_ALIGN, "ts_step_maps: updates must be 16-byte aligned");
+  MapArgs a = {c.requests, (const int4*)c.updates, c.tables, c.q_start, c.seq_lens, c.token_request, c.positions, c.slots, c.block_tables,
+               c.slots_g, c.tables_g, B, T, U, G, R, P, W, page};
   // blocks a request: one for every 1,024 entries of its tables, or tokens, at most (one block a request with two tables of 2,048
   // entries: 24 us for 129 requests)
   const long long most = (long long)W * G > T - B ? (long long)W * G : T - B;

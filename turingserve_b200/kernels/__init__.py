@@ -16,6 +16,7 @@ from __future__ import annotations
 import ctypes
 import math
 import os
+import struct
 
 import torch
 
@@ -37,6 +38,10 @@ def _code(dtype: torch.dtype) -> int:
         return _DTYPE_CODE[dtype]
     except KeyError:
         raise TypeError(f"kernels take float32 or bfloat16, not {dtype}") from None
+
+
+# Arguments that go to the library as one record (``csrc/kv_write_q8.cu`` and ``q8_cache.cuh``, ``step_maps.cu``)
+_WRITE_Q8, _ATTEND_Q8, _MAPS = struct.Struct("@12Pq8i"), struct.Struct("@10P2q14if4x"), struct.Struct("@9P2q8i")
 
 
 class KernelError(RuntimeError):
@@ -104,14 +109,17 @@ class CudaOps:
             "ts_linear_tc_ex": [P, P, P, P, P, I, I, I, I, I, I, P, P],
             "ts_reduce_rmsnorm": [P, P, I, P, P, P, F, I, I, I, P],
             "ts_feed_tokens": [P, P, P, P, I, I, P],
-            "ts_rope_kv_write_q8": [P, L, P, P, P, P, P, P, P, P, P, I, I, I, I, I, I, I, P, I, P, P],
+            "ts_rope_kv_write_q8": [ctypes.c_char_p, P],
             "ts_rope_kv_write_q8_takes_parts": [I, I, I],
-            "ts_attention_q8": [P, L, P, L, P, P, P, P, P, P, P, I, I, I, I, I, I, I, F, I, I, P],
-            "ts_attention_q8_decode": [P, L, P, L, P, P, P, P, P, P, P, P, I, I, I, I, I, I, I, I, I, F, I, I, P],
+            "ts_rope_kv_write_q8_record": [],
+            "ts_attention_q8_record": [],
+            "ts_step_maps_record": [],
+            "ts_attention_q8": [ctypes.c_char_p, P],
+            "ts_attention_q8_decode": [ctypes.c_char_p, P],
             "ts_attention_q8_decode_blocks_per_sm": [I, I],
             "ts_attention_q8_decode_clusters": [I, I, I],
-            "ts_attention_q8_prefill": [P, L, P, L, P, P, P, P, P, P, P, I, I, I, I, I, I, I, I, F, I, P],
-            "ts_step_maps": [P, P, P, P, P, P, P, P, L, P, L, I, I, I, I, I, I, I, I, P],
+            "ts_attention_q8_prefill": [ctypes.c_char_p, P],
+            "ts_step_maps": [ctypes.c_char_p, P],
             "ts_sample": [P, P, P, P, I, I, P, P],
             "ts_penalize": [P, P, P, P, I, I, P],
             "ts_sample_greedy": [P, P, I, I, P, P, P, P],
@@ -182,6 +190,9 @@ class CudaOps:
             fn = getattr(self.lib, name)
             fn.argtypes = args
             fn.restype = c_int
+        for name, record in (("rope_kv_write_q8", _WRITE_Q8), ("attention_q8", _ATTEND_Q8), ("step_maps", _MAPS)):
+            if getattr(self.lib, f"ts_{name}_record")() != record.size:
+                raise KernelError(f"{lib_path}: {name} takes another record than this package's {record.size} bytes")
         self.lib.ts_set_q8_prefill.argtypes = [I]
         self.lib.ts_set_q8_prefill.restype = None
         self.lib.ts_attention_diff_mma_supported.argtypes = [I, I, I, I, I]
@@ -752,13 +763,13 @@ class CudaOps:
                 qkv = self.materialize(qkv)
         if not qkv.is_contiguous() or q_out.stride(1) != 1:
             raise ValueError("rope_kv_write_q8: rows must be contiguous")
-        if k_cache is None:
-            pages = (None,) * 5
-        else:
+        pages = (0,) * 5
+        if k_cache is not None:
             pages = (k_cache.data_ptr(), v_cache.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr(), slots.data_ptr())
-        self._check(self.lib.ts_rope_kv_write_q8(
-            q_out.data_ptr(), q_out.stride(0), qkv.data_ptr(), positions.data_ptr(), _ptr(cos), _ptr(sin), *pages, T, H, KVH, D,
-            rotary_dim, page_size, code, _ptr(part), splits, _ptr(bias), self._stream()), "rope_kv_write_q8")
+        self._check(self.lib.ts_rope_kv_write_q8(_WRITE_Q8.pack(
+            q_out.data_ptr(), qkv.data_ptr(), positions.data_ptr(), cos.data_ptr() if rotary_dim else 0, sin.data_ptr() if rotary_dim else 0,
+            *pages, _ptr(part) or 0, _ptr(bias) or 0, q_out.stride(0), T, H, KVH, D, rotary_dim, page_size, code, splits), self._stream()),
+            "rope_kv_write_q8")
 
     # the most blocks that cut the keys of one (request, kv head) among themselves (0: by the sizes), whether as clusters
     q8_splits, q8_clusters = 0, True
@@ -785,8 +796,10 @@ class CudaOps:
         if KVH <= 0 or H % KVH:
             raise ValueError(f"attention_q8: {H} heads over {KVH} kv heads")
         q_ts, hs, one = q.stride()
-        if (code is None or one != 1 or (hs != D and H > 1) or out.dtype is not q.dtype or out.shape != (T, H * D)
-                or out.stride(1) != 1):
+        if code is None or one != 1 or (hs != D and H > 1) or out.dtype is not q.dtype or out.shape != (T, H * D):
+            raise ValueError("attention_q8: rows of contiguous heads, float32 or bfloat16, outputs [T, H D] in the queries' type")
+        o_ts, one = out.stride()
+        if one != 1:
             raise ValueError("attention_q8: rows of contiguous heads, float32 or bfloat16, outputs [T, H D] in the queries' type")
         if block_tables.dtype is not torch.int32 or not block_tables.is_contiguous() or block_tables.shape[0] < B:
             raise ValueError("attention_q8: an int32 block table for each request, rows contiguous")
@@ -794,37 +807,37 @@ class CudaOps:
         w = int(window) if window else 0
         if w < 0:
             raise ValueError(f"attention_q8: a window of {w} keys")
-        G, nd, width, stream = H // KVH, 0, block_tables.shape[1], self._stream()
-        o_ptr, o_ts, q_ptr, tables, q_start, seq_lens = (out.data_ptr(), out.stride(0), q.data_ptr(), block_tables.data_ptr(),
-                                                         step.q_start.data_ptr(), step.seq_lens.data_ptr())
-        pages = (k_cache.data_ptr(), v_cache.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr())
+        G, nd, width, stream, max_seq = H // KVH, 0, block_tables.shape[1], self._stream(), step.max_seq_len
+        rows = (out.data_ptr(), q.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr())
+        tables, q_start, seq_lens = block_tables.data_ptr(), step.q_start.data_ptr(), step.seq_lens.data_ptr()
+        sizes = (H, KVH, D, page_size, k_cache.shape[0], w, code)
         fast = self.use_fast_attention and code == 1 and (D == 128 or D == 64)
         if fast and G <= 16 and step.num_decode:
-            nd, reach = step.num_decode, step.max_seq_len
-            splits, cluster = self._q8_plan(nd * KVH, G, D, min(reach, w) if w else reach)
-            scratch = None
+            nd = step.num_decode
+            splits, cluster = self._q8_plan(nd * KVH, G, D, min(max_seq, w) if w else max_seq)
+            scratch, at = None, 0
             if splits > 1 and not cluster:
                 # (of this call's own: calls on two streams, or in two captured graphs, do not meet in it)
                 scratch = torch.empty(nd * H * splits * (D + 2), dtype=torch.float32, device=q.device)
+                at = scratch.data_ptr()
                 self.launches += 1
-            rc = self.lib.ts_attention_q8_decode(
-                o_ptr, o_ts, q_ptr, q_ts, *pages, tables, q_start, seq_lens, _ptr(scratch), nd, width, splits, cluster, H, KVH, D,
-                page_size, k_cache.shape[0], scale, w, getattr(step, "settled", False), stream)
+            rc = self.lib.ts_attention_q8_decode(_ATTEND_Q8.pack(
+                *rows, tables, q_start, seq_lens, at, o_ts, q_ts, nd, width, 1, max_seq, *sizes, splits, cluster,
+                getattr(step, "settled", False), scale), stream)
             if rc == self.UNSUPPORTED:
                 nd = 0
             else:
                 self._check(rc, "attention_q8_decode")
                 if nd == B:
                     return
-        where = (tables + 4 * nd * width, q_start + 4 * nd, seq_lens + 4 * nd)
+        record = _ATTEND_Q8.pack(*rows, tables + 4 * nd * width, q_start + 4 * nd, seq_lens + 4 * nd, 0, o_ts, q_ts, B - nd, width,
+                                 step.max_q_len, max_seq, *sizes, 1, 0, 0, scale)
         if fast and self.use_tc_attention and page_size % 16 == 0:
-            rc = self.lib.ts_attention_q8_prefill(o_ptr, o_ts, q_ptr, q_ts, *pages, *where, B - nd, width, step.max_q_len, step.max_seq_len,
-                                                  H, KVH, D, page_size, scale, w, stream)
+            rc = self.lib.ts_attention_q8_prefill(record, stream)
             if rc != self.UNSUPPORTED:
                 self._check(rc, "attention_q8_prefill")
                 return
-        self._check(self.lib.ts_attention_q8(o_ptr, o_ts, q_ptr, q_ts, *pages, *where, B - nd, width, step.max_q_len, H, KVH, D, page_size,
-                                             scale, w, code, stream), "attention_q8")
+        self._check(self.lib.ts_attention_q8(record, stream), "attention_q8")
 
     # -- a step's maps -----------------------------------------------------------------------------------------
     def step_maps(self, requests, updates, tables, page_size: int, q_start, seq_lens, token_request, positions, slot_mapping,
@@ -854,9 +867,9 @@ class CudaOps:
         t_g, t_b, t_w = block_tables.stride()
         if (s_t != 1 and T > 1) or (t_w != 1 and W > 1) or (t_b != W and B > 1):
             raise ValueError("step_maps: each group's slots and block tables are contiguous")
-        self._check(self.lib.ts_step_maps(
+        self._check(self.lib.ts_step_maps(_MAPS.pack(
             requests.data_ptr(), updates.data_ptr(), tables.data_ptr(), q_start.data_ptr(), seq_lens.data_ptr(), token_request.data_ptr(),
-            positions.data_ptr(), slot_mapping.data_ptr(), s_g, block_tables.data_ptr(), t_g, B, T, U, G, R, P, W, page_size,
+            positions.data_ptr(), slot_mapping.data_ptr(), block_tables.data_ptr(), s_g, t_g, B, T, U, G, R, P, W, page_size),
             self._stream()), "step_maps")
 
     # -- a residual stream in 32-bit ---------------------------------------------------------------------
