@@ -379,13 +379,15 @@ template <int D>
 cudaError_t launch_fast(FastArgs f, cudaStream_t s) {
   const WriteArgs& a = f.w;
   constexpr int ROWS = FAST_THREADS / (D / 16);
-  // spans of as many tokens as a block takes in one turn (no slower than a token a block: its rows lie side by side in the block's
-  // warps), wider where there are blocks enough; every block of a page's rows reads all of them
-  f.span = a.T <= 8 ? 1 : (a.T <= 1024 ? ROWS : SPAN_MAX);
+  // Spans of as many tokens as a block takes in one turn (no slower than a token a block: its rows lie side by side in the block's warps), wider
+  // where there are blocks enough: every block of a page's rows reads all of them.  (us at spans of 16 / 32 / 64: 1,999 tokens, 28 heads
+  // over 4, 17.7 / 17.8 / 20.2; 7,543 tokens 48 / 38 / 34; 8,000 tokens, 40 over 8, 81 / 60 / 51)
+  f.span = a.T <= 8 ? 1 : (a.T <= 1024 ? ROWS : (a.T <= 4096 ? 32 : SPAN_MAX));
   f.kv_blocks = a.cache[0] != nullptr ? 2 * a.KVH : 0;
-  // query heads a block: as many as keep about 2,048 threads on every SM, at least one row of lanes each
+  // query heads a block (they share a table row's conversion): as many as keep 4,096 lanes an SM, at least one row of lanes each (7,543 tokens, 2 / 4
+  // / 7 / 14 heads 34 / 35 / 40 / 52 us)
   const int least = f.span < ROWS ? ROWS / f.span : 1;
-  const long long lanes = (long long)a.T * (D / 16) * a.H, want = lanes / ((long long)ts_sm_count() * 2048);
+  const long long lanes = (long long)a.T * (D / 16) * a.H, want = lanes / ((long long)ts_sm_count() * 4096);
   f.q_heads = (int)(want < least ? least : (want > a.H ? a.H : want));
   const dim3 grid(ceil_div(a.T, f.span), f.kv_blocks + ceil_div(a.H, f.q_heads)), block(FAST_THREADS);
   return f.part != nullptr ? ts_launch(kv_write_q8_fast_kernel<D, true>, grid, block, 0, s, f)
