@@ -22,8 +22,6 @@
 //
 // NaN: a page whose scale is NaN (either) gives NaN scores, which the rows that do not see it drop by selection; its values are
 // finite bytes (writes store zeros under such a scale), so zero weights stay zeros.
-#include <type_traits>
-
 #include "mma_utils.cuh"
 #include "q8_cache.cuh"
 #include "tc_utils.cuh"
@@ -243,8 +241,16 @@ __global__ void __launch_bounds__(Shape<HD, NR>::THREADS, 1) attention_q8_prefil
       const unsigned see_n = (unsigned)max(0, min(TK, pos + 1 - j0) - see_lo);
       bool move = false;
       float corr = 1.f, rs = 0.f;
-      auto turn = [&](auto masked) {
-        constexpr bool MASK = decltype(masked)::value;
+      auto new_reference = [&](float mx) {
+        move = mx > m_ref + RESCALE_STEP || (m_ref == -INFINITY && mx > -INFINITY);
+        if (move) {
+          corr = ex2(m_ref - mx);                                  // 0 when there was no reference yet
+          m_ref = mx;
+        }
+        return m_ref == -INFINITY ? 0.f : m_ref;
+      };
+      // a turn whose keys every row of the warp sees
+      auto whole_turn = [&]() {
         uint32_t sv[TK];
 #pragma unroll
         for (int c = 0; c < TK / 32; ++c) tmem_ld32(s_addr + c * 32, *reinterpret_cast<uint32_t(*)[32]>(sv + c * 32));
@@ -254,24 +260,12 @@ __global__ void __launch_bounds__(Shape<HD, NR>::THREADS, 1) attention_q8_prefil
         for (int h = 0; h < GROUPS; ++h) {
           float top[2] = {-INFINITY, -INFINITY};
 #pragma unroll
-          for (int i = 0; i < 16; i += 2) {
-            if (MASK) {
-              if ((unsigned)(h * 16 + i - see_lo) >= see_n) sv[h * 16 + i] = 0xff800000u;
-              if ((unsigned)(h * 16 + i + 1 - see_lo) >= see_n) sv[h * 16 + i + 1] = 0xff800000u;
-            }
+          for (int i = 0; i < 16; i += 2)
             top[i >> 1 & 1] = max3(top[i >> 1 & 1], __uint_as_float(sv[h * 16 + i]), __uint_as_float(sv[h * 16 + i + 1]));
-          }
           const float4 x = sc[h];
-          const float best = fmaxf(top[0], top[1]);
-          // (nothing seen: no maximum, whatever the factor)
-          mx = fmaxf(mx, MASK && best == -INFINITY ? -INFINITY : fmaf(best, x.x * factor, x.y));
+          mx = fmaxf(mx, fmaf(fmaxf(top[0], top[1]), x.x * factor, x.y));
         }
-        move = mx > m_ref + RESCALE_STEP || (m_ref == -INFINITY && mx > -INFINITY);
-        if (move) {
-          corr = ex2(m_ref - mx);                                  // 0 when there was no reference yet
-          m_ref = mx;
-        }
-        const float m_use = m_ref == -INFINITY ? 0.f : m_ref;
+        const float m_use = new_reference(mx);
 #pragma unroll
         for (int h = 0; h < GROUPS; ++h) {
           const float4 x = sc[h];
@@ -279,12 +273,8 @@ __global__ void __launch_bounds__(Shape<HD, NR>::THREADS, 1) attention_q8_prefil
           float part[2] = {0.f, 0.f};
 #pragma unroll
           for (int i = 0; i < 16; i += 2) {
-            float p0 = ex2(fmaf(__uint_as_float(sv[h * 16 + i]), f, add));
-            float p1 = ex2(fmaf(__uint_as_float(sv[h * 16 + i + 1]), f, add));
-            if (MASK) {                                            // (a factor of 0 would make a NaN of it)
-              p0 = sv[h * 16 + i] == 0xff800000u ? 0.f : p0;
-              p1 = sv[h * 16 + i + 1] == 0xff800000u ? 0.f : p1;
-            }
+            const float p0 = ex2(fmaf(__uint_as_float(sv[h * 16 + i]), f, add));
+            const float p1 = ex2(fmaf(__uint_as_float(sv[h * 16 + i + 1]), f, add));
             part[0] += p0;
             part[1] += p1;
             sv[h * 8 + i / 2] = q8::pack_half(p0, p1);             // (its place has been read)
@@ -293,8 +283,57 @@ __global__ void __launch_bounds__(Shape<HD, NR>::THREADS, 1) attention_q8_prefil
           if (h % 4 == 3) tmem_st32(s_addr + (h / 4) * 32, *reinterpret_cast<const uint32_t(*)[32]>(sv + (h / 4) * 32));
         }
       };
-      if (all_visible) turn(std::false_type());
-      else turn(std::true_type());
+      // a turn at an edge of what is seen: 32 scores a turn of two loops, which stay loops (few turns are such, and code that is run once is
+      // mostly waited for)
+      auto edge_turn = [&]() {
+        auto seen = [&](int c) {                                   // of keys 32 c ..: a bit each
+          const int lo = min(max(see_lo - 32 * c, 0), 32), hi = min(max(see_lo + (int)see_n - 32 * c, 0), 32);
+          return (uint32_t)((1ull << hi) - 1) & ~(uint32_t)((1ull << lo) - 1);
+        };
+        float mx = -INFINITY;
+#pragma unroll 1
+        for (int c = 0; c < TK / 32; ++c) {
+          uint32_t sv[32];
+          tmem_ld32(s_addr + c * 32, sv);
+          const uint32_t bits = seen(c);
+          tmem_wait_ld();
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {
+            float top = -INFINITY;
+#pragma unroll
+            for (int i = 0; i < 16; i += 2)
+              top = max3(top, bits >> (h * 16 + i) & 1 ? __uint_as_float(sv[h * 16 + i]) : -INFINITY,
+                         bits >> (h * 16 + i + 1) & 1 ? __uint_as_float(sv[h * 16 + i + 1]) : -INFINITY);
+            const float4 x = sc[2 * c + h];
+            if (top > -INFINITY) mx = fmaxf(mx, fmaf(top, x.x * factor, x.y));            // (nothing seen: no maximum, whatever the factor)
+          }
+        }
+        const float m_use = new_reference(mx);
+#pragma unroll 1
+        for (int c = 0; c < TK / 32; ++c) {
+          uint32_t sv[32], pw[16];
+          tmem_ld32(s_addr + c * 32, sv);
+          const uint32_t bits = seen(c);
+          tmem_wait_ld();
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {
+            const float4 x = sc[2 * c + h];
+            const float f = x.x * factor, add = x.y - m_use;
+            float part = 0.f;
+#pragma unroll
+            for (int i = 0; i < 16; i += 2) {
+              const float p0 = bits >> (h * 16 + i) & 1 ? ex2(fmaf(__uint_as_float(sv[h * 16 + i]), f, add)) : 0.f;
+              const float p1 = bits >> (h * 16 + i + 1) & 1 ? ex2(fmaf(__uint_as_float(sv[h * 16 + i + 1]), f, add)) : 0.f;
+              part += p0 + p1;
+              pw[h * 8 + i / 2] = q8::pack_half(p0, p1);
+            }
+            rs = fmaf(part, x.z, rs);
+          }
+          tmem_st16(s_addr + c * 16, pw);                          // over scores that have been read
+        }
+      };
+      if (all_visible) whole_turn();
+      else edge_turn();
       l_run = l_run * corr + rs;
       if (t > 0 && __any_sync(0xffffffffu, move)) {
         if (NB == 2) {                                             // (one buffer: S(t) was issued behind the product before, and is complete)
