@@ -21,7 +21,7 @@ class NoLibrary:
 @pytest.fixture
 def ops():
     o = CudaOps.__new__(CudaOps)
-    o.lib, o.num_sms, o._device_index = NoLibrary(), 148, 0
+    o.lib, o.num_sms, o._device_index = NoLibrary(), 148, -1      # (-1: the CPU's, so that only what is wrong refuses)
     return o
 
 
@@ -111,6 +111,14 @@ def maps_args(**other):
 def test_maps_refuse(ops, other):
     with pytest.raises(ValueError):
         ops.step_maps(**maps_args(**other))
+
+
+def test_tensors_of_another_device_are_refused(ops):
+    ops._device_index = 0
+    for call, args in ((ops.rope_kv_write_q8, write_args()), (ops.rope_kv_write_q8, write_args(k_cache=None)), (ops.attention_q8, attend_args()),
+                       (ops.step_maps, maps_args())):
+        with pytest.raises(ValueError, match="on GPU 0"):
+            call(**args)
 
 
 def test_scales():

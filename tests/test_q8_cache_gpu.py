@@ -16,6 +16,7 @@ import pytest
 import torch
 
 from tests import plain_q8 as plain
+from turingserve_b200.kernels import KernelError
 
 pytestmark = pytest.mark.gpu
 DEV = "cuda"
@@ -224,6 +225,16 @@ def test_queries_alone_and_queries_as_columns_of_a_wider_tensor(ops):
     alone = torch.zeros((30, 512), dtype=BF16, device=DEV)
     ops.rope_kv_write_q8(alone, w.x, w.positions, w.cos, w.sin, 4, 2, 128, 128, None, None, None, None, w.slots, 16)
     assert torch.equal(alone, w.q)
+
+
+@pytest.mark.parametrize("dtype", [BF16, torch.float32])
+def test_queries_within_the_rows_they_come_from_are_refused(ops, dtype):
+    w = Write([5], [3], 4, 2, 64, 64, 16, dtype)
+    before, held = w.x.clone(), w.k.clone()
+    w.q = w.x[:, :256]
+    with pytest.raises(KernelError, match="lie in qkv"):
+        w.run(ops)
+    assert torch.equal(w.x, before) and torch.equal(w.k.view(torch.uint8), held.view(torch.uint8))
 
 
 # ------------------------------------------------------------------------------------------------------------ attention

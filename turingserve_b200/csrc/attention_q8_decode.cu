@@ -21,8 +21,8 @@
 // where the blocks of a request and kv head form one, else a second kernel sums what they left in scratch.
 //
 // What bounds it: long contexts the memory (1 request of 100,001 keys over 8 kv heads of 128 38 us, 5.4 TB/s; 128 of 3,000..4,096 over
-// 4 85 us, 5.5 TB/s; 64 of 4,100..8,192 81 us, 5.0 TB/s, the SMs with two of its 256 blocks being the last), short ones the chain launch,
-// table, rows, a tile or two, merge (1 request of 57 keys 3.3 us, 8 of 2,048 over 2 kv heads 6.8).  Measured beside it: two stages (twelve
+// 4 85 us, 5.5 TB/s; 64 of 4,100..8,192 80 us, 5.1 TB/s, the SMs with two of its 256 blocks being the last), short ones the chain launch,
+// table, rows, a tile or two, merge (1 request of 57 keys 3.2 us, 8 of 2,048 over 2 kv heads 6.6).  Measured beside it: two stages (twelve
 // warps an SM instead of eight) 105 us at one block a pair of the 64 requests and 77 to 80 at three and more, but 28 against 23 for 64 of
 // 1,024..2,048; boxes by TMA, whose rows a lane issues for all, 89 against 81.
 #include "mma_utils.cuh"

@@ -2,7 +2,7 @@
 //
 // Semantics as rope_kv_write (elementwise.cu): rotate-half over the first `rot` dims of each query and key head with the
 // table's rows rounded to the model's type and the arithmetic in 32 bits; slot < 0 writes nothing.  What differs: the
-// rotated queries go to `q_out` and qkv stays as it was (every block of rows reads its neighbours' keys for their page's
+// rotated queries go to `q_out`, which may not lie in qkv, and qkv stays as it was (every block of rows reads its neighbours' keys for their page's
 // largest value, so nothing may be turned in place), and the cache takes round_e4m3(x / s) with x the rotated key in 32
 // bits (not rounded to the model's type first) or the value, and s the page's scale for that kv head:
 //   s = the least power of two under which the rows fit, and, unless one of the rows is the page's first, not below the
@@ -114,8 +114,9 @@ __global__ void kv_write_q8_kernel(const WriteArgs a) {
 //   sides until the first and the last run end: their largest values then are every block's that shares a run, no block waits for
 //   another, and all compute the same scale (the scale that a page had is a lower bound: reading it after the run's first
 //   block has put the new one there gives the same).  The run's first block brings the page's other rows to a larger scale.
-// What bounds it: a few tokens the chain of loads (slots and rows, then the scale: two trips), thousands the bytes of qkv once and of the
-// outputs, at 64 tokens a block the rows read twice come out of L1 or L2.
+// What bounds it: a few tokens the chain of loads (slots and rows, then the scale: two trips; 1 token of 12 heads over 2 3.4 us in a graph, 64 of
+// 28 over 4 5.1), thousands the bytes of qkv once and of the outputs (7,543 tokens of 28 over 4 34 us, 4.1 TB/s of those), the rows
+// read twice coming out of L1 or L2.
 constexpr int FAST_THREADS = 128, SPAN_MAX = 64;
 
 struct FastArgs {
@@ -438,6 +439,11 @@ TS_API int ts_rope_kv_write_q8(const void* record, void* stream) {
   if (k_cache != nullptr && (v_cache == nullptr || k_scale == nullptr || v_scale == nullptr || slots == nullptr))
     TS_REFUSE(TS_ERR_SHAPE, "ts_rope_kv_write_q8: keys without values, scales or slots");
   if (dtype != TS_F32 && dtype != TS_BF16) TS_REFUSE(TS_ERR_DTYPE, "ts_rope_kv_write_q8: dtype %d", dtype);
+  // (turned queries over keys or halves that others still read)
+  const size_t elem = dtype == TS_F32 ? 4 : 2;
+  const char *const q0 = (const char*)q_out, *const q1 = q0 + ((size_t)(T - 1) * q_stride + (size_t)H * D) * elem;
+  if (q_stride < 0 || (q0 < (const char*)qkv + (size_t)T * (H + 2 * KVH) * D * elem && (const char*)qkv < q1))
+    TS_REFUSE(TS_ERR_SHAPE, "ts_rope_kv_write_q8: the queries' rows lie in qkv");
   WriteArgs a = {qkv, q_out, q_stride, positions, cos_t, sin_t, {(unsigned char*)k_cache, (unsigned char*)v_cache},
                  {k_scale, v_scale}, slots, T, H, KVH, D, rot, page};
   cudaStream_t s = (cudaStream_t)stream;

@@ -10,8 +10,8 @@
 // One block a request (several where tables are wide or portions long), which sums the lengths before its own, puts its row's updates in
 // place and writes its tokens and its table rows; one more block puts the others in place, of rows that are not in the step.
 // Only the update that holds in the end is ever written, so blocks that write the same place write the same value.  One launch
-// whatever the step: 8 requests of 2,048 tokens are bound by its latency (2.0 us in a graph, of which a launch is most); 129 requests
-// with two tables of 2,048 entries and a portion of 1,920 tokens move 3 MB.  The kernel does not let kernels behind it start early: they
+// whatever the step: 8 requests of 2,048 tokens are bound by its latency (2.2 us in a graph, of which a launch is most); 129 requests
+// with two tables of 2,048 entries and a portion of 1,920 tokens move 3 MB (4.9 us).  The kernel does not let kernels behind it start early: they
 // may read the maps before they wait.
 #include "common.cuh"
 

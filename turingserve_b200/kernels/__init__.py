@@ -724,14 +724,15 @@ class CudaOps:
             raise ValueError(f"{what}: contiguous pages [n, {KVH}, {page_size}, {D}] with scales [n, {KVH}], not {tuple(k_cache.shape)}, "
                              f"{tuple(v_cache.shape)} with {tuple(k_scale.shape)}, {tuple(v_scale.shape)}")
         if not k_cache.get_device() == v_cache.get_device() == k_scale.get_device() == v_scale.get_device() == device:
-            raise ValueError(f"{what}: pages and scales must be on the tokens' device")
+            raise ValueError(f"{what}: pages and scales must be on GPU {device}, whose kernels these are")
 
     def rope_kv_write_q8(self, q_out, qkv, positions, cos, sin, H: int, KVH: int, D: int, rotary_dim: int, k_cache, v_cache,
                          k_scale, v_scale, slots, page_size: int) -> None:
         """q_out [T, H D] = the rotated queries of ``qkv`` [T, (H + 2 KVH) D]; the rotated keys and the values go to pages of
         8 bits (float8_e4m3fn [pages, KVH, page, D], scales float32 [pages, KVH]: a power of two per page and kv head,
-        from 2^-50 to 2^50, NaN for a page with a value that is not finite or above 448 * 2^50).  ``qkv`` stays as it is (it may
-        be a product that is not finished: the kernel sums it, and finished it is written nowhere).  A page's scale grows with what is written to it, its other rows are brought to the new one; a call that writes the page's
+        from 2^-50 to 2^50, NaN for a page with a value that is not finite or above 448 * 2^50).  ``qkv`` stays as it is (``q_out``
+        may not lie in it; it may be a product that is not finished: the kernel sums it, and finished it is written nowhere).  A
+        page's scale grows with what is written to it, its other rows are brought to the new one; a call that writes the page's
         first row begins the page anew.  The rows of one page stand next to each other among the tokens that are written and no slot
         appears twice.  ``k_cache`` None: queries only; ``slots`` -1: that token is not written."""
         finished, part, splits, bias = isinstance(qkv, torch.Tensor), None, 0, None
@@ -743,6 +744,7 @@ class CudaOps:
                              f"{qkv.dtype} to {tuple(q_out.shape)} {q_out.dtype}")
         if positions.dtype is not i32 or positions.shape != (T,) or not positions.is_contiguous():
             raise ValueError("rope_kv_write_q8: an int32 position for each token")
+        gpu = self._device_index
         if rotary_dim:
             half = rotary_dim // 2
             if rotary_dim < 0 or rotary_dim > D or rotary_dim % 2:
@@ -750,10 +752,12 @@ class CudaOps:
             if (cos is None or sin is None or cos.dtype is not torch.float32 or sin.dtype is not torch.float32 or cos.shape[-1] != half
                     or sin.shape[-1] != half or not (cos.is_contiguous() and sin.is_contiguous())):
                 raise ValueError(f"rope_kv_write_q8: float32 tables [positions, {half}]")
+            if not cos.get_device() == sin.get_device() == gpu:
+                raise ValueError(f"rope_kv_write_q8: all tensors must be on GPU {gpu}, whose kernels these are")
         if k_cache is not None:
-            self._check_q8_cache("rope_kv_write_q8", k_cache, v_cache, k_scale, v_scale, KVH, D, page_size, q_out.get_device())
-            if slots is None or slots.dtype is not i32 or slots.shape != (T,) or not slots.is_contiguous():
-                raise ValueError("rope_kv_write_q8: an int32 slot for each token")
+            self._check_q8_cache("rope_kv_write_q8", k_cache, v_cache, k_scale, v_scale, KVH, D, page_size, gpu)
+            if slots is None or slots.dtype is not i32 or slots.shape != (T,) or not slots.is_contiguous() or slots.get_device() != gpu:
+                raise ValueError(f"rope_kv_write_q8: an int32 slot for each token, on GPU {gpu}")
         if not finished and isinstance(qkv, Deferred):
             if (self.lib.ts_rope_kv_write_q8_takes_parts(D, rotary_dim, code) and q_out.stride(0) % 8 == 0
                     and all(t is None or t.data_ptr() % 16 == 0 for t in (q_out, cos, sin, k_cache, v_cache, qkv.part))):
@@ -763,6 +767,8 @@ class CudaOps:
                 qkv = self.materialize(qkv)
         if not qkv.is_contiguous() or q_out.stride(1) != 1:
             raise ValueError("rope_kv_write_q8: rows must be contiguous")
+        if not q_out.get_device() == qkv.get_device() == positions.get_device() == gpu:
+            raise ValueError(f"rope_kv_write_q8: all tensors must be on GPU {gpu}, whose kernels these are")
         pages = (0,) * 5
         if k_cache is not None:
             pages = (k_cache.data_ptr(), v_cache.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr(), slots.data_ptr())
@@ -803,7 +809,10 @@ class CudaOps:
             raise ValueError("attention_q8: rows of contiguous heads, float32 or bfloat16, outputs [T, H D] in the queries' type")
         if block_tables.dtype is not torch.int32 or not block_tables.is_contiguous() or block_tables.shape[0] < B:
             raise ValueError("attention_q8: an int32 block table for each request, rows contiguous")
-        self._check_q8_cache("attention_q8", k_cache, v_cache, k_scale, v_scale, KVH, D, page_size, q.get_device())
+        gpu = self._device_index
+        if not q.get_device() == out.get_device() == block_tables.get_device() == gpu:
+            raise ValueError(f"attention_q8: all tensors must be on GPU {gpu}, whose kernels these are")
+        self._check_q8_cache("attention_q8", k_cache, v_cache, k_scale, v_scale, KVH, D, page_size, gpu)
         w = int(window) if window else 0
         if w < 0:
             raise ValueError(f"attention_q8: a window of {w} keys")
@@ -847,8 +856,8 @@ class CudaOps:
         the pages of every request, kept on the GPU; ``updates`` [U, 4]: (group, row, index, page) put into the tables first (of
         updates of one place the last holds).  Written: ``q_start`` [B + 1], ``seq_lens`` [B], ``token_request`` and
         ``positions`` [T], ``slot_mapping`` [groups, T] (-1 for padding), ``block_tables`` [groups, B, width] (0 behind a
-        request's last page); the groups of the last two may lie any distance apart.  Kernels that read their step's arrays before they wait (``attention``) may not follow without a copy
-        or an event between."""
+        request's last page); the groups of the last two may lie any distance apart.  Kernels that read their step's arrays before
+        they wait (``attention``) may not follow without a copy or an event between."""
         i32 = torch.int32
         if tables.dim() != 3 or page_size < 1 or not tables.is_contiguous():
             raise ValueError("step_maps: contiguous tables [groups, rows, pages] of pages of a token or more")
@@ -867,6 +876,10 @@ class CudaOps:
         t_g, t_b, t_w = block_tables.stride()
         if (s_t != 1 and T > 1) or (t_w != 1 and W > 1) or (t_b != W and B > 1):
             raise ValueError("step_maps: each group's slots and block tables are contiguous")
+        if not (requests.get_device() == updates.get_device() == tables.get_device() == q_start.get_device() == seq_lens.get_device()
+                == token_request.get_device() == positions.get_device() == slot_mapping.get_device() == block_tables.get_device()
+                == self._device_index):
+            raise ValueError(f"step_maps: all tensors must be on GPU {self._device_index}, whose kernels these are")
         self._check(self.lib.ts_step_maps(_MAPS.pack(
             requests.data_ptr(), updates.data_ptr(), tables.data_ptr(), q_start.data_ptr(), seq_lens.data_ptr(), token_request.data_ptr(),
             positions.data_ptr(), slot_mapping.data_ptr(), block_tables.data_ptr(), s_g, t_g, B, T, U, G, R, P, W, page_size),
