@@ -409,8 +409,9 @@ def test_scales_over_the_whole_range(ops, case):
 @pytest.fixture
 def forced(ops):
     """Sets the instance of the portions' kernel and the splits of the single tokens'; the rules hold again afterwards."""
-    def force(row_tiles=0, splits=0, clusters=True):
+    def force(row_tiles=0, splits=0, clusters=True, portion_splits=0):
         ops.lib.ts_set_q8_prefill(row_tiles)
+        ops.lib.ts_set_q8_prefill_splits(portion_splits)
         ops.q8_splits, ops.q8_clusters = splits, clusters
     yield force
     force()
@@ -421,11 +422,41 @@ def forced(ops):
                                                                             ([400], [400], 34, 2, 64, 48, 0)],
                          ids=lambda c: f"{len(c[0])}x{max(c[0])}of{max(c[1])}-{c[4]}-w{c[6]}")
 def test_one_and_two_row_tiles(ops, forced, case, row_tiles):
-    forced(row_tiles=row_tiles)
+    forced(row_tiles=row_tiles, portion_splits=1)
     for std in (1.0, 4.0):
         a = Attend(*case, std=std)
         a.run(ops)
         a.check()
+
+
+@pytest.mark.parametrize("splits", [2, 4, 8])
+@pytest.mark.parametrize("case", [c for c in ATTENDS if max(c[0]) > 1] + [([513, 2, 700], [1025, 2, 5000], 12, 2, 128, 16, 0),
+                                                                            ([400], [400], 34, 2, 64, 48, 0), ([3, 2, 9], [3000, 2, 1100], 4, 1, 128, 64, 700)],
+                         ids=lambda c: f"{len(c[0])}x{max(c[0])}of{max(c[1])}-{c[4]}-w{c[6]}")
+def test_portions_cut_over_blocks(ops, forced, case, splits):
+    forced(row_tiles=1, portion_splits=splits)
+    for std in (1.0, 4.0):
+        a = Attend(*case, std=std)
+        a.run(ops)
+        a.check()
+
+
+@pytest.mark.parametrize("splits", [2, 8])
+def test_a_portion_cut_over_blocks_sees_nan_where_it_does(ops, forced, splits):
+    """Shares whose keys are all NaN, none, or some, against one block for all of them: NaN in the same rows, the same values elsewhere.
+    (Either is off by 2^-8 of the output, and by weights of 2^-11 and sums in 32 bits, below 2^-10 of the largest value together.)"""
+    for poisoned in ([0], [7], list(range(3, 12)), list(range(25))):
+        outs = []
+        for n in (1, splits):
+            forced(row_tiles=1, portion_splits=n)
+            a = Attend([700], [1600], 6, 2, 128, 64, 500)
+            a.ks[a.tables[0][poisoned].long()] = math.nan
+            a.run(ops)
+            outs.append(a.out.float())
+        assert torch.equal(outs[0].isnan(), outs[1].isnan())
+        off = (outs[0] - outs[1]).nan_to_num().abs()
+        top = float((a.v.float() * a.vs[..., None, None]).abs().max())
+        assert float(off.max()) <= 2 * (2.0 ** -8 * float(outs[0].nan_to_num().abs().max()) + 2.0 ** -10 * top)
 
 
 @pytest.mark.parametrize("splits,clusters", [(1, False), (2, True), (3, False), (5, True), (8, True), (8, False), (29, False), (128, False)])

@@ -16,7 +16,8 @@
 // the rows: MN-major).  Rows outside the visible range are zeros.
 // NR = 2: a score buffer each, so that the softmax of one row tile runs beside the products of the other; a converted tile serves 256 rows;
 // tensor memory is full and a block fills an SM.  NR = 1, for launches of few row tiles, which are as slow as their longest block: two score
-// buffers, products two turns ahead.
+// buffers, products two turns ahead; where there are fewer row tiles than half the SMs, a cluster of 2 to 8 blocks cuts the keys of one among
+// itself, and every block finishes some of the rows out of its peers' shared memory.
 // The reference M moves only when a row's maximum has grown by more than 2^8 since: then O is rescaled in tensor memory.  Every wait is
 // bounded; a block that gives up records where, stops, and frees its tensor memory.
 //
@@ -30,7 +31,7 @@ namespace {
 
 using namespace tc;
 
-constexpr int TQ = 128, TK = 128, STAGES = 2, SCALE_STAGES = 4;
+constexpr int TQ = 128, TK = 128, STAGES = 2, SCALE_STAGES = 4, MAX_SPLITS = 8;
 constexpr float RESCALE_STEP = 8.f;
 constexpr float LOG2E_P = 1.4426950408889634f;
 
@@ -48,6 +49,8 @@ struct Shape {
   // 16 rows of keys or of values are a converter's job; so many jobs of its are on their way from the pages
   static constexpr int AHEAD = 2;
   static constexpr uint32_t JOB_BYTES = 16 * HD;
+  static constexpr int O_ROW = HD + 4;                             // floats of a row's sums in shared memory, over the tiles
+  static_assert(NR == 2 || (TQ * O_ROW + 2 * TQ) * 4 <= NR * Q_BYTES + 2 * STAGES * KV_BYTES, "sums and references over the tiles");
   static constexpr size_t TILES = NR * Q_BYTES + 2 * STAGES * KV_BYTES + CONV_WARPS * AHEAD * JOB_BYTES;
   // behind the tiles: scales [4][8] float4, scales on their way [converters][AHEAD][2], barriers, the tensor memory's address, the abort flag
   static constexpr size_t SMEM = TILES + SCALE_STAGES * (TK / 16) * 16 + CONV_WARPS * AHEAD * 8 + BARS * 8 + 16;
@@ -65,7 +68,7 @@ struct PreArgs {
   const int* seq_lens;
   int table_width, H, KVH, page;
   float scale;
-  int window;
+  int window, nsplit;
   int* status;
 };
 
@@ -109,6 +112,52 @@ __device__ __forceinline__ float max3(float x, float y, float z) {
   return r;
 }
 
+// Block `share` of a cluster of NS finishes rows share * TQ / NS .. of their row tile: 128 threads, four columns each, the sums of every
+// block out of its shared memory, in the order of the shares.  (Eight loads of a thread on their way at a time: one piece at a time
+// cost 5 us more.)
+template <int HD, int NS>
+__device__ __forceinline__ void merge_shares(const PreArgs& a, const unsigned char* smem, int tid, int share, int rows, int qs, int row0, int kvh,
+                                             int G) {
+  constexpr int O_ROW = Shape<HD, 1>::O_ROW, PB = MAX_SPLITS / NS, CPR = HD / 4, FIRST_ROWS = TQ / CPR;
+  const float* o_s = reinterpret_cast<const float*>(smem);
+  const float* m_s = o_s + TQ * O_ROW;
+  const int d = tid % CPR * 4;
+  for (int r0 = share * (TQ / NS) + tid / CPR; r0 < (share + 1) * (TQ / NS) && r0 < rows; r0 += FIRST_ROWS * PB) {
+    float m1[PB][NS], l1[PB][NS];
+    float4 x[PB][NS];
+#pragma unroll
+    for (int p = 0; p < PB; ++p)
+#pragma unroll
+      for (int i = 0; i < NS; ++i) {
+        const int r = r0 + p * FIRST_ROWS;
+        m1[p][i] = ld_peer_f32(peer_shared(m_s + r, i));
+        l1[p][i] = ld_peer_f32(peer_shared(m_s + TQ + r, i));
+        x[p][i] = ld_peer_v4(peer_shared(o_s + r * O_ROW + d, i));
+      }
+#pragma unroll
+    for (int p = 0; p < PB; ++p) {
+      const int r = r0 + p * FIRST_ROWS, row = row0 + r;
+      float M = -INFINITY, L = 0.f;
+      float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+      for (int i = 0; i < NS; ++i) M = fmaxf(M, m1[p][i]);
+#pragma unroll
+      for (int i = 0; i < NS; ++i) {
+        // (no reference: the share saw nothing, and weighs nothing, or NaN alone)
+        const float f = m1[p][i] == -INFINITY ? l1[p][i] : ex2(m1[p][i] - M);
+        L = fmaf(l1[p][i], f, L);
+        acc.x = fmaf(x[p][i].x, f, acc.x);
+        acc.y = fmaf(x[p][i].y, f, acc.y);
+        acc.z = fmaf(x[p][i].z, f, acc.z);
+        acc.w = fmaf(x[p][i].w, f, acc.w);
+      }
+      const float inv = L > 0.f ? 1.f / L : L;                     // nothing seen: 0; NaN stays
+      bf16* dst = a.out + (size_t)(qs + row / G) * a.o_ts + (size_t)(kvh * G + row % G) * HD + d;
+      if (r < rows) *reinterpret_cast<uint2*>(dst) = make_uint2(pack_bf16(acc.x * inv, acc.y * inv), pack_bf16(acc.z * inv, acc.w * inv));
+    }
+  }
+}
+
 template <int HD, int NR>
 __global__ void __launch_bounds__(Shape<HD, NR>::THREADS, 1) attention_q8_prefill_kernel(const PreArgs a) {
   using SH = Shape<HD, NR>;
@@ -134,6 +183,7 @@ __global__ void __launch_bounds__(Shape<HD, NR>::THREADS, 1) attention_q8_prefil
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bar_q + 1);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
 
+  const int nsplit = NR == 1 ? a.nsplit : 1, share = blockIdx.x % nsplit, block_row = blockIdx.x / nsplit;
   const int b = blockIdx.z, kvh = blockIdx.y, G = a.H / a.KVH;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   if ((smem_u32(smem) & 1023u) != 0) {                             // the swizzled tiles need 1024-byte alignment
@@ -143,8 +193,8 @@ __global__ void __launch_bounds__(Shape<HD, NR>::THREADS, 1) attention_q8_prefil
   pdl_wait();                                                      // what it reads is written by kernels before
   const int qs = a.q_start[b], q_len = a.q_start[b + 1] - qs, seq_len = a.seq_lens[b];
   const int n_rows = q_len * G, n_blocks = (n_rows + ROWS - 1) / ROWS;
-  if ((int)blockIdx.x >= n_blocks) return;
-  const int row0 = (n_blocks - 1 - blockIdx.x) * ROWS;             // longest blocks first
+  if (block_row >= n_blocks) return;                               // (the whole cluster)
+  const int row0 = (n_blocks - 1 - block_row) * ROWS;              // longest blocks first
   const int prefix = seq_len - q_len;
   if (tid == 0) {
     for (int s = 0; s < STAGES; ++s) {
@@ -175,10 +225,13 @@ __global__ void __launch_bounds__(Shape<HD, NR>::THREADS, 1) attention_q8_prefil
   const uint32_t tmem = *tmem_slot;
 
   const int last_row = min(row0 + ROWS, n_rows) - 1;
-  const int j_hi = prefix + last_row / G;                          // the last key that any row sees, and the first
+  const int key_hi = prefix + last_row / G;                        // the last key that any row sees, and the first
   const int key_lo = a.window > 0 ? max(0, prefix + row0 / G - a.window + 1) : 0;
-  const int j_lo = key_lo & ~15;
-  const int n_tiles = (seq_len > 0 && j_hi >= key_lo) ? (j_hi - j_lo) / TK + 1 : 0;
+  const int all_tiles = (seq_len > 0 && key_hi >= key_lo) ? (key_hi - (key_lo & ~15)) / TK + 1 : 0;
+  // this block's turns of them
+  const int first_tile = (int)((long long)all_tiles * share / nsplit);
+  const int n_tiles = (int)((long long)all_tiles * (share + 1) / nsplit) - first_tile;
+  const int j_lo = (key_lo & ~15) + first_tile * TK, j_hi = min(key_hi, j_lo + n_tiles * TK - 1);
 
   const int rt = warp >> 2, lane_row = tid & (TQ - 1);             // a softmax thread's row tile and row
   const bool softmax = warp < SH::SOFT_WARPS;
@@ -360,7 +413,27 @@ __global__ void __launch_bounds__(Shape<HD, NR>::THREADS, 1) attention_q8_prefil
       ok = mbar_wait(&bar_o[rt], 0, a.status, 25, abort_flag);
       ok = __all_sync(0xffffffffu, ok);
     }
-    if (ok) {
+    if (ok && nsplit > 1) {
+      // the row's sums, for whichever block of the cluster finishes it: over the tiles, which nobody reads any more
+      tc_fence_after();
+      float* dst = reinterpret_cast<float*>(smem) + lane_row * SH::O_ROW;
+#pragma unroll 1
+      for (int c = 0; c < HD; c += 32) {
+        uint32_t ov[32];
+        if (n_tiles > 0) {
+          tmem_ld32(lane_addr + O_COL + c, ov);
+          tmem_wait_ld();
+        } else {
+#pragma unroll
+          for (int i = 0; i < 32; ++i) ov[i] = 0u;
+        }
+#pragma unroll
+        for (int i = 0; i < 32; i += 4) *reinterpret_cast<uint4*>(dst + c + i) = make_uint4(ov[i], ov[i + 1], ov[i + 2], ov[i + 3]);
+      }
+      dst = reinterpret_cast<float*>(smem) + TQ * SH::O_ROW + lane_row;
+      dst[0] = m_ref;
+      dst[TQ] = l_run;
+    } else if (ok) {
       tc_fence_after();
       bf16* dst = a.out + (size_t)(qs + tok) * a.o_ts + (size_t)(kvh * G + g) * HD;
       const float inv = l_run > 0.f ? 1.f / l_run : l_run;         // nothing seen: 0; NaN stays
@@ -528,13 +601,24 @@ __global__ void __launch_bounds__(Shape<HD, NR>::THREADS, 1) attention_q8_prefil
         }
     }
   }
+  if (NR == 1 && nsplit > 1) {
+    // Block `share` finishes its share of the rows out of its peers' shared memory, in the order of the shares.
+    cluster_sync_all();
+    if (softmax) {
+      const int rows_here = n_rows - row0;
+      if (nsplit == 2) merge_shares<HD, 2>(a, smem, tid, share, rows_here, qs, row0, kvh, G);
+      else if (nsplit == 4) merge_shares<HD, 4>(a, smem, tid, share, rows_here, qs, row0, kvh, G);
+      else merge_shares<HD, 8>(a, smem, tid, share, rows_here, qs, row0, kvh, G);
+    }
+    cluster_sync_all();                                            // no block leaves while a peer still reads it
+  }
   tc_fence_before();
   __syncthreads();
   if (warp == SH::MMA_WARP)
     asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(SH::TMEM_COLS) : "memory");
 }
 
-int g_row_tiles = 0;
+int g_row_tiles = 0, g_splits = 0;
 
 template <int HD, int NR>
 cudaError_t launch(const PreArgs& a, int B, int max_q_len, cudaStream_t s) {
@@ -550,8 +634,36 @@ cudaError_t launch(const PreArgs& a, int B, int max_q_len, cudaStream_t s) {
     return cudaFuncSetAttribute(attention_q8_prefill_kernel<HD, NR>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)SH::SMEM);
   }();
   if (configured != cudaSuccess) return configured;
-  const dim3 grid(ceil_div(max_q_len * (a.H / a.KVH), NR * TQ), a.KVH, B);
-  return ts_launch(attention_q8_prefill_kernel<HD, NR>, grid, dim3(SH::THREADS), SH::SMEM, s, a);
+  const dim3 grid(ceil_div(max_q_len * (a.H / a.KVH), NR * TQ) * a.nsplit, a.KVH, B);
+  return ts_launch_cluster(attention_q8_prefill_kernel<HD, NR>, dim3(a.nsplit, 1, 1), grid, dim3(SH::THREADS), SH::SMEM, s, a);
+}
+
+// How many clusters of n blocks of one row tile the chip holds at once (0: none).
+template <int HD>
+int clusters_that_fit(int n) {
+  static int known[MAX_SPLITS + 1];
+  int& k = known[n];
+  if (k == 0) {
+    using SH = Shape<HD, 1>;
+    k = -1;
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(n, 1, 1);
+    cfg.blockDim = dim3(SH::THREADS);
+    cfg.dynamicSmemBytes = SH::SMEM;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim.x = (unsigned)n;
+    attr[0].val.clusterDim.y = 1;
+    attr[0].val.clusterDim.z = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    int clusters = 0;
+    if (cudaFuncSetAttribute(attention_q8_prefill_kernel<HD, 1>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)SH::SMEM) == cudaSuccess &&
+        cudaOccupancyMaxActiveClusters(&clusters, attention_q8_prefill_kernel<HD, 1>, &cfg) == cudaSuccess && clusters >= 1)
+      k = clusters;
+    cudaGetLastError();                                            // a refusal is an answer, not an error
+  }
+  return k < 0 ? 0 : k;
 }
 
 // About how many times the longest block's time a launch of n blocks takes, whose lengths fall evenly from 1 to `least`: the work over the
@@ -568,7 +680,9 @@ double launch_time(long long n, double least) {
 
 }  // namespace
 
-TS_API void ts_set_q8_prefill(int row_tiles) { g_row_tiles = row_tiles == 1 || row_tiles == 2 ? row_tiles : 0; }   // for measurements
+// For measurements: row tiles a block (1, 2), and blocks that cut its keys (1, 2, 4, 8, with one row tile); 0: by the rule.
+TS_API void ts_set_q8_prefill(int row_tiles) { g_row_tiles = row_tiles == 1 || row_tiles == 2 ? row_tiles : 0; }
+TS_API void ts_set_q8_prefill_splits(int splits) { g_splits = splits == 1 || splits == 2 || splits == 4 || splits == 8 ? splits : 0; }
 
 // Requests of any number of tokens (rows q_start[b] ..).  q, out: rows [H, D] q_ts / o_ts elements apart.
 TS_API int ts_attention_q8_prefill(const void* record, void* stream) {
@@ -586,19 +700,35 @@ TS_API int ts_attention_q8_prefill(const void* record, void* stream) {
     TS_REFUSE(TS_ERR_UNSUPPORTED, "ts_attention_q8_prefill: pages and rows of queries and outputs on 16 bytes");
   int* status = ts_attn_status_word();
   if (status == nullptr) TS_REFUSE(TS_ERR_LIMIT, "ts_attention_q8_prefill: no status word");
-  const PreArgs a = {(bf16*)out, o_ts, (const bf16*)q, q_ts, {(const unsigned char*)k_cache, (const unsigned char*)v_cache},
-                     {c.k_scale, c.v_scale}, c.block_tables, c.q_start, c.seq_lens, c.table_width, H, KVH, page, c.scale, window, status};
+  PreArgs a = {(bf16*)out, o_ts, (const bf16*)q, q_ts, {(const unsigned char*)k_cache, (const unsigned char*)v_cache},
+               {c.k_scale, c.v_scale}, c.block_tables, c.q_start, c.seq_lens, c.table_width, H, KVH, page, c.scale, window, 1, status};
   cudaStream_t s = (cudaStream_t)stream;
   // Two row tiles a block or one: a turn of 128 keys takes a block of two 1.64 times as long (4,750 against 2,900 cycles), so it is two where half
   // the blocks more than make up for that (us, one / two: 28 heads over 4, 4,096 tokens 194 / 169, 2,048 63 / 71, 1,024 30 / 32, 2,048 behind
   // 4,000 225 / 215; 40 over 8, 512 behind 4,000 109 / 98; 12 over 2, 2,048 31 / 49).
+  // A cluster of 2, 4 or 8 blocks of one row tile where all of them run at once and the turns that a block is spared are worth the merge (8,600
+  // cycles) and beat both: a block more for an SM costs it 10 us and more, however short (us, one / 2 / 4 / 8: 12 heads over 2, 64 tokens
+  // behind 2,000, 6 row tiles, 32 / 24 / 18 / 15; behind 16,000 186 / 102 / 58 / 34; 512 behind 4,000, 48 row tiles, 60 / 39 / 48 / 68; 512 alone
+  // 13.4 / 14.1 / 24 / 48; 1,024 alone, 96 row tiles, 19 / 27 / 39 / 84).
   const int rows = max_q_len * (H / KVH);
   const double reach = max_seq_len < 1 ? 1 : max_seq_len, sees = window > 0 && window < reach ? window : reach;
   const double before = max_q_len < reach ? reach - max_q_len : 0, least = (before < sees ? before : sees) / sees;
-  const bool two = g_row_tiles ? g_row_tiles == 2
-                               : launch_time((long long)ceil_div(rows, 2 * TQ) * KVH * B, least) * 1.64 < launch_time((long long)ceil_div(rows, TQ) * KVH * B, least);
-  const cudaError_t e = D == 64 ? (two ? launch<64, 2>(a, B, max_q_len, s) : launch<64, 1>(a, B, max_q_len, s))
-                                : (two ? launch<128, 2>(a, B, max_q_len, s) : launch<128, 1>(a, B, max_q_len, s));
+  const double longest = (sees / TK + 1) * 2900;
+  const long long row_tiles = (long long)ceil_div(rows, TQ) * KVH * B;
+  const double t_one = launch_time(row_tiles, least), t_two = launch_time((long long)ceil_div(rows, 2 * TQ) * KVH * B, least) * 1.64;
+  const bool two = g_row_tiles ? g_row_tiles == 2 : t_two < t_one;
+  if (g_splits && !two) a.nsplit = g_splits;
+  else if (!g_splits && g_row_tiles != 2 && ts_clusters_enabled()) {
+    double best = (two ? t_two : t_one) * longest;
+    for (int n = 2; n <= MAX_SPLITS && row_tiles * n <= ts_sm_count(); n *= 2)
+      if (longest / n + 8600 < best && row_tiles <= (D == 64 ? clusters_that_fit<64>(n) : clusters_that_fit<128>(n))) {
+        best = longest / n + 8600;
+        a.nsplit = n;
+      }
+  }
+  const bool pair = two && a.nsplit == 1;
+  const cudaError_t e = D == 64 ? (pair ? launch<64, 2>(a, B, max_q_len, s) : launch<64, 1>(a, B, max_q_len, s))
+                                : (pair ? launch<128, 2>(a, B, max_q_len, s) : launch<128, 1>(a, B, max_q_len, s));
   if (e != cudaSuccess) TS_REFUSE((int)e, "ts_attention_q8_prefill: %s", cudaGetErrorString(e));
   TS_LAUNCH_CHECK();
 }

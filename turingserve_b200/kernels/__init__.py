@@ -193,8 +193,9 @@ class CudaOps:
         for name, record in (("rope_kv_write_q8", _WRITE_Q8), ("attention_q8", _ATTEND_Q8), ("step_maps", _MAPS)):
             if getattr(self.lib, f"ts_{name}_record")() != record.size:
                 raise KernelError(f"{lib_path}: {name} takes another record than this package's {record.size} bytes")
-        self.lib.ts_set_q8_prefill.argtypes = [I]
-        self.lib.ts_set_q8_prefill.restype = None
+        for name in ("ts_set_q8_prefill", "ts_set_q8_prefill_splits"):
+            getattr(self.lib, name).argtypes = [I]
+            getattr(self.lib, name).restype = None
         self.lib.ts_attention_diff_mma_supported.argtypes = [I, I, I, I, I]
         self.lib.ts_attention_diff_mma_supported.restype = c_int
         self.lib.ts_attention_diff_mma_scratch_floats.argtypes = [I, I, I, I]
