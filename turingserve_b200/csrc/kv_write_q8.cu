@@ -117,7 +117,7 @@ __global__ void kv_write_q8_kernel(const WriteArgs a) {
 // What bounds it: a few tokens the chain of loads (slots and rows, then the scale: two trips; 1 token of 12 heads over 2 3.4 us in a graph, 64 of
 // 28 over 4 5.1), thousands the bytes of qkv once and of the outputs (7,543 tokens of 28 over 4 34 us, 4.1 TB/s of those), the rows
 // read twice coming out of L1 or L2.
-constexpr int FAST_THREADS = 128, SPAN_MAX = 64;
+constexpr int FAST_THREADS = 128, SPAN_MAX = 64, HEADS = 2;
 
 struct FastArgs {
   WriteArgs w;
@@ -129,17 +129,19 @@ struct FastArgs {
 
 // 16 values of a row: 8 at column c1 and 8 at c2 of token t's row of qkv, summed over the splits where it is not finished, and then
 // rounded as the product's own end would have rounded them
+__device__ __forceinline__ void widen16(const uint4& u, const uint4& v, float (&x)[16]) {
+  const unsigned w[8] = {u.x, u.y, u.z, u.w, v.x, v.y, v.z, v.w};
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    x[2 * i] = __uint_as_float(w[i] << 16);
+    x[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
+  }
+}
 template <bool PART>
 __device__ __forceinline__ void load16(const FastArgs& a, int t, int row_elems, int c1, int c2, float (&x)[16]) {
   if constexpr (!PART) {
     const bf16* r = (const bf16*)a.w.qkv + (size_t)t * row_elems;
-    const uint4 u = *reinterpret_cast<const uint4*>(r + c1), v = *reinterpret_cast<const uint4*>(r + c2);
-    const unsigned w[8] = {u.x, u.y, u.z, u.w, v.x, v.y, v.z, v.w};
-#pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      x[2 * i] = __uint_as_float(w[i] << 16);
-      x[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
-    }
+    widen16(*reinterpret_cast<const uint4*>(r + c1), *reinterpret_cast<const uint4*>(r + c2), x);
   } else {
 #pragma unroll
     for (int i = 0; i < 16; ++i) x[i] = 0.f;
@@ -163,8 +165,8 @@ __device__ __forceinline__ void load16(const FastArgs& a, int t, int row_elems, 
     }
   }
 }
-__device__ __forceinline__ void load_table(const WriteArgs& a, int t, int half, int j, float (&c)[8], float (&s)[8]) {
-  const size_t at = (size_t)a.positions[t] * half + 8 * j;
+__device__ __forceinline__ void load_table(const WriteArgs& a, int position, int half, int j, float (&c)[8], float (&s)[8]) {
+  const size_t at = (size_t)position * half + 8 * j;
 #pragma unroll
   for (int i = 0; i < 8; i += 4) {
     const float4 u = *reinterpret_cast<const float4*>(a.cos_t + at + i), v = *reinterpret_cast<const float4*>(a.sin_t + at + i);
@@ -197,24 +199,46 @@ __global__ void __launch_bounds__(FAST_THREADS) kv_write_q8_fast_kernel(const Fa
   if ((int)blockIdx.y >= f.kv_blocks) {
     const int h0 = (blockIdx.y - f.kv_blocks) * f.q_heads, h1 = min(a.H, h0 + f.q_heads);
     const int rows = min(f.span, ROWS), abreast = ROWS / rows;
+    auto position_of = [&](int t) { return a.rot && t < w1 ? a.positions[t] : 0; };
+    int position = position_of(w0 + r % rows);
     for (int t = w0 + r % rows; t < w1; t += rows) {
+      const int next = position_of(t + rows);
       float c[8], s[8];
-      if (a.rot) load_table(a, t, HALF, j, c, s);
       bf16* dst = (bf16*)a.q_out + (size_t)t * a.q_stride;
-#pragma unroll 2
-      for (int h = h0 + r / rows; h < h1; h += abreast) {
-        float x[16];
-        load16<PART>(f, t, row_elems, h * D + 8 * j, h * D + HALF + 8 * j, x);
-        if (a.rot) turn(x, c, s);
-        unsigned w[8];
+      const bf16* src = (const bf16*)a.qkv + (size_t)t * row_elems;
+      bool first = true;
+      // two heads' rows on their way at a time, and the table's: no load can pass a store of unknown address by itself
+      for (int h = h0 + r / rows; h < h1; h += HEADS * abreast) {
+        uint4 u[HEADS], v[HEADS];
+        if (!PART) {
 #pragma unroll
-        for (int i = 0; i < 8; ++i) {
-          const __nv_bfloat162 p = __floats2bfloat162_rn(x[2 * i], x[2 * i + 1]);
-          w[i] = *reinterpret_cast<const unsigned*>(&p);
+          for (int k = 0; k < HEADS; ++k) {
+            const int hk = min(h + k * abreast, h1 - 1);
+            u[k] = *reinterpret_cast<const uint4*>(src + hk * D + 8 * j);
+            v[k] = *reinterpret_cast<const uint4*>(src + hk * D + HALF + 8 * j);
+          }
         }
-        *reinterpret_cast<uint4*>(dst + h * D + 8 * j) = make_uint4(w[0], w[1], w[2], w[3]);
-        *reinterpret_cast<uint4*>(dst + h * D + HALF + 8 * j) = make_uint4(w[4], w[5], w[6], w[7]);
+        if (first && a.rot) load_table(a, position, HALF, j, c, s);
+        first = false;
+#pragma unroll
+        for (int k = 0; k < HEADS; ++k) {
+          const int hk = h + k * abreast;
+          if (hk >= h1) break;
+          float x[16];
+          if (PART) load16<PART>(f, t, row_elems, hk * D + 8 * j, hk * D + HALF + 8 * j, x);
+          else widen16(u[k], v[k], x);
+          if (a.rot) turn(x, c, s);
+          unsigned w[8];
+#pragma unroll
+          for (int i = 0; i < 8; ++i) {
+            const __nv_bfloat162 p = __floats2bfloat162_rn(x[2 * i], x[2 * i + 1]);
+            w[i] = *reinterpret_cast<const unsigned*>(&p);
+          }
+          *reinterpret_cast<uint4*>(dst + hk * D + 8 * j) = make_uint4(w[0], w[1], w[2], w[3]);
+          *reinterpret_cast<uint4*>(dst + hk * D + HALF + 8 * j) = make_uint4(w[4], w[5], w[6], w[7]);
+        }
       }
+      position = next;
     }
     return;
   }
@@ -227,7 +251,7 @@ __global__ void __launch_bounds__(FAST_THREADS) kv_write_q8_fast_kernel(const Fa
     load16<PART>(f, t, row_elems, col, col + HALF, x);
     if (kv == 0 && a.rot) {
       float c[8], s[8];
-      load_table(a, t, HALF, j, c, s);
+      load_table(a, a.positions[t], HALF, j, c, s);
       turn(x, c, s);
     }
   };
