@@ -115,9 +115,9 @@ __global__ void kv_write_q8_kernel(const WriteArgs a) {
 //   another, and all compute the same scale (the scale that a page had is a lower bound: reading it after the run's first
 //   block has put the new one there gives the same).  The run's first block brings the page's other rows to a larger scale.
 // What bounds it: a few tokens the chain of loads (slots and rows, then the scale: two trips; 1 token of 12 heads over 2 3.4 us in a graph, 64 of
-// 28 over 4 5.1), thousands the bytes of qkv once and of the outputs (7,543 tokens of 28 over 4 34 us, 4.1 TB/s of those), the rows
+// 28 over 4 5.1), thousands the bytes of qkv once and of the outputs (7,543 tokens of 28 over 4 31 us, 4.5 TB/s of those), the rows
 // read twice coming out of L1 or L2.
-constexpr int FAST_THREADS = 128, SPAN_MAX = 64, HEADS = 2;
+constexpr int SPAN_MAX = 64, HEADS = 2;
 
 struct FastArgs {
   WriteArgs w;
@@ -188,11 +188,11 @@ __device__ __forceinline__ unsigned four_e4m3(float a, float b, float c, float d
   return lo | hi << 16;
 }
 
-template <int D, bool PART>
-__global__ void __launch_bounds__(FAST_THREADS) kv_write_q8_fast_kernel(const FastArgs f) {
+template <int D, int THREADS, bool PART>
+__global__ void __launch_bounds__(THREADS) kv_write_q8_fast_kernel(const FastArgs f) {
   pdl_launch_dependents();
   pdl_wait();
-  constexpr int LPR = D / 16, ROWS = FAST_THREADS / LPR, HALF = D / 2;
+  constexpr int LPR = D / 16, ROWS = THREADS / LPR, HALF = D / 2;
   const WriteArgs& a = f.w;
   const int tid = threadIdx.x, j = tid % LPR, r = tid / LPR, row_elems = (a.H + 2 * a.KVH) * D;
   const int w0 = blockIdx.x * f.span, w1 = min(a.T, w0 + f.span);
@@ -400,23 +400,33 @@ __global__ void __launch_bounds__(FAST_THREADS) kv_write_q8_fast_kernel(const Fa
   if (tid < n_runs && begins_here(tid)) a.scale[kv][(size_t)(slot_s[lead_s[tid]] / a.page) * a.KVH + kvh] = now_s[tid];
 }
 
-template <int D>
-cudaError_t launch_fast(FastArgs f, cudaStream_t s) {
+template <int D, int THREADS>
+cudaError_t launch_fast(FastArgs f, int span, cudaStream_t s) {
   const WriteArgs& a = f.w;
-  constexpr int ROWS = FAST_THREADS / (D / 16);
-  // Spans of as many tokens as a block takes in one turn (no slower than a token a block: its rows lie side by side in the block's warps), wider
-  // where there are blocks enough: every block of a page's rows reads all of them.  (us at spans of 16 / 32 / 64: 1,999 tokens, 28 heads
-  // over 4, 17.7 / 17.8 / 20.2; 7,543 tokens 48 / 38 / 34; 8,000 tokens, 40 over 8, 81 / 60 / 51)
-  f.span = a.T <= 8 ? 1 : (a.T <= 1024 ? ROWS : (a.T <= 4096 ? 32 : SPAN_MAX));
+  constexpr int ROWS = THREADS / (D / 16);
+  f.span = span;
   f.kv_blocks = a.cache[0] != nullptr ? 2 * a.KVH : 0;
   // query heads a block (they share a table row's conversion): as many as keep 4,096 lanes an SM, at least one row of lanes each (7,543 tokens, 2 / 4
-  // / 7 / 14 heads 34 / 35 / 40 / 52 us)
+  // / 7 / 14 heads 31 / 31 / 36 / 43 us)
   const int least = f.span < ROWS ? ROWS / f.span : 1;
   const long long lanes = (long long)a.T * (D / 16) * a.H, want = lanes / ((long long)ts_sm_count() * 4096);
   f.q_heads = (int)(want < least ? least : (want > a.H ? a.H : want));
-  const dim3 grid(ceil_div(a.T, f.span), f.kv_blocks + ceil_div(a.H, f.q_heads)), block(FAST_THREADS);
-  return f.part != nullptr ? ts_launch(kv_write_q8_fast_kernel<D, true>, grid, block, 0, s, f)
-                           : ts_launch(kv_write_q8_fast_kernel<D, false>, grid, block, 0, s, f);
+  const dim3 grid(ceil_div(a.T, f.span), f.kv_blocks + ceil_div(a.H, f.q_heads)), block(THREADS);
+  return f.part != nullptr ? ts_launch(kv_write_q8_fast_kernel<D, THREADS, true>, grid, block, 0, s, f)
+                           : ts_launch(kv_write_q8_fast_kernel<D, THREADS, false>, grid, block, 0, s, f);
+}
+// Threads a block and tokens a block.  Every block of a page's rows reads all of them, in turns of as many rows as its threads hold: of 256 threads
+// it takes half as long (us at 128 / 256, spans of 16: a portion of 200 tokens, 28 heads over 4, 12.6 / 8.6, of 700 14.1 / 9.8; 64 single
+// tokens in pages of 16 5.2 / 5.0), and wider spans read them in fewer blocks (256 threads, spans of 16 / 32 / 64: 1,999 tokens 19.2 / 14.7
+// / 13.6, 1,000 10.5 / 10.5 / 10.9; 64 single tokens 5.0 / 6.2 / 10.8).  Where the work is many times what the chip holds smaller blocks fill it better (spans of
+// 64, 128 / 256: 4,096 tokens 22.6 / 23.9, with 12 heads over 2 20.6 / 13.5; 5,500 24.6 / 27.0; 7,543 31.0 / 35.6); a few tokens want a block
+// each (8 single tokens, 128 threads, spans of 1 / 16: 3.8 / 4.2).
+template <int D>
+cudaError_t launch_fast(const FastArgs& f, cudaStream_t s) {
+  const int T = f.w.T;
+  if (T <= 8) return launch_fast<D, 128>(f, 1, s);
+  if (T <= 4096) return launch_fast<D, 256>(f, T <= 1024 ? 16 : SPAN_MAX, s);
+  return launch_fast<D, 128>(f, SPAN_MAX, s);
 }
 
 }  // namespace
