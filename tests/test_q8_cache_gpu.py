@@ -75,6 +75,9 @@ WRITES = [
     ([19], [3], 4, 4, 64, 0, 16, BF16),                      # no rotation: the values are exact
     ([1, 21], [30, 3], 6, 2, 128, 128, 16, torch.float32),
     ([700], [100], 40, 8, 128, 128, 64, BF16),
+    ([1, 1, 1100, 190], [64, 300, 37, 1], 6, 2, 64, 64, 48, BF16),       # wider spans
+    ([1300], [7], 7, 1, 128, 128, 256, BF16),
+    ([1, 2500, 1650], [5, 61, 0], 4, 1, 128, 128, 16, BF16),             # and smaller blocks
 ]
 
 

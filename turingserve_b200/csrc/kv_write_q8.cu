@@ -115,7 +115,7 @@ __global__ void kv_write_q8_kernel(const WriteArgs a) {
 //   another, and all compute the same scale (the scale that a page had is a lower bound: reading it after the run's first
 //   block has put the new one there gives the same).  The run's first block brings the page's other rows to a larger scale.
 // What bounds it: a few tokens the chain of loads (slots and rows, then the scale: two trips; 1 token of 12 heads over 2 3.4 us in a graph, 64 of
-// 28 over 4 5.1), thousands the bytes of qkv once and of the outputs (7,543 tokens of 28 over 4 31 us, 4.5 TB/s of those), the rows
+// 28 over 4 5.1), thousands the bytes of qkv once and of the outputs (7,787 tokens of 28 over 4 31 us, 4.5 TB/s of those), the rows
 // read twice coming out of L1 or L2.
 constexpr int SPAN_MAX = 64, HEADS = 2;
 
@@ -406,7 +406,7 @@ cudaError_t launch_fast(FastArgs f, int span, cudaStream_t s) {
   constexpr int ROWS = THREADS / (D / 16);
   f.span = span;
   f.kv_blocks = a.cache[0] != nullptr ? 2 * a.KVH : 0;
-  // query heads a block (they share a table row's conversion): as many as keep 4,096 lanes an SM, at least one row of lanes each (7,543 tokens, 2 / 4
+  // query heads a block (they share a table row's conversion): as many as keep 4,096 lanes an SM, at least one row of lanes each (7,787 tokens, 2 / 4
   // / 7 / 14 heads 31 / 31 / 36 / 43 us)
   const int least = f.span < ROWS ? ROWS / f.span : 1;
   const long long lanes = (long long)a.T * (D / 16) * a.H, want = lanes / ((long long)ts_sm_count() * 4096);
@@ -419,7 +419,7 @@ cudaError_t launch_fast(FastArgs f, int span, cudaStream_t s) {
 // it takes half as long (us at 128 / 256, spans of 16: a portion of 200 tokens, 28 heads over 4, 12.6 / 8.6, of 700 14.1 / 9.8; 64 single
 // tokens in pages of 16 5.2 / 5.0), and wider spans read them in fewer blocks (256 threads, spans of 16 / 32 / 64: 1,999 tokens 19.2 / 14.7
 // / 13.6, 1,000 10.5 / 10.5 / 10.9; 64 single tokens 5.0 / 6.2 / 10.8).  Where the work is many times what the chip holds smaller blocks fill it better (spans of
-// 64, 128 / 256: 4,096 tokens 22.6 / 23.9, with 12 heads over 2 20.6 / 13.5; 5,500 24.6 / 27.0; 7,543 31.0 / 35.6); a few tokens want a block
+// 64, 128 / 256: 4,096 tokens 22.6 / 23.9, with 12 heads over 2 20.6 / 13.5; 5,500 24.6 / 27.0; 7,787 31.0 / 35.6); a few tokens want a block
 // each (8 single tokens, 128 threads, spans of 1 / 16: 3.8 / 4.2).
 template <int D>
 cudaError_t launch_fast(const FastArgs& f, cudaStream_t s) {
