@@ -1,0 +1,39 @@
+"""The 8-bit cache's operators where a block, a warp or a call has nothing of its own to do, and what else the widest use of them meets."""
+
+import math
+
+import pytest
+import torch
+
+from tests.test_q8_cache_gpu import BF16, Attend, forced, ops  # noqa: F401
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.mark.parametrize("splits", [0, 2, 4, 8])
+@pytest.mark.parametrize("H,KVH,D", [(12, 2, 128), (14, 2, 64), (5, 5, 128)])
+def test_queries_of_nan_beside_shares_without_keys(ops, forced, H, KVH, D, splits):  # noqa: F811
+    """Short prompts beside a long context, keys cut over 2, 4 and 8 blocks (0: by the rule, which goes by the longest): most blocks of a short
+    prompt's row tiles have no keys.  Queries with NaN in every odd column, in the last rows of a tile and in its first: their own rows are NaN,
+    every other row has the bits that it has beside clean queries."""
+    a = Attend([40, 130, 17, 1, 64, 33], [40, 130, 17, 1, 4000, 33], H, KVH, D, 16)
+    a.step.num_decode = 0
+    G, odd = H // KVH, torch.zeros(a.q.shape[0], H, dtype=torch.bool, device=a.q.device)
+    start = 0
+    for n in a.q_lens:
+        for row in range(n * G):                                   # (a row tile is 128 (token, head-in-group) pairs)
+            if row % 128 >= 120 or row % 128 < 3:
+                odd[start + row // G, row % G] = True
+        start += n
+    forced(row_tiles=1 if splits else 0, portion_splits=splits)
+    clean = a.run(ops).clone().view(a.q.shape)
+    a.check()
+    q = a.q.clone()
+    a.q[..., 1::2][odd] = math.nan
+    for _ in range(20):
+        a.out.fill_(7.0)
+        got = a.run(ops).view(a.q.shape)
+        assert got[odd].isnan().all()
+        assert torch.equal(got[~odd], clean[~odd])
+    a.q = q
+    assert torch.equal(a.run(ops).view(a.q.shape), clean)

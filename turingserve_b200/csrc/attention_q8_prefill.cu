@@ -414,7 +414,10 @@ __global__ void __launch_bounds__(Shape<HD, NR>::THREADS, 1) attention_q8_prefil
       ok = __all_sync(0xffffffffu, ok);
     }
     if (ok && nsplit > 1) {
-      // the row's sums, for whichever block of the cluster finishes it: over the tiles, which nobody reads any more
+      // The row's sums, for whichever block of the cluster finishes it: over the tiles, which nobody reads any more, and which all rows have
+      // written: the last product has seen every query, and in a share without turns, where there is no product, the rows meet here.
+      // (A query stored late would lie in another row's sums, and a NaN in it counts even at no weight.)
+      if (n_tiles == 0) asm volatile("bar.sync 1, %0;" ::"n"(TQ) : "memory");
       tc_fence_after();
       float* dst = reinterpret_cast<float*>(smem) + lane_row * SH::O_ROW;
 #pragma unroll 1
