@@ -1,0 +1,37 @@
+"""More of what the operators of the 8-bit cache and of the step's maps refuse, and how their front chooses, without a GPU."""
+
+from types import SimpleNamespace
+
+import pytest
+import torch
+
+from tests.test_q8_cache_cpu import I32, attend_args, ops  # noqa: F401
+
+
+def step(**other):
+    a = dict(num_requests=3, num_decode=3, q_start=torch.arange(4, dtype=I32), seq_lens=torch.ones(3, dtype=I32), max_q_len=1, max_seq_len=1)
+    a.update(other)
+    return SimpleNamespace(**a)
+
+
+@pytest.mark.parametrize("other", [
+    dict(q_start=torch.arange(4)), dict(q_start=torch.arange(4.0)), dict(q_start=torch.arange(3, dtype=I32)),
+    dict(q_start=torch.arange(8, dtype=I32)[::2]), dict(q_start=torch.zeros(4, 1, dtype=I32)),
+    dict(seq_lens=torch.ones(3, dtype=torch.int64)), dict(seq_lens=torch.ones(2, dtype=I32)), dict(seq_lens=torch.ones(6, dtype=I32)[::2]),
+    dict(seq_lens=torch.ones(1, 3, dtype=I32)), dict(num_decode=4), dict(num_decode=-1),
+], ids=lambda o: "-".join(f"{k}{tuple(v.shape)}{v.dtype}" if isinstance(v, torch.Tensor) else f"{k}{v}" for k, v in o.items()))
+def test_attention_refuses_a_step_that_does_not_fit(ops, other):  # noqa: F811
+    with pytest.raises(ValueError, match="query starts"):
+        ops.attention_q8(**attend_args(step=step(**other)))
+
+
+class Elsewhere(torch.Tensor):
+    def get_device(self):
+        return 1
+
+
+@pytest.mark.parametrize("which", ["q_start", "seq_lens"])
+def test_attention_refuses_a_step_of_another_device(ops, which):  # noqa: F811
+    """Everything on the kernels' device (the CPU's number here) but one of the step's arrays."""
+    with pytest.raises(ValueError, match="must be on GPU"):
+        ops.attention_q8(**attend_args(step=step(**{which: getattr(step(), which).as_subclass(Elsewhere)})))

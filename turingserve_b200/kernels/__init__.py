@@ -808,10 +808,15 @@ class CudaOps:
         o_ts, one = out.stride()
         if one != 1:
             raise ValueError("attention_q8: rows of contiguous heads, float32 or bfloat16, outputs [T, H D] in the queries' type")
-        if block_tables.dtype is not torch.int32 or not block_tables.is_contiguous() or block_tables.shape[0] < B:
+        i32, q_start, seq_lens = torch.int32, step.q_start, step.seq_lens
+        if block_tables.dtype is not i32 or not block_tables.is_contiguous() or block_tables.dim() != 2 or block_tables.shape[0] < B:
             raise ValueError("attention_q8: an int32 block table for each request, rows contiguous")
+        if (q_start.dtype is not i32 or seq_lens.dtype is not i32 or q_start.dim() != 1 or seq_lens.dim() != 1 or q_start.shape[0] <= B
+                or seq_lens.shape[0] < B or not (q_start.is_contiguous() and seq_lens.is_contiguous()) or not 0 <= step.num_decode <= B):
+            raise ValueError(f"attention_q8: {B} requests want {B + 1} contiguous int32 query starts, {B} lengths and at most as many single "
+                             f"tokens, not {tuple(q_start.shape)} {q_start.dtype}, {tuple(seq_lens.shape)} {seq_lens.dtype}, {step.num_decode}")
         gpu = self._device_index
-        if not q.get_device() == out.get_device() == block_tables.get_device() == gpu:
+        if not q.get_device() == out.get_device() == block_tables.get_device() == q_start.get_device() == seq_lens.get_device() == gpu:
             raise ValueError(f"attention_q8: all tensors must be on GPU {gpu}, whose kernels these are")
         self._check_q8_cache("attention_q8", k_cache, v_cache, k_scale, v_scale, KVH, D, page_size, gpu)
         w = int(window) if window else 0
@@ -819,7 +824,7 @@ class CudaOps:
             raise ValueError(f"attention_q8: a window of {w} keys")
         G, nd, width, stream, max_seq = H // KVH, 0, block_tables.shape[1], self._stream(), step.max_seq_len
         rows = (out.data_ptr(), q.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr())
-        tables, q_start, seq_lens = block_tables.data_ptr(), step.q_start.data_ptr(), step.seq_lens.data_ptr()
+        tables, q_start, seq_lens = block_tables.data_ptr(), q_start.data_ptr(), seq_lens.data_ptr()
         sizes = (H, KVH, D, page_size, k_cache.shape[0], w, code)
         fast = self.use_fast_attention and code == 1 and (D == 128 or D == 64)
         if fast and G <= 16 and step.num_decode:
