@@ -5,7 +5,7 @@ import math
 import pytest
 import torch
 
-from tests.test_q8_cache_gpu import BF16, Attend, forced, ops  # noqa: F401
+from tests.test_q8_cache_gpu import BF16, Attend, Write, forced, ops  # noqa: F401
 
 pytestmark = pytest.mark.gpu
 
@@ -37,3 +37,17 @@ def test_queries_of_nan_beside_shares_without_keys(ops, forced, H, KVH, D, split
         assert torch.equal(got[~odd], clean[~odd])
     a.q = q
     assert torch.equal(a.run(ops).view(a.q.shape), clean)
+
+
+@pytest.mark.parametrize("slot", [-2, -3, -(1 << 31)])
+@pytest.mark.parametrize("case", [([200], [5], 4, 2, 64, 64, 256, BF16), ([1300], [7], 4, 2, 128, 128, 256, BF16), ([1, 5], [9, 3], 4, 2, 64, 64, 16, BF16),
+                                  ([40, 9], [5, 0], 3, 1, 80, 80, 64, BF16)], ids=lambda c: f"{len(c[0])}x{max(c[0])}-{c[4]}")
+def test_any_negative_slot_is_a_token_that_is_not_written(ops, case, slot):  # noqa: F811
+    """Tokens without a place in the middle of pages, at the edges of spans of 1, 16 and 64 tokens among them: the page's other rows are one
+    run all the same, with one scale."""
+    w = Write(*case)
+    for t in (1, 2, 14, 15, 16, 31, 47, 48, 63, 64, 100, 127, 128, 191, 640, 895):
+        if t < w.slots.shape[0] - 1:
+            w.slots[t] = slot
+    w.run(ops)
+    w.check()

@@ -259,11 +259,12 @@ __global__ void __launch_bounds__(THREADS) kv_write_q8_fast_kernel(const FastArg
   // the span's rows, if it is no more of them than the block takes in one turn.
   const bool back = tid < 32;
   int around[4];
+  auto neighbour = [&](int t) { return t >= 0 && t < a.T ? max(a.slots[t], -1) : -2; };         // (-2: no token there; -1: one that is not written)
   if (tid < 64) {
 #pragma unroll
     for (int u = 0; u < 4; ++u) {
       const int t = back ? w0 - 1 - (u * 32 + lane) : w1 + u * 32 + lane;
-      around[u] = t >= 0 && t < a.T ? a.slots[t] : -2;
+      around[u] = neighbour(t);
     }
   }
   if (tid < SPAN_MAX) {
@@ -322,7 +323,7 @@ __global__ void __launch_bounds__(THREADS) kv_write_q8_fast_kernel(const FastArg
 #pragma unroll
       for (int u = 0; u < 4; ++u) {
         const int t = back ? at - (u * 32 + lane) : at + u * 32 + lane;
-        around[u] = t >= 0 && t < a.T ? a.slots[t] : -2;
+        around[u] = neighbour(t);
       }
     }
     if (lane == 0) edge_s[back ? 0 : 1] = edge;

@@ -735,7 +735,7 @@ class CudaOps:
         may not lie in it; it may be a product that is not finished: the kernel sums it, and finished it is written nowhere).  A
         page's scale grows with what is written to it, its other rows are brought to the new one; a call that writes the page's
         first row begins the page anew.  The rows of one page stand next to each other among the tokens that are written and no slot
-        appears twice.  ``k_cache`` None: queries only; ``slots`` -1: that token is not written."""
+        appears twice.  ``k_cache`` None: queries only; a negative slot: that token is not written."""
         finished, part, splits, bias = isinstance(qkv, torch.Tensor), None, 0, None
         if not finished:
             qkv = self._settle(qkv)
