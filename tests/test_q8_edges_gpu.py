@@ -51,3 +51,20 @@ def test_any_negative_slot_is_a_token_that_is_not_written(ops, case, slot):  # n
             w.slots[t] = slot
     w.run(ops)
     w.check()
+
+
+@pytest.mark.parametrize("n", [0, 3, 600])
+def test_maps_of_a_step_without_requests(ops, n):  # noqa: F811
+    """The page tables take what is to go into them, the query starts begin at 0, tokens that no request brings have no place."""
+    i32 = torch.int32
+    tables = torch.randint(1, 999, (2, 5, 9), dtype=i32, device="cuda")
+    g = torch.Generator().manual_seed(n)
+    updates = torch.stack([torch.randint(0, m, (n,), generator=g) for m in (2, 5, 9, 5000)], 1).int()
+    want = tables.clone().cpu()
+    for a, b, c, p in updates.tolist():
+        want[a, b, c] = p
+    new = lambda *s: torch.full(s, -77, dtype=i32, device="cuda")  # noqa: E731
+    out = [new(1), new(0), new(4), new(4), new(2, 4), new(2, 0, 9)]
+    ops.step_maps(new(3, 0), updates.cuda(), tables, 16, *out)
+    assert torch.equal(tables.cpu(), want)
+    assert out[0].tolist() == [0] and not out[2].any() and not out[3].any() and out[4].eq(-1).all()

@@ -163,9 +163,8 @@ TS_API int ts_step_maps_record() { return (int)sizeof(MapCall); }
 TS_API int ts_step_maps(const void* record, void* stream) {
   const MapCall& c = *(const MapCall*)record;
   const int B = c.B, T = c.T, U = c.U, G = c.G, R = c.R, P = c.P, W = c.W, page = c.page;
-  if (B <= 0) return 0;
-  if (T < 0 || U < 0 || G < 0 || R <= 0 || P <= 0 || W < 0 || page <= 0)
-    TS_REFUSE(TS_ERR_SHAPE, "ts_step_maps: T=%d U=%d G=%d R=%d P=%d W=%d page=%d", T, U, G, R, P, W, page);
+  if (B < 0 || T < 0 || U < 0 || G < 0 || R <= 0 || P <= 0 || W < 0 || page <= 0)
+    TS_REFUSE(TS_ERR_SHAPE, "ts_step_maps: B=%d T=%d U=%d G=%d R=%d P=%d W=%d page=%d", B, T, U, G, R, P, W, page);
   if (((uintptr_t)c.updates & 15) != 0) TS_REFUSE(TS_ERR_ALIGN, "ts_step_maps: updates must be 16-byte aligned");
   MapArgs a = {c.requests, (const int4*)c.updates, c.tables, c.q_start, c.seq_lens, c.token_request, c.positions, c.slots, c.block_tables,
                c.slots_g, c.tables_g, B, T, U, G, R, P, W, page};
