@@ -185,7 +185,8 @@ class StepInputBuilder:
                 sample.append(row_of[i] + w_)
         S = len(sample)
 
-        if self.tables is not None and B >= self.device_map_rows:
+        # (a request of more pages than the GPU's tables have columns: from the host, if its arena holds the step)
+        if self.tables is not None and B >= self.device_map_rows and max(widths) <= self.max_pages:
             return self._build_on_device(rows_e, q_lens, starts, num_decode, max(widths), sample, arena)
         host_t = self._host[self._turn]
         ev = self._events[self._turn]
