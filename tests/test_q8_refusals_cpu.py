@@ -35,3 +35,26 @@ def test_attention_refuses_a_step_of_another_device(ops, which):  # noqa: F811
     """Everything on the kernels' device (the CPU's number here) but one of the step's arrays."""
     with pytest.raises(ValueError, match="must be on GPU"):
         ops.attention_q8(**attend_args(step=step(**{which: getattr(step(), which).as_subclass(Elsewhere)})))
+
+
+def test_portions_where_the_device_does_not_hold_a_block_are_left_to_the_kernel_for_any_sizes():
+    """The tensor cores' kernel answers "not taken by this kernel", upon which the front calls the other one: on a machine without a GPU it
+    cannot be configured."""
+    import ctypes
+    import os
+
+    from turingserve_b200 import kernels
+    from turingserve_b200.kernels import _ATTEND_Q8, CudaOps
+
+    if torch.cuda.is_available():
+        pytest.skip("this machine's GPU holds the kernel")
+    path = os.path.join(os.path.dirname(kernels.__file__), "libturingserve_b200.so")
+    if not os.path.exists(path):
+        pytest.skip("the library is not built")
+    lib = ctypes.CDLL(path)
+    lib.ts_attention_q8_prefill.argtypes = [ctypes.c_char_p, ctypes.c_void_p]
+    for D in (64, 128):
+        page = torch.zeros(64 * 128 * 2, dtype=torch.uint8)
+        at = page.data_ptr() // 16 * 16 + 16
+        record = _ATTEND_Q8.pack(*(at,) * 6, at, at, at, 0, D, D, 1, 1, 16, 16, 1, 1, D, 16, 1, 0, 1, 1, 0, 0, 0.1)
+        assert lib.ts_attention_q8_prefill(record, None) == CudaOps.UNSUPPORTED

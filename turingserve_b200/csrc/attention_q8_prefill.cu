@@ -623,20 +623,26 @@ __global__ void __launch_bounds__(Shape<HD, NR>::THREADS, 1) attention_q8_prefil
 
 int g_row_tiles = 0, g_splits = 0;
 
+// Whether the device holds a block of the instance.
 template <int HD, int NR>
-cudaError_t launch(const PreArgs& a, int B, int max_q_len, cudaStream_t s) {
+bool prepare_kernel() {
   using SH = Shape<HD, NR>;
   constexpr int SOFT = SH::SOFT_WARPS * 32;
   static_assert(SOFT * SH::SOFT_REGS + (SH::THREADS - SOFT) * SH::OTHER_REGS <= SH::THREADS * 128, "more registers than the block has");
-  static const cudaError_t configured = [] {
+  static const bool ready = [] {
     // the split of registers counts on 128 a thread at launch: with fewer a warpgroup would wait for what nobody gives
     cudaFuncAttributes attr;
-    const cudaError_t e = cudaFuncGetAttributes(&attr, attention_q8_prefill_kernel<HD, NR>);
-    if (e != cudaSuccess) return e;
-    if (attr.numRegs != 128) return cudaErrorLaunchOutOfResources;
-    return cudaFuncSetAttribute(attention_q8_prefill_kernel<HD, NR>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)SH::SMEM);
+    const bool ok = cudaFuncGetAttributes(&attr, attention_q8_prefill_kernel<HD, NR>) == cudaSuccess && attr.numRegs == 128 &&
+                    cudaFuncSetAttribute(attention_q8_prefill_kernel<HD, NR>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)SH::SMEM) == cudaSuccess;
+    cudaGetLastError();                                            // a refusal is an answer, not an error
+    return ok;
   }();
-  if (configured != cudaSuccess) return configured;
+  return ready;
+}
+
+template <int HD, int NR>
+cudaError_t launch(const PreArgs& a, int B, int max_q_len, cudaStream_t s) {
+  using SH = Shape<HD, NR>;
   const dim3 grid(ceil_div(max_q_len * (a.H / a.KVH), NR * TQ) * a.nsplit, a.KVH, B);
   return ts_launch_cluster(attention_q8_prefill_kernel<HD, NR>, dim3(a.nsplit, 1, 1), grid, dim3(SH::THREADS), SH::SMEM, s, a);
 }
@@ -661,7 +667,7 @@ int clusters_that_fit(int n) {
     cfg.attrs = attr;
     cfg.numAttrs = 1;
     int clusters = 0;
-    if (cudaFuncSetAttribute(attention_q8_prefill_kernel<HD, 1>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)SH::SMEM) == cudaSuccess &&
+    if (prepare_kernel<HD, 1>() &&
         cudaOccupancyMaxActiveClusters(&clusters, attention_q8_prefill_kernel<HD, 1>, &cfg) == cudaSuccess && clusters >= 1)
       k = clusters;
     cudaGetLastError();                                            // a refusal is an answer, not an error
@@ -701,6 +707,8 @@ TS_API int ts_attention_q8_prefill(const void* record, void* stream) {
     TS_REFUSE(TS_ERR_UNSUPPORTED, "ts_attention_q8_prefill: %d requests of up to %d tokens, %d kv heads", B, max_q_len, KVH);
   if ((((uintptr_t)q | (uintptr_t)out | (uintptr_t)k_cache | (uintptr_t)v_cache) & 15) != 0 || (q_ts & 7) != 0 || (o_ts & 7) != 0)
     TS_REFUSE(TS_ERR_UNSUPPORTED, "ts_attention_q8_prefill: pages and rows of queries and outputs on 16 bytes");
+  if (!(D == 64 ? prepare_kernel<64, 1>() && prepare_kernel<64, 2>() : prepare_kernel<128, 1>() && prepare_kernel<128, 2>()))
+    TS_REFUSE(TS_ERR_UNSUPPORTED, "ts_attention_q8_prefill: the device does not hold a block");
   int* status = ts_attn_status_word();
   if (status == nullptr) TS_REFUSE(TS_ERR_LIMIT, "ts_attention_q8_prefill: no status word");
   PreArgs a = {(bf16*)out, o_ts, (const bf16*)q, q_ts, {(const unsigned char*)k_cache, (const unsigned char*)v_cache},
