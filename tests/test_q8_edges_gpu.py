@@ -68,3 +68,19 @@ def test_maps_of_a_step_without_requests(ops, n):  # noqa: F811
     ops.step_maps(new(3, 0), updates.cuda(), tables, 16, *out)
     assert torch.equal(tables.cpu(), want)
     assert out[0].tolist() == [0] and not out[2].any() and not out[3].any() and out[4].eq(-1).all()
+
+
+def test_clusters_switched_off_after_the_first_call(ops):  # noqa: F811
+    a = Attend([1] * 8, [2048 - 37 * i for i in range(8)], 12, 2, 128, 64)
+    launches = []
+    try:
+        for on in (1, 0, 1):
+            ops.lib.ts_set_clusters(on)
+            before = ops.launches
+            a.out.fill_(7.0)
+            a.run(ops)
+            a.check()
+            launches.append(ops.launches - before)
+    finally:
+        ops.lib.ts_set_clusters(1)
+    assert launches == [1, 2, 1]

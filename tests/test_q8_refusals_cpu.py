@@ -58,3 +58,39 @@ def test_portions_where_the_device_does_not_hold_a_block_are_left_to_the_kernel_
         at = page.data_ptr() // 16 * 16 + 16
         record = _ATTEND_Q8.pack(*(at,) * 6, at, at, at, 0, D, D, 1, 1, 16, 16, 1, 1, D, 16, 1, 0, 1, 1, 0, 0, 0.1)
         assert lib.ts_attention_q8_prefill(record, None) == CudaOps.UNSUPPORTED
+
+
+class Recorder:
+    """A library whose single tokens' kernel notes what it is called with; clusters may be switched off behind the front's back."""
+
+    def __init__(self):
+        self.clusters, self.calls = True, []
+
+    def ts_attention_q8_decode_blocks_per_sm(self, G, D):
+        return 2
+
+    def ts_attention_q8_decode_clusters(self, G, D, n):
+        return 100
+
+    def ts_attention_q8_decode(self, record, stream):
+        from turingserve_b200.kernels import _ATTEND_Q8
+        fields = _ATTEND_Q8.unpack(record)
+        scratch, splits, cluster = fields[9], fields[-4], fields[-3]
+        self.calls.append((splits, bool(cluster), scratch != 0))
+        return -4 if cluster and not self.clusters else 0
+
+
+def test_clusters_switched_off_after_the_first_call(ops, monkeypatch):  # noqa: F811
+    """And on again: the choice between a cluster and scratch is the call's, not the first call's."""
+    ops.lib, ops._q8_plans, ops.launches, ops.use_fast_attention = Recorder(), {}, 0, True
+    monkeypatch.setattr(ops, "_stream", lambda: 0, raising=False)
+    args = attend_args(step=step(max_seq_len=600))
+    launches = []
+    for on in (True, False, True):
+        ops.lib.clusters = on
+        before = ops.launches
+        ops.attention_q8(**args)
+        launches.append(ops.launches - before)
+        splits, cluster, scratch = ops.lib.calls[-1]
+        assert splits > 1 and cluster == on and scratch == (not on)
+    assert launches == [1, 2, 1]

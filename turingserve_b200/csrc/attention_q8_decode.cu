@@ -532,9 +532,9 @@ TS_API int ts_attention_q8_decode_blocks_per_sm(int G, int D) {
   return G <= 8 ? prepare_kernel<128, 1, true>() : prepare_kernel<128, 2, true>();
 }
 
-// Clusters of n blocks (2 to 8) that the device holds at once; 0: none.
+// Clusters of n blocks (2 to 8) that the device holds at once, whether or not they are switched on; 0: none.
 TS_API int ts_attention_q8_decode_clusters(int G, int D, int n) {
-  if (n < 2 || n > 8 || !ts_clusters_enabled() || ts_attention_q8_decode_blocks_per_sm(G, D) == 0) return 0;
+  if (n < 2 || n > 8 || ts_attention_q8_decode_blocks_per_sm(G, D) == 0) return 0;
   const int k = D == 64 ? (G <= 8 ? clusters_that_fit<64, 1, true>(n) : clusters_that_fit<64, 2, true>(n))
                         : (G <= 8 ? clusters_that_fit<128, 1, true>(n) : clusters_that_fit<128, 2, true>(n));
   return k < 0 ? 0 : k;
@@ -555,6 +555,7 @@ TS_API int ts_attention_q8_decode(const void* record, void* stream) {
     TS_REFUSE(TS_ERR_UNSUPPORTED, "ts_attention_q8_decode: H=%d KVH=%d D=%d page=%d is not taken by this kernel", H, KVH, D, page);
   if (nsplit < 1 || nsplit > 128 || (cluster && (nsplit < 2 || nsplit > 8)) || (nsplit > 1 && !cluster && scratch == nullptr))
     TS_REFUSE(TS_ERR_LIMIT, "ts_attention_q8_decode: %d splits%s", nsplit, cluster ? " as a cluster" : "");
+  if (cluster && !ts_clusters_enabled()) TS_REFUSE(TS_ERR_UNSUPPORTED, "ts_attention_q8_decode: thread-block clusters are switched off");
   if (B > 65535 || KVH > 65535) TS_REFUSE(TS_ERR_UNSUPPORTED, "ts_attention_q8_decode: %d requests / %d kv heads", B, KVH);
   if ((((uintptr_t)k_cache | (uintptr_t)v_cache | (uintptr_t)scratch) & 15) != 0 || (((uintptr_t)q | (uintptr_t)out) & 7) != 0 ||
       (q_ts & 3) != 0 || (o_ts & 3) != 0)

@@ -830,15 +830,18 @@ class CudaOps:
         if fast and G <= 16 and step.num_decode:
             nd = step.num_decode
             splits, cluster = self._q8_plan(nd * KVH, G, D, min(max_seq, w) if w else max_seq)
-            scratch, at = None, 0
-            if splits > 1 and not cluster:
-                # (of this call's own: calls on two streams, or in two captured graphs, do not meet in it)
-                scratch = torch.empty(nd * H * splits * (D + 2), dtype=torch.float32, device=q.device)
-                at = scratch.data_ptr()
-                self.launches += 1
-            rc = self.lib.ts_attention_q8_decode(_ATTEND_Q8.pack(
-                *rows, tables, q_start, seq_lens, at, o_ts, q_ts, nd, width, 1, max_seq, *sizes, splits, cluster,
-                getattr(step, "settled", False), scale), stream)
+            for as_cluster in ((True, False) if cluster else (False,)):         # (without, where clusters have been switched off)
+                scratch, at = None, 0
+                if splits > 1 and not as_cluster:
+                    # (of this call's own: calls on two streams, or in two captured graphs, do not meet in it)
+                    scratch = torch.empty(nd * H * splits * (D + 2), dtype=torch.float32, device=q.device)
+                    at = scratch.data_ptr()
+                rc = self.lib.ts_attention_q8_decode(_ATTEND_Q8.pack(
+                    *rows, tables, q_start, seq_lens, at, o_ts, q_ts, nd, width, 1, max_seq, *sizes, splits, as_cluster,
+                    getattr(step, "settled", False), scale), stream)
+                if rc != self.UNSUPPORTED:
+                    self.launches += 1 if at else 0                 # (the merge)
+                    break
             if rc == self.UNSUPPORTED:
                 nd = 0
             else:
