@@ -84,3 +84,100 @@ def test_clusters_switched_off_after_the_first_call(ops):  # noqa: F811
     finally:
         ops.lib.ts_set_clusters(1)
     assert launches == [1, 2, 1]
+
+
+# Long contexts.  Values of + and - the same size in the two halves of a context cancel, so that a block's or a warp's share of the keys that got
+# lost, or counted twice, shows as 1 / 128 of them and more.  The bound charges a weight's rounding to a half float as it is: 2^-11 of it, or, where
+# weight * scale lies below 2^-14 of the row's largest, 2^-25 of that largest (a reference below the largest rounds finer); the sums' by the
+# longest chain of additions, a quarter of the keys (four warps a block) and the merges' 140 for single tokens, all of them for portions; scores and
+# exponentials as in test_q8_cache_gpu.py.
+
+def halves_that_cancel(a):
+    """The requests' values: the same size, with the other sign in the second half of what is seen of each context, and some noise."""
+    noise = torch.randn(a.v.shape, generator=torch.Generator(device="cuda").manual_seed(1), device="cuda") * 20
+    v = noise + 150
+    for b, n in enumerate(a.lens):
+        held = -(-n // a.page)
+        first = max(0, n - a.window) // a.page if a.window else 0
+        v[a.tables[b, (first + held) // 2:held].long()] -= 300
+    a.v, a.vs = v.to(a.v.dtype), torch.full_like(a.vs, 2.0 ** -7)
+
+
+def sharp(a, b, chain, leave_out=None):
+    """(outputs of request ``b`` in 64 bits, what each may be off by); ``leave_out``: keys whose weights are dropped."""
+    H, D = a.q.shape[1:]
+    G, n, t = H // a.KVH, a.lens[b], sum(a.q_lens[:b])
+    ids = a.tables[b, :-(-n // a.page)].long()
+    outs, bounds = [], []
+    j, pos = torch.arange(n, device="cuda"), torch.arange(n - a.q_lens[b], n, device="cuda")[:, None]
+    seen = (j <= pos) & ((j > pos - a.window) if a.window else True)
+    for h in range(H):
+        k, v8 = ((x[ids, h // G].double()).flatten(0, 1)[:n] for x in (a.k, a.v))
+        ks, vs = (s[ids, h // G].double().repeat_interleave(a.page)[:n] for s in (a.ks, a.vs))
+        q = a.q[t:t + a.q_lens[b], h].double()
+        s = (q @ (k * ks[:, None]).T * a.scale).masked_fill(~seen, -math.inf)
+        w = torch.softmax(s, -1)
+        if leave_out is not None:
+            w[:, leave_out] = 0
+            w = w / w.sum(-1, keepdim=True)
+        x = w * vs
+        top = x.amax(-1, keepdim=True)
+        off = torch.where(x >= 2.0 ** -14 * top, 2.0 ** -11 * x, torch.where(seen, 2.0 ** -25 * top, torch.zeros_like(top)))
+        size, want = x @ v8.abs(), x @ v8
+        mags = (q.abs() @ (k.abs() * ks[:, None]).T * a.scale).masked_fill(~seen, 0).amax(-1, keepdim=True)
+        outs.append(want)
+        bounds.append(2.0 ** -8 * want.abs() + (2 * (D + 4) * 2.0 ** -24 * mags + 2.0 ** -17 + chain * 2.0 ** -24) * size + off @ v8.abs())
+    return torch.stack(outs, 1), torch.stack(bounds, 1)
+
+
+@pytest.mark.parametrize("splits", [0, 1, 128])
+@pytest.mark.parametrize("case", [([1], [30011], 12, 2, 128, 64, 0), ([1], [100003], 16, 2, 64, 16, 0), ([1] * 3, [8000, 20011, 33], 28, 4, 128, 16, 0),
+                                  ([1], [50000], 12, 2, 128, 64, 16385)], ids=lambda c: f"{len(c[0])}x{max(c[1])}-{c[4]}-w{c[6]}")
+def test_no_share_of_a_long_context_is_lost(ops, forced, case, splits):  # noqa: F811
+    forced(splits=splits, clusters=False if splits > 8 else True)
+    a = Attend(*case)
+    halves_that_cancel(a)
+    got = a.run(ops).double().view(a.q.shape)
+    for b, n in enumerate(a.lens):
+        chain = n / 4 + 140
+        want, bound = sharp(a, b, chain)
+        off = (got[b:b + 1] - want).abs()
+        assert bool((off <= bound).all()), float((off / bound).max())
+        if n < 1000:
+            continue
+        # what is lost without 1 / 128 of the keys that are seen is seen
+        first = max(0, n - a.window) if a.window else 0
+        lost, _ = sharp(a, b, chain, slice(first, first + (n - first) // 128))
+        assert bool(((lost - want).abs() > bound).any(-1).all())
+
+
+@pytest.mark.parametrize("row_tiles,splits", [(0, 0), (1, 1), (2, 1), (1, 2), (1, 4), (1, 8)])
+@pytest.mark.parametrize("case", [([70], [16011], 12, 2, 128, 64, 0), ([1, 40, 90], [5, 9000, 4100], 14, 2, 64, 16, 0),
+                                  ([64], [20000], 6, 2, 128, 16, 8200)], ids=lambda c: f"{len(c[0])}x{max(c[1])}-{c[4]}-w{c[6]}")
+def test_no_share_of_a_portions_long_context_is_lost(ops, forced, case, row_tiles, splits):  # noqa: F811
+    forced(row_tiles=row_tiles, portion_splits=splits)
+    a = Attend(*case)
+    halves_that_cancel(a)
+    got = a.run(ops).double().view(a.q.shape)
+    t = 0
+    for b, n in enumerate(a.lens):
+        want, bound = sharp(a, b, n)
+        off = (got[t:t + a.q_lens[b]] - want).abs()
+        assert bool((off <= bound).all()), float((off / bound).max())
+        if n > 1000:
+            first = max(0, n - a.window) if a.window else 0        # (a turn's 128 keys)
+            lost, _ = sharp(a, b, n, slice(first + 1024, first + 1152))
+            assert bool(((lost - want).abs() > bound).any(-1).all())
+        t += a.q_lens[b]
+
+
+@pytest.mark.parametrize("case", [([1] * 8, [2048 - 37 * i for i in range(8)], 12, 2, 128, 64, 0), ([1, 1, 130, 2], [99, 640, 463, 150], 28, 4, 128, 16, 0),
+                                  ([90, 7], [1500, 20], 14, 2, 64, 32, 70)], ids=["singles", "mixed", "window"])
+@pytest.mark.parametrize("splits,portion_splits", [(1, 1), (4, 2), (8, 8)])
+def test_the_same_bits_whatever_the_longest_context_with_the_same_cuts(ops, forced, case, splits, portion_splits):  # noqa: F811
+    """A captured step is launched for the longest context that the engine allows.  That may change how many blocks cut a request's keys, and so the
+    order of the sums; nothing else."""
+    forced(row_tiles=1, splits=splits, portion_splits=portion_splits)
+    a, b = Attend(*case), Attend(*case, limit=40000)
+    b.tables = torch.cat([b.tables, torch.zeros((b.tables.shape[0], 600), dtype=torch.int32, device="cuda")], 1).contiguous()
+    assert torch.equal(a.run(ops), b.run(ops))
