@@ -3,7 +3,8 @@
 //
 // A scale is 2^e, e the least integer >= -50 with max |x| <= 448 * 2^e over the rows of the page.  Powers of two cost an
 // e4m3 value nothing (it has its own exponent), and a page whose scale has to grow for a new row only moves its rows'
-// exponents: no second rounding but below 2^-6 of the scale's unit, 2^-18 of the page's largest value.  A page with a
+// exponents: what lies below 2^-6 of the new scale is rounded again, each time by at most 2^-10 of that scale, and nothing else
+// is.  (Above the least scale a page's largest value is above 224 scales: below 2^-13.8 of that, by 2^-17.8 of it.)  A page with a
 // value that is not finite, or above 448 * 2^50, has the scale NaN: all that it holds reads as NaN until its first row is
 // written again.  The range of e, 101 steps, is what lets the attention kernels keep one reference for a score and a
 // value's scale together (attention_q8_decode.cu).
