@@ -326,10 +326,14 @@ def run_ours(a) -> dict:
         for rid in list(eng.requests):
             eng.abort(rid)
         eng.step()
-        # per step: the input arena (ids, positions, request index, starts, lengths, slots, rows, slot
-        # map, block tables) goes up (greedy rows need no sampler parameters); tokens and flags come back
-        width = runner.max_pages
-        h2d = 4 * (4 * B + (B + 1) + 3 * B + B * width)
+        # per step: the input arena goes up (greedy rows need no sampler parameters); tokens and flags come back.  Where the
+        # GPU makes the maps: ids, state slots, rows and the two arrays of fed-back tokens, each request's table row and lengths, and
+        # four numbers a page that is begun, every kv_block tokens; else ids, positions, request index, starts, lengths, slots, rows,
+        # slot map, block tables
+        if runner.builder.tables is not None and B >= runner.builder.device_map_rows:
+            h2d = 4 * (5 * B + 3 * B) + 16 * B // a.kv_block
+        else:
+            h2d = 4 * (4 * B + (B + 1) + 3 * B + B * runner.max_pages)
         d2h = (2 * B + ops.STATUS_WORDS) * 4
         e2e = {"value": round(n_tok / e2e_s, 1), "unit": "tok/s", "h2d_bytes_per_step": h2d,
                "d2h_bytes_per_step": d2h, "ms_per_step": round(1e3 * e2e_s / steps, 4)}

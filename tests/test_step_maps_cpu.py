@@ -42,3 +42,13 @@ def test_a_request_of_more_pages_than_the_tables_have_columns(monkeypatch, longe
     table = entries[-1].cache.tables[0]
     assert step.groups[0].slot_mapping[-1] == table[longest // 4] * 4 + longest % 4
     assert step.groups[0].block_tables[-1].tolist() == table
+
+
+@pytest.mark.parametrize("rows,on_gpu", [(1, False), (4, False), (5, False), (6, True), (16, True)])
+def test_steps_of_few_rows_come_from_the_host(monkeypatch, rows, on_gpu):
+    """(a step of one to four requests is no faster with its maps from the GPU; padding rows count)"""
+    _, b, entries = builder_and_steps([5] * max(1, rows - 2), 8)
+    took = []
+    monkeypatch.setattr(b, "_build_on_device", lambda *a, **kw: took.append(True))
+    b.build(entries, pad_requests=rows - len(entries))
+    assert bool(took) == on_gpu

@@ -99,13 +99,17 @@ class StepInputBuilder:
     On a GPU the page tables of all live requests stay there (a row per state slot), and what the arena brings of the maps is each
     request's row, its length and its new tokens' number, with the pages that were added or given back since the request's
     last step: positions, slots and block tables are made from that by one kernel (``ops().step_maps``).  Without a GPU,
-    or without a cache, and for a step of fewer rows than ``device_map_rows``, the host lays them out (a captured step is bound to
-    the layout of its rows' number, so the rule goes by nothing else)."""
+    or without a cache, for a step of fewer rows than ``device_map_rows``, and for one whose block tables are wider than
+    ``max_pages_per_request``, the host lays them out (a captured step is bound to the layout of its rows' number and its tables' fixed width, so
+    the rule goes by nothing else)."""
 
-    # ms a decode step of 8 layers through ``LLMEngine.step``, maps from the host / from the GPU: 1 request 0.303 / 0.306 (0.295 /
-    # 0.303 at 500 tokens), 3 of 2,000 tokens 0.315 / 0.317, 4 in pages of 64 0.324 / 0.324, 8 0.389 / 0.375 (pages of 16 0.427 / 0.379), 64
-    # in pages of 16 1.81 / 1.22, 128 of 4,000 tokens 5.87 / 3.92
-    device_map_rows = 4
+    # ms a decode step through ``LLMEngine.step``, maps from the host / from the GPU (medians of eight runs of 50 steps in turn on one engine, contexts of
+    # 2,048, 12 heads over 2, 28 layers, where the GPU bounds the step and most of the host's work is hidden): pages of 16, 2 requests 1.043 /
+    # 1.047, 3 1.057 / 1.061, 4 1.080 / 1.081, 6 1.110 / 1.105 (the GPU's less in 8 pairs of 8), 8 1.150 / 1.146 (8 of 8), 12 1.295 / 1.292, 16 to 64
+    # within the runs' spread, 128 4.11 / 3.96; pages of 64, 4 1.072 / 1.074 (2 of 8), 6 1.104 / 1.101 (7 of 8), 8 1.148 / 1.143 (8 of 8), 128 3.96 /
+    # 3.95.  Of 8 layers, where the host bounds it: 1 0.303 / 0.306, 4 in pages of 64 0.324 / 0.324, 8 0.389 / 0.375 (pages of 16 0.427 / 0.379), 64 in
+    # pages of 16 1.81 / 1.22, 128 of 4,000 tokens 5.87 / 3.92.
+    device_map_rows = 6
 
     def __init__(self, cache: CacheManager, max_tokens: int, max_requests: int,
                  max_pages_per_request: int, device) -> None:
