@@ -115,8 +115,11 @@ __global__ void kv_write_q8_kernel(const WriteArgs a) {
 //   another, and all compute the same scale (the scale that a page had is a lower bound: reading it after the run's first
 //   block has put the new one there gives the same).  The run's first block brings the page's other rows to a larger scale.
 // What bounds it: a few tokens the chain of loads (slots and rows, then the scale: two trips; 1 token of 12 heads over 2 3.4 us in a graph, 64 of
-// 28 over 4 5.1), thousands the bytes of qkv once and of the outputs (7,787 tokens of 28 over 4 31 us, 4.5 TB/s of those), the rows
-// read twice coming out of L1 or L2.
+// 28 over 4 5.0), thousands the bytes of qkv once and of the outputs (7,787 tokens of 28 over 4 31 us, 4.5 TB/s of those), the rows
+// read twice coming out of L1 or L2.  A decode step of up to 128 tokens brings the product's sums instead (PART): rows of floats, one for each
+// split that `linear` left, read again by every block of a run (us, single tokens in pages of 16, finished / sums: 12 heads over 2, 1 token 3.4 / 3.7, 8
+// 3.6 / 4.0, 16 4.5 / 5.2, 64 of 6 splits 4.9 / 6.4, 128 of 3 5.0 / 6.1; 28 over 4, 64 of 4 5.0 / 6.0, 128 of 4 5.2 / 6.8; 14 over 2 of 64, 64 of 3
+// 4.9 / 5.9), and nothing has to finish the product before it.
 constexpr int SPAN_MAX = 64, HEADS = 2;
 
 struct FastArgs {
@@ -419,9 +422,16 @@ cudaError_t launch_fast(FastArgs f, int span, cudaStream_t s) {
 // Threads a block and tokens a block.  Every block of a page's rows reads all of them, in turns of as many rows as its threads hold: of 256 threads
 // it takes half as long (us at 128 / 256, spans of 16: a portion of 200 tokens, 28 heads over 4, 12.6 / 8.6, of 700 14.1 / 9.8; 64 single
 // tokens in pages of 16 5.2 / 5.0), and wider spans read them in fewer blocks (256 threads, spans of 16 / 32 / 64: 1,999 tokens 19.2 / 14.7
-// / 13.6, 1,000 10.5 / 10.5 / 10.9; 64 single tokens 5.0 / 6.2 / 10.8).  Where the work is many times what the chip holds smaller blocks fill it better (spans of
-// 64, 128 / 256: 4,096 tokens 22.6 / 23.9, with 12 heads over 2 20.6 / 13.5; 5,500 24.6 / 27.0; 7,787 31.0 / 35.6); a few tokens want a block
-// each (8 single tokens, 128 threads, spans of 1 / 16: 3.8 / 4.2).
+// / 13.6, 1,000 10.5 / 10.5 / 10.9; 64 single tokens 5.0 / 6.2 / 10.8).  Where the work is many times what the chip holds smaller blocks fill it better.
+// Spans of 64, 128 / 256 threads, pages of 64:
+//   tokens                 1,500          2,500          4,096          5,500          7,787          8,192
+//   14 over 2 of 64      9.0 /  7.6     9.7 /  7.9    11.7 /  9.0    12.1 / 10.9    13.5 / 14.9    13.7 / 15.5
+//   12 over 2 of 128    14.8 / 10.0    17.0 / 10.9    20.3 / 13.3    20.6 / 15.8    21.8 / 20.8    21.9 / 21.8
+//   28 over 4           19.1 / 12.4    20.5 / 15.7    22.0 / 23.6    24.1 / 26.7    31.8 / 37.1    35.3 / 40.0
+//   40 over 8           20.1 / 15.4    22.1 / 24.3    29.1 / 33.1    38.8 / 43.5    53.3 / 60.4    55.2 / 62.5
+// The border, 4,096 tokens for every model, is a compromise: of few heads it comes too early (12 over 2 of 4,097 tokens get 20.2 where 13.3 is
+// had), of many too late (40 over 8 of 2,500 and 4,096 tokens lose 2 and 4 us).  A few tokens want a block each (8 single tokens, 128 threads, spans
+// of 1 / 16: 3.8 / 4.2).
 template <int D>
 cudaError_t launch_fast(const FastArgs& f, cudaStream_t s) {
   const int T = f.w.T;
